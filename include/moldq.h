@@ -296,6 +296,36 @@ int mq_attention_bf16(const void *q, const void *k, const void *v, int64_t batch
  * it needs none.  With less, or NULL, it runs without. */
 size_t mq_attention_scratch_size(int64_t batch, int heads, int64_t valid);
 
+/* --- Text attention: the layers between a GGUF text model's linears (the text
+ *     encoders of crates/mold-inference/src/encoders and the prompt-expansion
+ *     model of src/expand.rs:200-203, whose attention candle composes of
+ *     matmul, mask and softmax and whose cache grows by concatenation). ------ */
+
+/* How packed prompts of given lengths are attended: made once per batch, used
+ * by every layer with these heads.  mq_prompt_plan_make fills `plan` and, if
+ * `tiles` (host memory) is not NULL, its plan->tiles entries of 4 int32
+ * (capacity counts entries), which the caller copies to the device; called
+ * with tiles NULL it gives the size.  heads a multiple of kv_heads, head_dim 64
+ * or 128, lengths >= 0 (a prompt of no tokens has no rows). */
+typedef struct mq_prompt_plan {
+    int64_t tokens, tiles;
+    int32_t heads, kv_heads, head_dim, tile_tokens, waves;
+} mq_prompt_plan;
+int mq_prompt_plan_make(const int64_t *lengths, int64_t count, int heads, int kv_heads, int head_dim,
+                        mq_prompt_plan *plan, int32_t *tiles, int64_t capacity);
+/* Causal attention inside each prompt of the pack: row i of a prompt attends to
+ * its rows 0 .. i, query head h to k/v head h / (heads / kv_heads);
+ * softmax(scale q . k) v with f32 scores, softmax and sums.  q, out: bf16, token
+ * t and head h at t * token_stride + h * head_stride, unit stride inside a head;
+ * k, v likewise with kv_heads.  16-byte aligned, strides multiples of 8 elements
+ * below 2^24, out apart from q, k and v; tiles: the plan's, on the device.  What
+ * a row does not see does not reach it, infinities and NaN included.
+ * Asynchronous on stream. */
+int mq_prompt_attention(const mq_prompt_plan *plan, const int32_t *tiles, const void *q, int64_t q_token_stride,
+                        int64_t q_head_stride, const void *k, int64_t k_token_stride, int64_t k_head_stride,
+                        const void *v, int64_t v_token_stride, int64_t v_head_stride, float scale, void *out,
+                        int64_t out_token_stride, int64_t out_head_stride, void *stream);
+
 /* Quantize activations once for several Q4_K GEMVs: x [m, k] (F32 or BF16,
  * row stride ldx, 16-byte aligned rows) -> m * k / 256 blocks of
  * MQ_X_Q8K_BLOCK_BYTES at dst (16-byte aligned), by the Q8_K quantization

@@ -25,6 +25,13 @@ class LoraPatchC(ctypes.Structure):
 
 MQ_LORA_MAX_PATCHES = 8
 
+
+class PromptPlanC(ctypes.Structure):
+    """mq_prompt_plan"""
+    _fields_ = [("tokens", ctypes.c_int64), ("tiles", ctypes.c_int64)] + [
+        (f, ctypes.c_int32) for f in ("heads", "kv_heads", "head_dim", "tile_tokens", "waves")]
+
+
 SIGNATURES = {
     "mq_last_error": (ctypes.c_char_p, []),
     "mq_version": (_int, []),
@@ -63,6 +70,10 @@ SIGNATURES = {
     "mq_attention_bf16": (_int, [_vp, _vp, _vp, _i64, _int, _i64, _int, _i64, ctypes.POINTER(_i64), _vp, _i64, _i64, _vp,
                                  _vp, _vp, _sz, _vp]),
     "mq_attention_scratch_size": (_sz, [_i64, _int, _i64]),
+    "mq_prompt_plan_make": (_int, [ctypes.POINTER(_i64), _i64, _int, _int, _int, ctypes.POINTER(PromptPlanC),
+                                   ctypes.POINTER(ctypes.c_int32), _i64]),
+    "mq_prompt_attention": (_int, [ctypes.POINTER(PromptPlanC), _vp] + [_vp, _i64, _i64] * 3 + [ctypes.c_float]
+                            + [_vp, _i64, _i64] + [_vp]),
     "mq_gguf_open": (_int, [ctypes.c_char_p, _pp]),
     "mq_gguf_close": (None, [_vp]),
     "mq_gguf_tensor_count": (_i64, [_vp]),

@@ -42,7 +42,7 @@
 // where the separate correction rounded to bf16 a second time (2.8e-3 ->
 // 2.3e-3).
 #include "../../include/moldq.h"
-#include "mq_kernels.h"
+#include "mq_attn.h"
 
 namespace mq {
 int set_error(int code, const char *msg);
@@ -50,9 +50,6 @@ int set_error(int code, const char *msg);
 
 namespace mq {
 namespace {
-
-typedef __attribute__((address_space(3))) char lds_char;
-typedef short s16x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kHd = 128;       // head dim
 constexpr int kKeys = 64;      // keys per block
@@ -67,38 +64,6 @@ struct AttnKeys {
   int nk[kMaxBatch], lo[kMaxBatch], gap[kMaxBatch];
   float npad[kMaxBatch];
 };
-
-// 16 bytes per lane from base + off straight into LDS (lane i at lds + 16 i);
-// base and lds are wave-uniform.  Read only after block_barrier.
-__device__ __forceinline__ void dma16(const char *base, uint32_t off, uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(lds)
-               : "memory", "m0");
-}
-
-// This wave's DMA has landed and its LDS reads are complete; then every wave arrives.
-__device__ __forceinline__ void block_barrier() {
-  __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0) expcnt(7) lgkmcnt(0)
-  asm volatile("s_barrier" ::: "memory");
-}
-
-// The value combined with lane ^ 32's.
-__device__ __forceinline__ float half_max(float v) {
-  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  return __builtin_fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
-}
-__device__ __forceinline__ float half_add(float v) {
-  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
-}
-
-__device__ __forceinline__ uint32_t pack2(float a, float b) {
-  typedef float f32x2 __attribute__((ext_vector_type(2)));
-  typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
-  const bf16x2 p = __builtin_convertvector((f32x2){a, b}, bf16x2);
-  uint32_t u;
-  __builtin_memcpy(&u, &p, 4);
-  return u;
-}
 
 // The log-sum-exp and guard of a row with sum l relative to 2^ms, which all
 // lanes of a half wave (or both halves) share or hold one each; `one`: the

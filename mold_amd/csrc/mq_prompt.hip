@@ -1,0 +1,467 @@
+// mq_prompt.hip — causal attention of whole prompts: packed sequences of
+// different lengths, grouped heads, what a text encoder's or a decoder's layer
+// runs between its projections (the GGUF text encoders and the prompt-expansion
+// model of crates/mold-inference/src/encoders and src/expand.rs:200-203).
+//
+//   out[i, h] = sum_{j <= i} p_ij v[j, g],  p_i = softmax_j(scale q[i, h] . k[j, g]),
+//
+// i, j inside one prompt and g = h / (heads / kv_heads), in one pass over the
+// keys with the running maximum and sum of the softmax (f32).
+//
+// The wave's inner loop is the joint attention's: transposed scores S^T = K Q^T
+// (v_mfma_f32_32x32x16, a lane holds 16 keys of one query), probabilities as the
+// B operand of O^T = V^T P^T in place, K and V blocks of 64 keys by LDS DMA one
+// block ahead, V read transposed from LDS, the scores half a block ahead of the
+// softmax.  What is different here:
+//   * a workgroup's waves take 32 tokens of several heads of one group where the
+//     group has them (4 heads x 32 tokens; 2 x 64; 1 x 128), so that they share
+//     the K and V blocks and end at the same diagonal: with 128 tokens of one
+//     head the first wave would wait through three half blocks of 32 keys that
+//     it masks whole;
+//   * a wave computes the 32-key halves up to its own diagonal and no further,
+//     and masks the diagonal one alone;
+//   * tiles run longest first (the list the host makes of the packed prompts),
+//     so that the short ones fill the launch's end;
+//   * a key that a row does not see must not reach it even as 0 x NaN: the
+//     diagonal half, the only one that mixes seen and unseen keys, looks for
+//     non-finite values among its V and, if there are any, adds them row by row
+//     (accumulate_seen).  Rows past a prompt's end are clamped to its last row,
+//     so no neighbour in the pack is ever read.
+#include "../../include/moldq.h"
+#include "mq_attn.h"
+
+#include <algorithm>
+
+namespace mq {
+int set_error(int code, const char *msg);
+}
+
+namespace mq {
+namespace {
+
+constexpr int kKeys = 64;  // keys per block
+
+struct PromptArgs {
+  const __bf16 *q, *k, *v;
+  __bf16 *out;
+  int64_t sq, sk, sv, so;  // token strides
+  int64_t hq, hk, hv, ho;  // head strides
+  const int4 *tiles;       // first row of the prompt, its length, first token of the tile, 0
+  int64_t total;           // rows of q
+  int units, group, log_heads;  // head units (of 1 << log_heads heads), heads per k/v head
+  float scale;             // times log2(e)
+};
+
+template <int S>
+struct Slot {
+  static constexpr int v = S;
+};
+
+__device__ __forceinline__ bool any_not_finite(const uint4 &u) {
+  bool odd = false;
+  for (const uint32_t two : {u.x, u.y, u.z, u.w})
+    odd = odd || (two & 0x7F80u) == 0x7F80u || (two & 0x7F800000u) == 0x7F800000u;
+  return odd;
+}
+
+template <int D, int W>
+__global__ __launch_bounds__(64 * W, D == 128 ? 2 : 3) void prompt_kernel(const PromptArgs a) {
+  constexpr int kRow = 2 * D;              // bytes of a row in LDS
+  constexpr int kBlock = kKeys * kRow;     // of a block
+  constexpr int kChunks = kRow / 16;       // 16-byte chunks of a row
+  constexpr int kDmaRows = 1024 / kRow;    // rows a wave's DMA instruction fills
+  constexpr int kDmas = kKeys / kDmaRows / W;
+  __shared__ uint4 lds_k[2][kBlock / 16];
+  __shared__ uint4 lds_v[3][kBlock / 16];
+
+  const int4 tile = a.tiles[blockIdx.x / a.units];
+  const int unit = blockIdx.x % a.units;
+  const int len = tile.y, first = tile.z;
+  // a list that does not belong to these rows: nothing is read or stored
+  if (tile.x < 0 || len <= 0 || first < 0 || first >= len || (int64_t)tile.x + len > a.total) return;
+
+  const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, h = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int head = (unit << a.log_heads) + (wave & ((1 << a.log_heads) - 1));
+  const int tok0 = first + 32 * (wave >> a.log_heads);
+  const int end = min(first + ((32 * W) >> a.log_heads), len);  // past the tile's last token
+  const int nblk = (end + kKeys - 1) / kKeys;
+  const int halves = tok0 < len ? tok0 / 32 + 1 : 0;  // 32-key halves this wave computes; the last is its diagonal
+  const int row = tok0 + l32;                         // this lane's query
+  const int64_t kvhead = (unit << a.log_heads) / a.group;
+
+  bf16x8 qf[D / 16];  // the B operand of the scores; rows past the prompt's end repeat its last and are not stored
+  {
+    const __bf16 *p = a.q + (tile.x + (int64_t)min(row, len - 1)) * a.sq + head * a.hq + 8 * h;
+#pragma unroll
+    for (int s = 0; s < D / 16; ++s) qf[s] = *reinterpret_cast<const bf16x8 *>(p + 16 * s);
+  }
+
+  // DMA of a block: load j of a wave fills LDS rows kDmaRows (wave + W j) + 0 ..,
+  // each lane fetching the chunk that the swizzle puts in its slot.  The swizzles
+  // keep 16 rows' reads of one K chunk, and 4 rows' of one V segment, on
+  // different banks.
+  const int drow = kDmaRows * wave + lane / kChunks, dch = lane % kChunks;
+  const int dk = D == 128 ? drow & 15 : (drow >> 1) & 7, dv = D == 128 ? drow & 3 : (drow >> 1) & 1;
+  const uint32_t kch = (uint32_t)((dch ^ dk) << 4), vch = (uint32_t)((dch ^ (dv << 2)) << 4);
+  const uint32_t lkw = (uint32_t)(uintptr_t)(&lds_k[0][0]) + 1024 * wave;
+  const uint32_t lvw = (uint32_t)(uintptr_t)(&lds_v[0][0]) + 1024 * wave;
+  const char *kbase = reinterpret_cast<const char *>(a.k + tile.x * a.sk + kvhead * a.hk);
+  const char *vbase = reinterpret_cast<const char *>(a.v + tile.x * a.sv + kvhead * a.hv);
+  const uint32_t kstep = (uint32_t)(2 * a.sk), vstep = (uint32_t)(2 * a.sv);
+  auto dma = [&](int blk, int kslot, int vslot) {
+    const char *kb = kbase + (int64_t)blk * (2 * kKeys) * a.sk, *vb = vbase + (int64_t)blk * (2 * kKeys) * a.sv;
+    const int top = len - 1 - blk * kKeys;
+#pragma unroll
+    for (int j = 0; j < kDmas; ++j) {
+      const uint32_t r = (uint32_t)min(drow + kDmaRows * W * j, top);
+      dma16(kb, r * kstep + kch, __builtin_amdgcn_readfirstlane(lkw + kslot * kBlock + 1024 * W * j));
+      dma16(vb, r * vstep + vch, __builtin_amdgcn_readfirstlane(lvw + vslot * kBlock + 1024 * W * j));
+    }
+  };
+
+  f32x16 o[D / 32];  // O^T: this lane's query, columns 32 d + 8 (e / 4) + 4 h + e % 4
+#pragma unroll
+  for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) o[d][e] = 0.f;
+  float m = -__FLT_MAX__, l = 0.f;  // running maximum (both halves) and this half's sum
+
+  const int i16 = lane & 15;
+  lds_char *ka[D / 16], *va[D / 32];
+  {
+    const int fk = D == 128 ? l32 & 15 : (l32 >> 1) & 7, fv = D == 128 ? i16 >> 2 : i16 >> 3;
+#pragma unroll
+    for (int s = 0; s < D / 16; ++s) ka[s] = (lds_char *)&lds_k[0][0] + (uint32_t)(l32 * kRow + (((2 * s + h) ^ fk) << 4));
+#pragma unroll
+    for (int d = 0; d < D / 32; ++d)
+      va[d] = (lds_char *)&lds_v[0][0] +
+              (uint32_t)((4 * h + (i16 >> 2)) * kRow + ((d ^ fv) << 6) + 32 * ((lane >> 4) & 1) + 8 * (i16 & 3));
+  }
+
+  // scores of keys 32 kb .. + 31 of the block in K slot `slot`: lane l32's
+  // query, keys 8 (e / 4) + 4 h + e % 4
+  auto scores = [&](int slot, int kb, f32x16 &s) {
+#pragma unroll
+    for (int e = 0; e < 16; ++e) s[e] = 0.f;
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i) {
+      const bf16x8 x = *(__attribute__((address_space(3))) bf16x8 *)(ka[i] + slot * kBlock + kb * (kBlock / 2));
+      s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x, qf[i], s, 0, 0, 0);
+    }
+  };
+  // the diagonal half: its keys tok0 + 0 .. 31 against rows tok0 + l32
+  auto mask = [&](f32x16 &s) {
+#pragma unroll
+    for (int e = 0; e < 16; ++e)
+      if (8 * (e >> 2) + 4 * h + (e & 3) > l32) s[e] = -__builtin_inff();
+  };
+  auto max16 = [&](const f32x16 &s) {
+    float r = s[0];
+#pragma unroll
+    for (int e = 1; e < 16; ++e) r = __builtin_fmaxf(r, s[e]);
+    return r;
+  };
+  auto raise_max = [&](float mx) {
+    mx = half_max(mx);
+    if (__any(mx > m)) {
+      const float mn = __builtin_fmaxf(m, mx);
+      const float f = __builtin_amdgcn_exp2f((m - mn) * a.scale);
+      m = mn;
+      l *= f;
+#pragma unroll
+      for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) o[d][e] *= f;
+    }
+  };
+  // probabilities 2^(scale (s - m)): summed in f32, rounded once to bf16, the
+  // matrix operand's type, in its order (relative 2^-9 each, independent from
+  // key to key)
+  auto probs = [&](const f32x16 &s, bf16x8 *p) {
+    const float ms = m * a.scale;
+    float sum[2] = {0.f, 0.f};
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      uint32_t u[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[8 * t + 2 * i], a.scale, -ms));
+        const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(s[8 * t + 2 * i + 1], a.scale, -ms));
+        sum[t] += x + y;
+        u[i] = pack2(x, y);
+      }
+      __builtin_memcpy(&p[t], u, 16);
+    }
+    l += sum[0] + sum[1];
+  };
+  // V^T of keys 32 kb + 16 t .. + 15, columns 32 d .. + 31: the A operand, its
+  // key order the probabilities' (4 h + 0..3 and 8 + 4 h + 0..3 of each 16)
+  auto values = [&](int slot, int kb, int t, int d) {
+    s16x4 x[2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+      x[j] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+          (__attribute__((address_space(3))) s16x4 *)(va[d] + slot * kBlock + (2 * kb + t) * (16 * kRow) + j * (8 * kRow)));
+    uint4 u;
+    __builtin_memcpy(&u, x, 16);
+    return u;
+  };
+  auto as_bf16 = [](const uint4 &u) {
+    bf16x8 x;
+    __builtin_memcpy(&x, &u, 16);
+    return x;
+  };
+  auto accumulate = [&](int slot, int kb, const bf16x8 *p) {
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int d = 0; d < D / 32; ++d)
+        o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf16(values(slot, kb, t, d)), p[t], o[d], 0, 0, 0);
+  };
+  // The diagonal half, whose V holds a value that is not finite: the finite
+  // values by their probabilities as ever, and for each row the infinities and
+  // NaN (which count as both) that it sees, counted by products with its mask.
+  auto accumulate_seen = [&](int slot, int kb, const bf16x8 *p) {
+    bf16x8 seen[2];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      uint32_t u[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int key = 16 * t + 8 * (i >> 1) + 4 * h + 2 * (i & 1);
+        u[i] = (key <= l32 ? 0x3F80u : 0u) | (key + 1 <= l32 ? 0x3F800000u : 0u);
+      }
+      __builtin_memcpy(&seen[t], u, 16);
+    }
+#pragma unroll
+    for (int d = 0; d < D / 32; ++d) {
+      f32x16 up, down;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) up[e] = down[e] = 0.f;
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const uint4 v4 = values(slot, kb, t, d);
+        const uint32_t w[4] = {v4.x, v4.y, v4.z, v4.w};
+        uint32_t fine[4], pos[4], neg[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          fine[i] = pos[i] = neg[i] = 0;
+#pragma unroll
+          for (int b = 0; b < 32; b += 16) {
+            const uint32_t x = (w[i] >> b) & 0xFFFFu;
+            const bool ok = (x & 0x7F80u) != 0x7F80u, nan = !ok && (x & 0x7Fu);
+            fine[i] |= ok ? x << b : 0u;
+            pos[i] |= !ok && (nan || !(x & 0x8000u)) ? 0x3F80u << b : 0u;
+            neg[i] |= !ok && (nan || (x & 0x8000u)) ? 0x3F80u << b : 0u;
+          }
+        }
+        o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf16(make_uint4(fine[0], fine[1], fine[2], fine[3])), p[t], o[d], 0, 0, 0);
+        up = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf16(make_uint4(pos[0], pos[1], pos[2], pos[3])), seen[t], up, 0, 0, 0);
+        down = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf16(make_uint4(neg[0], neg[1], neg[2], neg[3])), seen[t], down, 0, 0, 0);
+      }
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        if (up[e] > 0.f) o[d][e] += __builtin_inff();
+        if (down[e] > 0.f) o[d][e] -= __builtin_inff();
+      }
+    }
+  };
+  auto diagonal = [&](int slot, int kb, f32x16 &s, bf16x8 *p) {
+    mask(s);
+    raise_max(max16(s));
+    probs(s, p);
+    bool odd = false;
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int d = 0; d < D / 32; ++d) odd = any_not_finite(values(slot, kb, t, d)) || odd;
+    if (__any(odd)) accumulate_seen(slot, kb, p);
+    else accumulate(slot, kb, p);
+  };
+
+  dma(0, 0, 0);
+  block_barrier();
+  if (nblk > 1) dma(1, 1, 1);
+  f32x16 s0, s1;
+  if (halves) scores(0, 0, s0);
+  int vs = 0;  // V slot of block i
+  // The barrier in the middle of block i says that block i + 1 has landed and
+  // that every wave has read all of K(i) and V(i - 1), whose slots block i + 2
+  // then takes.  Waves pass it wherever they are: past their diagonal they only
+  // fetch for the others.
+  auto turn = [&](int i, int ks) {
+    if (i + 1 < nblk) {
+      block_barrier();
+      if (i + 2 < nblk) dma(i + 2, ks, vs == 0 ? 2 : vs - 1);
+    }
+  };
+  // a block whose keys are all seen and that is not the wave's last; its first half's scores are in s0
+  auto full = [&](int i, auto kslot) {
+    constexpr int ks = decltype(kslot)::v;
+    bf16x8 p[2];
+    raise_max(max16(s0));
+    scores(ks, 1, s1);
+    probs(s0, p);
+    accumulate(vs, 0, p);
+    const float mx = max16(s1);
+    turn(i, ks);
+    raise_max(mx);
+    scores(ks ^ 1, 0, s0);
+    probs(s1, p);
+    accumulate(vs, 1, p);
+    vs = vs == 2 ? 0 : vs + 1;
+  };
+  int i = 0;
+  for (; 2 * i + 4 < halves; i += 2) {
+    full(i, Slot<0>{});
+    full(i + 1, Slot<1>{});
+  }
+  if (2 * i + 2 < halves) full(i++, Slot<0>{});
+  if (halves) {
+    bf16x8 p[2];
+    const int ks = i & 1, kb = (halves - 1) & 1;
+    if (kb) {
+      raise_max(max16(s0));
+      scores(ks, 1, s1);
+      probs(s0, p);
+      accumulate(vs, 0, p);
+      s0 = s1;
+    }
+    turn(i, ks);
+    diagonal(vs, kb, s0, p);
+    vs = vs == 2 ? 0 : vs + 1;
+    ++i;
+  }
+  for (; i < nblk; ++i) {
+    turn(i, i & 1);
+    vs = vs == 2 ? 0 : vs + 1;
+  }
+
+  l = half_add(l);
+  const float inv = 1.f / l;
+  const bool stored = row < len;
+  __bf16 *orow = a.out + (tile.x + (int64_t)row) * a.so + head * a.ho;
+#pragma unroll
+  for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+    for (int g = 0; g < 2; ++g) {
+      // columns 32 d + 16 g + 0..15 of this query sit in lanes l32 and l32 + 32
+      // by fours; exchanged so that lane half h stores columns 8 h .. 8 h + 7
+      const f32x16 &t = o[d];
+      const uint32_t a0 = pack2(t[8 * g] * inv, t[8 * g + 1] * inv), a1 = pack2(t[8 * g + 2] * inv, t[8 * g + 3] * inv);
+      const uint32_t c0 = pack2(t[8 * g + 4] * inv, t[8 * g + 5] * inv),
+                     c1 = pack2(t[8 * g + 6] * inv, t[8 * g + 7] * inv);
+      const auto x = __builtin_amdgcn_permlane32_swap(a0, c0, false, false);
+      const auto y = __builtin_amdgcn_permlane32_swap(a1, c1, false, false);
+      if (stored) *reinterpret_cast<uint4 *>(orow + 32 * d + 16 * g + 8 * h) = make_uint4(x[0], y[0], x[1], y[1]);
+    }
+}
+
+bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+int invalid(const char *msg) { return set_error(MQ_E_INVALID, msg); }
+
+constexpr int kWaves = 4;
+
+// Heads that a workgroup of `waves` waves takes together: the largest power of
+// two that divides the group.
+int unit_log(int group, int waves) {
+  int n = 0;
+  while ((2 << n) <= waves && group % (2 << n) == 0) ++n;
+  return n;
+}
+
+// The bytes from a view's first element to past its last.
+struct Span {
+  uintptr_t lo, hi;
+};
+Span span(const void *p, int64_t rows, int64_t row_stride, int64_t heads, int64_t head_stride, int64_t dim) {
+  const uintptr_t lo = reinterpret_cast<uintptr_t>(p);
+  return {lo, lo + 2 * (uintptr_t)((rows - 1) * row_stride + (heads - 1) * head_stride + dim)};
+}
+
+}  // namespace
+}  // namespace mq
+
+extern "C" int mq_prompt_plan_make(const int64_t *lengths, int64_t count, int heads, int kv_heads, int head_dim,
+                                   mq_prompt_plan *plan, int32_t *tiles, int64_t capacity) {
+  using namespace mq;
+  if (!plan || (count > 0 && !lengths)) return invalid("mq_prompt_plan_make: NULL pointer");
+  if (head_dim != 64 && head_dim != 128) return invalid("mq_prompt_plan_make: head_dim must be 64 or 128");
+  if (count < 0 || heads < 1 || heads > 65536 || kv_heads < 1 || heads % kv_heads)
+    return invalid("mq_prompt_plan_make: negative count, or heads not a multiple of kv_heads");
+  int64_t total = 0;
+  for (int64_t s = 0; s < count; ++s) {
+    if (lengths[s] < 0 || lengths[s] >= (int64_t(1) << 31) || (total += lengths[s]) >= (int64_t(1) << 31))
+      return invalid("mq_prompt_plan_make: a negative length, or 2^31 tokens or more");
+  }
+  const int tile = (32 * kWaves) >> unit_log(heads / kv_heads, kWaves);
+  int64_t n = 0, longest = 0;
+  for (int64_t s = 0; s < count; ++s) {
+    n += (lengths[s] + tile - 1) / tile;
+    longest = std::max(longest, lengths[s]);
+  }
+  *plan = mq_prompt_plan{total, n, heads, kv_heads, head_dim, tile, kWaves};
+  if (!tiles) return MQ_OK;
+  if (capacity < n) return invalid("mq_prompt_plan_make: tiles holds fewer than the plan's tiles");
+  // longest first: the tiles at one distance from their prompts' starts, the furthest first
+  int64_t at = 0;
+  for (int64_t first = (longest - 1) / tile * tile; longest > 0 && first >= 0; first -= tile) {
+    int64_t start = 0;
+    for (int64_t s = 0; s < count; start += lengths[s++])
+      if (lengths[s] > first) {
+        int32_t *t = tiles + 4 * at++;
+        t[0] = (int32_t)start;
+        t[1] = (int32_t)lengths[s];
+        t[2] = (int32_t)first;
+        t[3] = 0;
+      }
+  }
+  return MQ_OK;
+}
+
+extern "C" int mq_prompt_attention(const mq_prompt_plan *plan, const int32_t *tiles, const void *q, int64_t q_token_stride,
+                                   int64_t q_head_stride, const void *k, int64_t k_token_stride, int64_t k_head_stride,
+                                   const void *v, int64_t v_token_stride, int64_t v_head_stride, float scale, void *out,
+                                   int64_t out_token_stride, int64_t out_head_stride, void *stream) {
+  using namespace mq;
+  if (!plan) return invalid("mq_prompt_attention: NULL plan");
+  const int heads = plan->heads, kv = plan->kv_heads, dim = plan->head_dim;
+  if ((dim != 64 && dim != 128) || heads < 1 || heads > 65536 || kv < 1 || heads % kv || plan->tokens < 0 ||
+      plan->tokens >= (int64_t(1) << 31) || plan->tiles < 0 || plan->tiles > plan->tokens || plan->waves != kWaves ||
+      plan->tile_tokens != (32 * kWaves) >> unit_log(heads / kv, kWaves))
+    return invalid("mq_prompt_attention: not a plan of mq_prompt_plan_make");
+  if (!(scale > 0.f) || scale > 3e38f) return invalid("mq_prompt_attention: scale must be positive and finite");
+  if (plan->tokens == 0 || plan->tiles == 0) return MQ_OK;
+  if (!tiles || !q || !k || !v || !out) return invalid("mq_prompt_attention: NULL pointer");
+  if (!aligned16(tiles) || !aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(out))
+    return invalid("mq_prompt_attention: buffers must be 16-byte aligned");
+  for (int64_t s : {q_token_stride, q_head_stride, k_token_stride, k_head_stride, v_token_stride, v_head_stride,
+                    out_token_stride, out_head_stride})
+    if (s < 0 || s % 8 || s >= (int64_t(1) << 24))
+      return invalid("mq_prompt_attention: strides must be multiples of 8 elements, 0 to 2^24");
+  // rows and heads of out apart from each other
+  const int64_t small = std::min(heads > 1 ? out_head_stride : out_token_stride, out_token_stride);
+  const bool by_token = heads == 1 || out_token_stride >= out_head_stride;
+  if (small < dim || (heads > 1 && plan->tokens > 1 &&
+                      (by_token ? out_token_stride < (heads - 1) * out_head_stride + dim
+                                : out_head_stride < (plan->tokens - 1) * out_token_stride + dim)))
+    return invalid("mq_prompt_attention: rows or heads of out overlap");
+  const Span o = span(out, plan->tokens, out_token_stride, heads, out_head_stride, dim);
+  for (const Span &in : {span(q, plan->tokens, q_token_stride, heads, q_head_stride, dim),
+                         span(k, plan->tokens, k_token_stride, kv, k_head_stride, dim),
+                         span(v, plan->tokens, v_token_stride, kv, v_head_stride, dim)})
+    if (o.lo < in.hi && in.lo < o.hi) return invalid("mq_prompt_attention: out lies over q, k or v");
+  const int log_heads = unit_log(heads / kv, kWaves), units = heads >> log_heads;
+  const int64_t grid = plan->tiles * units;
+  if (grid >= (int64_t(1) << 31)) return invalid("mq_prompt_attention: 2^31 tiles or more");
+  const PromptArgs a{static_cast<const __bf16 *>(q), static_cast<const __bf16 *>(k), static_cast<const __bf16 *>(v),
+                     static_cast<__bf16 *>(out), q_token_stride, k_token_stride, v_token_stride, out_token_stride,
+                     q_head_stride, k_head_stride, v_head_stride, out_head_stride, reinterpret_cast<const int4 *>(tiles),
+                     plan->tokens, units, heads / kv, log_heads, scale * 1.44269504f};
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  if (dim == 128) hipLaunchKernelGGL((prompt_kernel<128, kWaves>), dim3((unsigned)grid), dim3(64 * kWaves), 0, s, a);
+  else hipLaunchKernelGGL((prompt_kernel<64, kWaves>), dim3((unsigned)grid), dim3(64 * kWaves), 0, s, a);
+  const hipError_t e = hipGetLastError();
+  return e == hipSuccess ? MQ_OK : set_error(MQ_E_HIP, hipGetErrorString(e));
+}

@@ -1,0 +1,137 @@
+"""Attention of the GGUF text models (text encoders, prompt expansion): whole prompts, and new
+tokens over a paged key/value cache, run by libmoldq (mq_prompt_attention, mq_kv_cache_* and
+mq_cache_attention in include/moldq.h).
+
+candle composes both of matmul, mask and softmax and grows its cache by concatenation
+(quantized_qwen3's attention, used at crates/mold-inference/src/expand.rs:200-203).  Here the
+prompts of a batch are packed without padding, query heads share k/v heads, and the cache
+holds BF16 or the ggml block types Q8_0 and Q4_0.
+
+Everything runs on torch's current stream of the tensors' device and allocates only outputs
+and scratch.  Inference only: calls that autograd or a tracer would record are refused.
+"""
+from __future__ import annotations
+
+import ctypes
+
+import numpy as np
+import torch
+
+from . import _lib
+from ._lib import check
+from .fused import recorded
+from .quantized import _stream_ptr
+
+_MAX_STRIDE = 1 << 24
+
+
+def _on(device):
+    """The device made current, unless it is."""
+    return torch.cuda.device(device)
+
+
+def _heads_view(name, t, heads, dim, device):
+    """t as the library reads it: bf16 [tokens, heads, dim] on `device` with unit stride along
+    the head, 16-byte rows and strides; copied if it is anything else of that shape."""
+    if t.dtype is not torch.bfloat16 or t.dim() != 3 or t.shape[1] != heads or t.shape[2] != dim or t.device != device:
+        raise ValueError(f"{name} must be bf16 [tokens, {heads}, {dim}] on {device}")
+    return t if _readable(t) else t.contiguous()
+
+
+def _readable(t):
+    st, sh, sd = t.stride()
+    n, h, _ = t.shape
+    return (sd == 1 and t.data_ptr() % 16 == 0 and (n <= 1 or (st % 8 == 0 and st < _MAX_STRIDE))
+            and (h == 1 or (sh % 8 == 0 and sh < _MAX_STRIDE)))
+
+
+def _strides(t):
+    """Token and head stride; those of a single token or head, which may be anything, as if packed."""
+    n, h, d = t.shape
+    sh = t.stride(1) if h > 1 else d
+    return (t.stride(0) if n > 1 else h * d), sh
+
+
+def _writable(t):
+    """Whether the kernels can store into t as it is: readable, with rows and heads apart."""
+    if not _readable(t):
+        return False
+    n, h, d = t.shape
+    st, sh = _strides(t)
+    if n == 1 or h == 1:
+        return (n == 1 or st >= d) and (h == 1 or sh >= d)
+    return st >= d and sh >= d and (st >= (h - 1) * sh + d or sh >= (n - 1) * st + d)
+
+
+def _span(t):
+    """The addresses from t's first byte to past its last."""
+    last = sum((n - 1) * stride for n, stride in zip(t.shape, t.stride()))
+    return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
+
+
+def _apart(out, t):
+    (lo, hi), (a, b) = _span(out), _span(t)
+    return b <= lo or hi <= a
+
+
+def _out(name, out, shape, device, inputs):
+    """The tensor to write: `out`, or a temporary where the kernel cannot store into it (another
+    device, unaligned or overlapping rows, over an input that other workgroups still read)."""
+    if out is None:
+        return torch.empty(shape, dtype=torch.bfloat16, device=device)
+    if out.dtype is not torch.bfloat16 or tuple(out.shape) != tuple(shape):
+        raise ValueError(f"{name}: out must be bf16 {list(shape)}")
+    if out.device == device and _writable(out) and all(_apart(out, t) for t in inputs):
+        return out
+    return torch.empty(shape, dtype=torch.bfloat16, device=device)
+
+
+def _given(out, res):
+    if out is None or res is out:
+        if out is not None:
+            torch.autograd.graph.increment_version(out)     # written in place, as a copy_ tells autograd
+        return res
+    return out.copy_(res)
+
+
+class PromptPlan:
+    """How a batch of packed prompts is attended, made once for its lengths and used by every
+    layer with these heads: prompt s is the `lengths[s]` rows after those of the prompts before
+    it.  heads a multiple of kv_heads, head_dim 64 or 128."""
+
+    def __init__(self, lengths, heads: int, kv_heads: int, head_dim: int = 128, device="cuda"):
+        self.lengths = [int(x) for x in lengths]
+        lib = _lib.load()
+        host = (ctypes.c_int64 * max(1, len(self.lengths)))(*self.lengths)
+        self.c = _lib.PromptPlanC()
+        args = (host, len(self.lengths), int(heads), int(kv_heads), int(head_dim), ctypes.byref(self.c))
+        check(lib.mq_prompt_plan_make(*args, None, 0))
+        tiles = np.zeros((max(1, self.c.tiles), 4), dtype=np.int32)
+        check(lib.mq_prompt_plan_make(*args, tiles.ctypes.data_as(ctypes.POINTER(ctypes.c_int32)), len(tiles)))
+        self.tiles = torch.from_numpy(tiles).to(device)
+        self.device = self.tiles.device
+        self.tokens = int(self.c.tokens)
+        self.heads, self.kv_heads, self.head_dim = int(heads), int(kv_heads), int(head_dim)
+        self._ref = ctypes.byref(self.c)
+
+
+def prompt_attention(q, k, v, plan: PromptPlan, scale=None, out=None):
+    """Causal attention inside each of the plan's prompts: q bf16 [tokens, heads, dim], k and v
+    bf16 [tokens, kv_heads, dim] (views of one projection's output are read in place) ->
+    bf16 [tokens, heads, dim], `out` if given.  scale defaults to dim ** -0.5."""
+    dim, device = plan.head_dim, plan.device
+    if recorded(q, k, v):
+        raise ValueError("prompt_attention: inference only, nothing may record the call")
+    q = _heads_view("prompt_attention: q", q, plan.heads, dim, device)
+    k = _heads_view("prompt_attention: k", k, plan.kv_heads, dim, device)
+    v = _heads_view("prompt_attention: v", v, plan.kv_heads, dim, device)
+    n = plan.tokens
+    if not q.shape[0] == k.shape[0] == v.shape[0] == n:
+        raise ValueError(f"prompt_attention: q, k and v must have the plan's {n} tokens")
+    res = _out("prompt_attention", out, q.shape, device, (q, k, v))
+    if n:
+        with _on(device):
+            check(_lib.load().mq_prompt_attention(
+                plan._ref, plan.tiles.data_ptr(), q.data_ptr(), *_strides(q), k.data_ptr(), *_strides(k), v.data_ptr(),
+                *_strides(v), dim ** -0.5 if scale is None else scale, res.data_ptr(), *_strides(res), _stream_ptr()))
+    return _given(out, res)
