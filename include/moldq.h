@@ -326,6 +326,34 @@ int mq_prompt_attention(const mq_prompt_plan *plan, const int32_t *tiles, const 
                         const void *v, int64_t v_token_stride, int64_t v_head_stride, float scale, void *out,
                         int64_t out_token_stride, int64_t out_head_stride, void *stream);
 
+/* A paged key/value cache: `pages` pages of page_tokens tokens (a multiple of
+ * 32) of kv_heads heads of head_dim 64 or 128, held as BF16 or in ggml's Q8_0 or
+ * Q4_0 blocks along the head.  Slot s is token s % page_tokens of page s /
+ * page_tokens.  `data` is mq_kv_cache_size bytes of device memory (16-byte
+ * aligned) of the caller's, in a layout of the library's own; it needs no
+ * clearing.  The size is 0 for a description that is not valid. */
+typedef struct mq_kv_cache {
+    void *data;
+    int64_t pages;
+    int32_t dtype, kv_heads, head_dim, page_tokens;
+} mq_kv_cache;
+size_t mq_kv_cache_size(const mq_kv_cache *cache);
+/* Write rows t < tokens of k and v (F32 or BF16, head h of row t at t *
+ * token_stride + h * head_stride, unit stride inside a head, 16-byte aligned,
+ * strides multiples of 16 bytes) to slots[t] (device memory).  BF16 rounds to
+ * nearest even; a block type's blocks are those of mq_quantize, and a block with
+ * a value that is not finite reads back as NaN.  Slots outside the cache are
+ * skipped (a padding row's is -1); two rows of one call must not share a slot.
+ * Asynchronous on stream. */
+int mq_kv_cache_append(const mq_kv_cache *cache, const void *k, int64_t k_token_stride, int64_t k_head_stride,
+                       const void *v, int64_t v_token_stride, int64_t v_head_stride, int x_dtype, int64_t tokens,
+                       const int64_t *slots, void *stream);
+/* Read the slots' keys and values back into k and v (F32 or BF16, contiguous
+ * [count, kv_heads, head_dim], 16-byte aligned); zeros for a slot outside the
+ * cache.  Asynchronous on stream. */
+int mq_kv_cache_read(const mq_kv_cache *cache, const int64_t *slots, int64_t count, void *k, void *v, int out_dtype,
+                     void *stream);
+
 /* Quantize activations once for several Q4_K GEMVs: x [m, k] (F32 or BF16,
  * row stride ldx, 16-byte aligned rows) -> m * k / 256 blocks of
  * MQ_X_Q8K_BLOCK_BYTES at dst (16-byte aligned), by the Q8_K quantization

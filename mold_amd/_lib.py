@@ -32,6 +32,12 @@ class PromptPlanC(ctypes.Structure):
         (f, ctypes.c_int32) for f in ("heads", "kv_heads", "head_dim", "tile_tokens", "waves")]
 
 
+class KvCacheC(ctypes.Structure):
+    """mq_kv_cache"""
+    _fields_ = [("data", ctypes.c_void_p), ("pages", ctypes.c_int64)] + [
+        (f, ctypes.c_int32) for f in ("dtype", "kv_heads", "head_dim", "page_tokens")]
+
+
 SIGNATURES = {
     "mq_last_error": (ctypes.c_char_p, []),
     "mq_version": (_int, []),
@@ -74,6 +80,9 @@ SIGNATURES = {
                                    ctypes.POINTER(ctypes.c_int32), _i64]),
     "mq_prompt_attention": (_int, [ctypes.POINTER(PromptPlanC), _vp] + [_vp, _i64, _i64] * 3 + [ctypes.c_float]
                             + [_vp, _i64, _i64] + [_vp]),
+    "mq_kv_cache_size": (_sz, [ctypes.POINTER(KvCacheC)]),
+    "mq_kv_cache_append": (_int, [ctypes.POINTER(KvCacheC)] + [_vp, _i64, _i64] * 2 + [_int, _i64, _vp, _vp]),
+    "mq_kv_cache_read": (_int, [ctypes.POINTER(KvCacheC), _vp, _i64, _vp, _vp, _int, _vp]),
     "mq_gguf_open": (_int, [ctypes.c_char_p, _pp]),
     "mq_gguf_close": (None, [_vp]),
     "mq_gguf_tensor_count": (_i64, [_vp]),

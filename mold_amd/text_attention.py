@@ -20,7 +20,7 @@ import torch
 from . import _lib
 from ._lib import check
 from .fused import recorded
-from .quantized import _stream_ptr
+from .quantized import GgmlDType, _dtype_code, _stream_ptr
 
 _MAX_STRIDE = 1 << 24
 
@@ -135,3 +135,72 @@ def prompt_attention(q, k, v, plan: PromptPlan, scale=None, out=None):
                 plan._ref, plan.tiles.data_ptr(), q.data_ptr(), *_strides(q), k.data_ptr(), *_strides(k), v.data_ptr(),
                 *_strides(v), dim ** -0.5 if scale is None else scale, res.data_ptr(), *_strides(res), _stream_ptr()))
     return _given(out, res)
+
+
+class KvCache:
+    """A paged key/value cache on the device, of `pages` pages of `page_tokens` tokens (a multiple
+    of 32), BF16 or in Q8_0 / Q4_0 blocks along the head; head_dim 64 or 128.  Slot s is token
+    s % page_tokens of page s // page_tokens; which pages a sequence has is the caller's page table."""
+
+    def __init__(self, pages: int, kv_heads: int, head_dim: int = 128, page_tokens: int = 64,
+                 dtype: GgmlDType = GgmlDType.Q8_0, device="cuda"):
+        self.c = _lib.KvCacheC(None, int(pages), int(dtype), int(kv_heads), int(head_dim), int(page_tokens))
+        self._ref = ctypes.byref(self.c)
+        lib = _lib.load()
+        size = lib.mq_kv_cache_size(self._ref)
+        if size == 0 and pages != 0:
+            raise ValueError("KvCache: BF16, Q8_0 or Q4_0, heads of 64 or 128, pages of a multiple of 32 tokens up to 65536, "
+                             f"1 to 4096 heads; got {GgmlDType(dtype).name}, {head_dim}, {page_tokens}, {kv_heads}")
+        self.data = torch.empty(size, dtype=torch.uint8, device=device)
+        self.c.data = self.data.data_ptr()
+        self.device = self.data.device
+        self.pages, self.kv_heads, self.head_dim, self.page_tokens = int(pages), int(kv_heads), int(head_dim), int(page_tokens)
+        self.dtype = GgmlDType(dtype)
+
+    def slots(self, page_table, positions):
+        """The slots of `positions` [batch, n] of the sequences whose pages are page_table
+        [batch, pages]; -1 (skipped by append) for a negative position."""
+        at = positions.clamp(min=0).long()
+        page = torch.gather(page_table.long(), 1, at // self.page_tokens)
+        return torch.where(positions < 0, -1, page * self.page_tokens + at % self.page_tokens)
+
+    def _slots(self, name, slots):
+        if slots.dtype is not torch.int64 or slots.dim() != 1 or slots.device != self.device:
+            raise ValueError(f"{name}: slots must be int64 [tokens] on {self.device}")
+        return slots if slots.is_contiguous() else slots.contiguous()
+
+    def append(self, k, v, slots):
+        """Write k and v [tokens, kv_heads, head_dim] (bf16 or f32, both the same) to `slots`, int64
+        [tokens] on the device; a slot outside the cache is skipped.  Two tokens must not share one."""
+        if recorded(k, v):
+            raise ValueError("KvCache.append: inference only, nothing may record the call")
+        slots = self._slots("KvCache.append", slots)
+        n = slots.shape[0]
+        parts = []
+        for t in (k, v):
+            if t.dtype not in (torch.bfloat16, torch.float32) or t.dtype != k.dtype or t.device != self.device \
+                    or tuple(t.shape) != (n, self.kv_heads, self.head_dim):
+                raise ValueError("KvCache.append: k and v must be bf16 or f32 "
+                                 f"[{n}, {self.kv_heads}, {self.head_dim}] on {self.device}")
+            unit = 16 // t.element_size()
+            st, sh = _strides(t)
+            parts.append(t if t.stride(2) == 1 and t.data_ptr() % 16 == 0 and st % unit == 0 and sh % unit == 0
+                         else t.contiguous())
+        k, v = parts
+        if n:
+            with _on(self.device):
+                check(_lib.load().mq_kv_cache_append(self._ref, k.data_ptr(), *_strides(k), v.data_ptr(), *_strides(v),
+                                                     _dtype_code(k.dtype), n, slots.data_ptr(), _stream_ptr()))
+
+    def read(self, slots, dtype=torch.bfloat16):
+        """(k, v) [tokens, kv_heads, head_dim] of `slots`, bf16 or f32; zeros for a slot outside the cache."""
+        slots = self._slots("KvCache.read", slots)
+        if dtype not in (torch.bfloat16, torch.float32):
+            raise ValueError("KvCache.read: dtype must be bf16 or f32")
+        shape = (slots.shape[0], self.kv_heads, self.head_dim)
+        k, v = (torch.empty(shape, dtype=dtype, device=self.device) for _ in range(2))
+        if shape[0]:
+            with _on(self.device):
+                check(_lib.load().mq_kv_cache_read(self._ref, slots.data_ptr(), shape[0], k.data_ptr(), v.data_ptr(),
+                                                   _dtype_code(dtype), _stream_ptr()))
+        return k, v
