@@ -342,7 +342,8 @@ size_t mq_kv_cache_size(const mq_kv_cache *cache);
  * token_stride + h * head_stride, unit stride inside a head, 16-byte aligned,
  * strides multiples of 16 bytes) to slots[t] (device memory).  BF16 rounds to
  * nearest even; a block type's blocks are those of mq_quantize, and a block with
- * a value that is not finite reads back as NaN.  Slots outside the cache are
+ * a value that is not finite reads back as NaN (one whose scale passes float16
+ * as infinities and NaN).  Slots outside the cache are
  * skipped (a padding row's is -1); two rows of one call must not share a slot.
  * Asynchronous on stream. */
 int mq_kv_cache_append(const mq_kv_cache *cache, const void *k, int64_t k_token_stride, int64_t k_head_stride,
@@ -353,6 +354,24 @@ int mq_kv_cache_append(const mq_kv_cache *cache, const void *k, int64_t k_token_
  * cache.  Asynchronous on stream. */
 int mq_kv_cache_read(const mq_kv_cache *cache, const int64_t *slots, int64_t count, void *k, void *v, int out_dtype,
                      void *stream);
+
+/* Attention of one new token of each of `batch` sequences over the cache:
+ * out[b, h] = softmax(scale q[b, h] . k) v over the first lengths[b] tokens of
+ * sequence b, whose token t lies in page page_table[b * table_stride + t /
+ * page_tokens]; query head h reads k/v head h / (heads / kv_heads).  q, out: bf16,
+ * head h of sequence b at b * batch_stride + h * head_stride, 16-byte aligned,
+ * strides multiples of 8 elements, out apart from q.  page_table and lengths are
+ * device memory: the host neither reads them nor waits.  f32 scores, softmax and
+ * sums.  A sequence of no tokens gives zeros; one that names a page outside the
+ * cache, or is longer than its max_pages pages, gives NaN.  scratch: at least
+ * mq_cache_attention_scratch_size bytes (device, 16-byte aligned, of this call
+ * alone).  Asynchronous on stream; may be captured in a graph, whose replays
+ * read the lengths anew. */
+int mq_cache_attention(const mq_kv_cache *cache, const void *q, int64_t q_batch_stride, int64_t q_head_stride,
+                       int64_t batch, int heads, const int32_t *page_table, int64_t table_stride, int64_t max_pages,
+                       const int32_t *lengths, float scale, void *out, int64_t out_batch_stride,
+                       int64_t out_head_stride, void *scratch, size_t scratch_bytes, void *stream);
+size_t mq_cache_attention_scratch_size(const mq_kv_cache *cache, int64_t batch, int heads, int64_t max_pages);
 
 /* Quantize activations once for several Q4_K GEMVs: x [m, k] (F32 or BF16,
  * row stride ldx, 16-byte aligned rows) -> m * k / 256 blocks of

@@ -83,6 +83,9 @@ SIGNATURES = {
     "mq_kv_cache_size": (_sz, [ctypes.POINTER(KvCacheC)]),
     "mq_kv_cache_append": (_int, [ctypes.POINTER(KvCacheC)] + [_vp, _i64, _i64] * 2 + [_int, _i64, _vp, _vp]),
     "mq_kv_cache_read": (_int, [ctypes.POINTER(KvCacheC), _vp, _i64, _vp, _vp, _int, _vp]),
+    "mq_cache_attention": (_int, [ctypes.POINTER(KvCacheC), _vp, _i64, _i64, _i64, _int, _vp, _i64, _i64, _vp,
+                                  ctypes.c_float, _vp, _i64, _i64, _vp, _sz, _vp]),
+    "mq_cache_attention_scratch_size": (_sz, [ctypes.POINTER(KvCacheC), _i64, _int, _i64]),
     "mq_gguf_open": (_int, [ctypes.c_char_p, _pp]),
     "mq_gguf_close": (None, [_vp]),
     "mq_gguf_tensor_count": (_i64, [_vp]),

@@ -204,3 +204,35 @@ class KvCache:
                 check(_lib.load().mq_kv_cache_read(self._ref, slots.data_ptr(), shape[0], k.data_ptr(), v.data_ptr(),
                                                    _dtype_code(dtype), _stream_ptr()))
         return k, v
+
+    def attend(self, q, page_table, lengths, scale=None, out=None):
+        """Attention of one new token per sequence: q bf16 [batch, heads, head_dim] over the first
+        lengths[b] tokens (int32 [batch], the new one's included once it is appended) of the pages
+        page_table[b] (int32 [batch, pages]) -> bf16 [batch, heads, head_dim], `out` if given.
+        scale defaults to head_dim ** -0.5.  Table and lengths are read on the device."""
+        device, dim = self.device, self.head_dim
+        if recorded(q):
+            raise ValueError("KvCache.attend: inference only, nothing may record the call")
+        if q.dim() != 3 or q.shape[1] == 0 or q.shape[1] % self.kv_heads:
+            raise ValueError(f"KvCache.attend: q must be [batch, heads, {dim}] with a multiple of {self.kv_heads} heads")
+        n, heads, _ = q.shape
+        q = _heads_view("KvCache.attend: q", q, heads, dim, device)
+        for name, t, dims in (("page_table", page_table, 2), ("lengths", lengths, 1)):
+            if t.dtype is not torch.int32 or t.dim() != dims or t.shape[0] != n or t.device != device:
+                raise ValueError(f"KvCache.attend: {name} must be int32 [{n}{', pages' if dims == 2 else ''}] on {device}")
+        pages = page_table.shape[1]
+        if n > 1 and page_table.stride(0) < pages or pages > 1 and page_table.stride(1) != 1:
+            page_table = page_table.contiguous()
+        lengths = lengths if lengths.is_contiguous() else lengths.contiguous()
+        res = _out("KvCache.attend", out, q.shape, device, (q,))
+        if n:
+            lib = _lib.load()
+            with _on(device):
+                nbytes = lib.mq_cache_attention_scratch_size(self._ref, n, heads, pages)
+                scratch = torch.empty(nbytes, dtype=torch.uint8, device=device)     # freed to this stream
+                check(lib.mq_cache_attention(
+                    self._ref, q.data_ptr(), *_strides(q), n, heads, page_table.data_ptr(),
+                    page_table.stride(0) if n > 1 else pages, pages, lengths.data_ptr(),
+                    dim ** -0.5 if scale is None else scale, res.data_ptr(), *_strides(res), scratch.data_ptr(), nbytes,
+                    _stream_ptr()))
+        return _given(out, res)
