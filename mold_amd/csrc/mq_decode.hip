@@ -34,10 +34,10 @@ int set_error(int code, const char *msg);
 namespace mq {
 namespace {
 
-constexpr int kWaves = 4;           // of a workgroup
+constexpr int kWaves = 4;           // of a workgroup whose waves take runs of the line
 constexpr int kMaxWaves = 2048;     // of a launch: 8 a CU
-constexpr int kMinTiles = 1;        // of a run
 constexpr int kHeads = 16;          // columns of the matrix instruction
+constexpr int kPairWaves = 8;       // of a workgroup that takes one (sequence, head unit)
 
 struct DecodeArgs {
   CacheView cache;
@@ -55,6 +55,10 @@ struct DecodeArgs {
 
 __device__ __forceinline__ int lane_of(int v, int lane) { return __builtin_amdgcn_readlane(v, lane); }
 
+// A value that is the same in all lanes, as the scalar that the compiler does not
+// make of a division's result (or of what follows from it) by itself.
+__device__ __forceinline__ int scalar(int v) { return __builtin_amdgcn_readfirstlane(v); }
+
 // Sums over lanes 0 .. lane.
 __device__ __forceinline__ int scan64(int x) {
   x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);  // row_shr 1, 2, 4, 8
@@ -71,36 +75,43 @@ __device__ __forceinline__ int scan64(int x) {
 // c0 + i; every wave sees the same line.
 struct Line {
   int c0, before;      // first sequence of the 64 at hand, tiles of those before
-  int tiles, upto;     // this lane's: its tiles, the tiles of c0 .. its own
+  int n, tiles, upto;  // this lane's: its length, its tiles, the tiles of c0 .. its own
   int total, heads;    // tiles of all sequences, head units
   int runs, base, rest;  // runs, their least length, how many are one longer
 
-  __device__ static int tiles_of(const DecodeArgs &a, int b) {
-    if (b >= a.batch) return 0;
-    const int64_t cap = (int64_t)a.max_pages * a.cache.page_tokens;
-    const int64_t n = a.lengths[b];
-    return n <= 0 ? 0 : (int)(((n < cap ? n : cap) + kTileTokens - 1) / kTileTokens);
+  // The tiles of a sequence of n tokens, as far as its table reaches.
+  __device__ static int tiles_of(const DecodeArgs &a, int n) {
+    return n > 0 ? (min(n, a.max_pages * a.cache.page_tokens) + kTileTokens - 1) / kTileTokens : 0;
   }
   __device__ void load(const DecodeArgs &a, int lane) {
-    tiles = tiles_of(a, c0 + lane);
+    const int b = c0 + lane, len = a.lengths[min(b, a.batch - 1)];
+    n = b < a.batch ? len : 0;
+    tiles = tiles_of(a, n);
     upto = scan64(tiles);
   }
-  __device__ Line(const DecodeArgs &a, int lane) : c0(0), before(0), total(0), heads(a.cache.kv_heads * a.chunks) {
+  __device__ void make(const DecodeArgs &a, int lane) {
+    c0 = before = total = 0;
+    heads = a.cache.kv_heads * a.chunks;
     for (int c = (a.batch - 1) & ~63; c >= 0; c -= 64) {  // the first 64 last: they stay
       c0 = c;
       load(a, lane);
       total += lane_of(upto, 63);
     }
     const int units = total * heads;
-    runs = min(a.waves, units / kMinTiles);
-    runs = max(runs, 1);
-    base = units / runs;
+    runs = max(min(a.waves, units), 1);
+    base = scalar(units / runs);
     rest = units - base * runs;
   }
   __device__ int start(int run) const { return run * base + min(run, rest); }
   __device__ int run_of(int unit) const {
     const int longer = rest * (base + 1);
     return unit < longer ? unit / (base + 1) : rest + (unit - longer) / base;
+  }
+  // Whether the runs of `run`'s workgroup are all within the units u0 .. u1 - 1 of
+  // one (sequence, head unit): then their sums are one record, at the first's place.
+  __device__ bool together(int run, int u0, int u1) const {
+    const int r0 = run & -kWaves;
+    return r0 + kWaves <= runs && start(r0) >= u0 && start(r0 + kWaves) <= u1;
   }
   // The lane of the sequence that holds `unit`, after its 64 have been loaded.
   __device__ int seek(const DecodeArgs &a, int lane, int unit) {
@@ -119,32 +130,38 @@ struct Tile {
   static constexpr int kKeyWords = L::kKeyLane / 4, kScaleWords = L::kQuant ? 4 * L::kBlocks : 0;
   uint32_t k[2][kKeyWords], v[2 * kKeyWords], ks[kScaleWords + 1], vs[kScaleWords + 1];
 
-  __device__ __forceinline__ static void get16(uint32_t *to, const uint8_t *p) {
-    const uint4 u = *reinterpret_cast<const uint4 *>(p);
+  // Buffer loads: the tile's address is in scalar registers, a lane adds only its
+  // place in a piece, so that no load needs vector registers for an address.
+  __device__ __forceinline__ static void get16(uint32_t *to, __amdgpu_buffer_rsrc_t tile, int lane_at, int at) {
+    typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+    const u32x4 u = __builtin_amdgcn_raw_buffer_load_b128(tile, lane_at, at, 0);
     to[0] = u.x; to[1] = u.y; to[2] = u.z; to[3] = u.w;
   }
-  __device__ __forceinline__ void load(const uint8_t *tile, int lane) {
+  __device__ __forceinline__ void load(const uint8_t *at, int lane) {
+    const __amdgpu_buffer_rsrc_t tile =
+        __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(at), 0, L::kBytes, 0x00027000);
     if constexpr (L::kKeyPiece == 16) {
 #pragma unroll
       for (int u = 0; u < 2; ++u)
 #pragma unroll
-        for (int i = 0; i < kKeyWords; i += 4) get16(&k[u][i], tile + u * 64 * L::kKeyLane + i * 256 + lane * 16);
+        for (int i = 0; i < kKeyWords; i += 4) get16(&k[u][i], tile, lane * 16, u * 64 * L::kKeyLane + i * 256);
     } else {
+      typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
-        const uint2 w = *reinterpret_cast<const uint2 *>(tile + u * 64 * L::kKeyLane + lane * 8);
+        const u32x2 w = __builtin_amdgcn_raw_buffer_load_b64(tile, lane * 8, u * 64 * L::kKeyLane, 0);
         k[u][0] = w.x;
         k[u][1] = w.y;
       }
     }
 #pragma unroll
-    for (int i = 0; i < 2 * kKeyWords; i += 4) get16(&v[i], tile + L::kPlane + i * 256 + lane * 16);
+    for (int i = 0; i < 2 * kKeyWords; i += 4) get16(&v[i], tile, lane * 16, L::kPlane + i * 256);
     if constexpr (L::kQuant) {
-      const uint8_t *s = tile + 2 * L::kPlane + (lane >> 4) * (16 * L::kBlocks);
+      const int mine = (lane >> 4) * (16 * L::kBlocks);
 #pragma unroll
       for (int i = 0; i < kScaleWords; i += 4) {
-        get16(&ks[i], s + 4 * i);
-        get16(&vs[i], s + L::kScales + 4 * i);
+        get16(&ks[i], tile, mine, 2 * L::kPlane + 4 * i);
+        get16(&vs[i], tile, mine, 2 * L::kPlane + L::kScales + 4 * i);
       }
     }
   }
@@ -211,83 +228,131 @@ __device__ __forceinline__ float column_add(float v) {
   return half_add(__uint_as_float(r[0]) + __uint_as_float(r[1]));
 }
 
-template <int T, int D>
-__global__ __launch_bounds__(64 * kWaves, 2) void decode_kernel(const DecodeArgs a) {
-  using L = CacheTile<T, D>;
-  constexpr int kB = L::kBlocks, kC = D / 16;
-  const int lane = threadIdx.x & 63, g = lane >> 4, r = lane & 15;
-  const int run = __builtin_amdgcn_readfirstlane(blockIdx.x * kWaves + (threadIdx.x >> 6));
-  Line line(a, lane);
-  if (line.total == 0 || run >= line.runs) return;
-  const int first = line.start(run), end = line.start(run + 1);
-  const int tpp = a.cache.page_tokens / kTileTokens;
+// Shares of one (sequence, head unit) that the waves of a workgroup hold, added
+// in the order of the waves, each relative to its own maximum.
+template <int D, int W>
+struct Shares {
+  float o[W][kHeads][D + 4], m[W][kHeads], l[W][kHeads];
 
-  // The unit whose tile is loaded next.
-  struct Unit {
-    int at, b, kv, chunk, t, tiles;  // place on the line, sequence, k/v head, chunk of its heads, tile of the sequence's tiles
-    bool bad;                   // its page is not one of the cache's
-  };
-  int idx = line.seek(a, lane, first);  // its sequence's lane
-  Unit nx;
-  {
-    const int tiles = lane_of(line.tiles, idx), in = first - (line.before + lane_of(line.upto, idx) - tiles) * line.heads;
-    const int head = in / tiles;
-    nx = Unit{first, line.c0 + idx, head / a.chunks, head % a.chunks, in - head * tiles, tiles, false};
+  __device__ __forceinline__ void put(int wave, int lane, const f32x4 *x, float ms, float sum) {
+    const int g = lane >> 4, r = lane & 15;
+#pragma unroll
+    for (int c = 0; c < D / 16; ++c) *reinterpret_cast<f32x4 *>(&o[wave][r][16 * c + 4 * g]) = x[c];
+    if (g == 0) {
+      m[wave][r] = ms;
+      l[wave][r] = sum;
+    }
   }
-  // its sequence's page numbers page0 .. page0 + 63, one a lane
-  int page0 = nx.t / tpp, page = page0, in_page = nx.t % tpp, numbers = 0;
-  auto number_pages = [&]() {
-    numbers = page0 + lane < a.max_pages ? a.table[nx.b * a.table_stride + page0 + lane] : 0;
-  };
-  number_pages();
-  auto fetch = [&](Tile<T, D> &to) {
-    const uint32_t id = (uint32_t)lane_of(numbers, page - page0);
-    nx.bad = id >= a.pages;
-    const int64_t at = ((int64_t)(nx.bad ? 0 : id) * a.cache.kv_heads + nx.kv) * tpp + in_page;
-    to.load(a.cache.data + at * L::kBytes, lane);
-  };
-  auto advance = [&]() {  // to the run's next unit; past its last the tile stays where it is
-    if (nx.at + 1 >= end) return;
-    ++nx.at;
-    if (++nx.t < nx.tiles) {
-      if (++in_page == tpp) {
-        in_page = 0;
-        if (++page == page0 + 64) {
-          page0 = page;
-          number_pages();
-        }
-      }
+  // head r's sums of columns 4 col .. + 3, relative to 2^top
+  __device__ __forceinline__ f32x4 add(int r, int col, float &top, float &sum) const {
+    top = m[0][r];
+#pragma unroll
+    for (int w = 1; w < W; ++w) top = __builtin_fmaxf(top, m[w][r]);
+    f32x4 x{0.f, 0.f, 0.f, 0.f};
+    sum = 0.f;
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+      const float e = m[w][r] == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(m[w][r] - top);
+      sum = __builtin_fmaf(e, l[w][r], sum);
+      const f32x4 v = *reinterpret_cast<const f32x4 *>(&o[w][r][4 * col]);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[i] = __builtin_fmaf(e, v[i], x[i]);
+    }
+    return x;
+  }
+};
+
+__device__ __forceinline__ void store4(__bf16 *p, const f32x4 &x, float inv) {
+  *reinterpret_cast<uint2 *>(p) = make_uint2(pack2(x[0] * inv, x[1] * inv), pack2(x[2] * inv, x[3] * inv));
+}
+
+// kPair: a workgroup takes a (sequence, head unit), its waves equal shares of its
+// tiles, and stores the result.  Otherwise a wave takes a run of the line.
+template <int T, int D, bool kPair>
+__global__ __launch_bounds__(64 * (kPair ? kPairWaves : kWaves), 2) void decode_kernel(const DecodeArgs a) {
+  using L = CacheTile<T, D>;
+  constexpr int kB = L::kBlocks, kC = D / 16, kW = kPair ? kPairWaves : kWaves;
+  __shared__ Shares<D, kW> shares;
+  const int lane = threadIdx.x & 63, g = lane >> 4, r = lane & 15;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int run = blockIdx.x * kW + wave;
+  const int tpp = scalar(a.cache.page_tokens / kTileTokens), nh = min(a.group, kHeads);
+
+  // What the wave works on: tiles t .. t + count - 1 of a sequence, for one head unit.
+  int b, n, tiles, kv, chunk, t;  // sequence, its length, its tiles, k/v head, chunk of its heads
+  Line line;
+  int at, end;              // this wave's units
+  int idx = 0;              // the lane of sequence b
+  bool together = kPair;    // the workgroup's waves hold shares of one (sequence, head unit)
+  bool whole = kPair;       // and no other wave does
+  if constexpr (kPair) {
+    const int units = a.cache.kv_heads * a.chunks, head = blockIdx.x % units;
+    b = blockIdx.x / units;
+    kv = head / a.chunks;
+    chunk = head - kv * a.chunks;
+    n = a.lengths[b];
+    tiles = Line::tiles_of(a, n);
+    if (tiles == 0) {
+      const uint32_t v = n > 0 ? 0x7FC07FC0u : 0u;  // tokens, but a table without pages: NaN
+      const int count = min(a.group - chunk * kHeads, kHeads);
+      for (int i = threadIdx.x; i < count * (D / 4); i += 64 * kW)
+        *reinterpret_cast<uint2 *>(a.out + b * a.so + (int64_t)(kv * a.group + chunk * kHeads + i / (D / 4)) * a.ho +
+                                   4 * (i % (D / 4))) = make_uint2(v, v);
       return;
     }
-    nx.t = 0;
-    if (++nx.chunk == a.chunks) {
-      nx.chunk = 0;
-      ++nx.kv;
-    }
-    if (nx.kv == a.cache.kv_heads) {
-      nx.kv = 0;
-      uint64_t more = __ballot(line.tiles > 0) & ~((2ull << idx) - 1);
-      while (more == 0) {
-        line.before += lane_of(line.upto, 63);
-        line.c0 += 64;
-        line.load(a, lane);
-        more = __ballot(line.tiles > 0);
+    at = t = tiles * wave / kW;
+    end = tiles * (wave + 1) / kW;
+  } else {
+    line.make(a, lane);
+    if (line.total == 0 || run >= line.runs) return;
+    at = line.start(run);
+    end = line.start(run + 1);
+    idx = line.seek(a, lane, at);
+    b = line.c0 + idx;
+    n = lane_of(line.n, idx);
+    tiles = lane_of(line.tiles, idx);
+    const int in = at - (line.before + lane_of(line.upto, idx) - tiles) * line.heads, head = scalar(in / tiles);
+    t = in - head * tiles;
+    kv = scalar(head / a.chunks);
+    chunk = head - kv * a.chunks;
+    const int u0 = at - t, u1 = u0 + tiles;
+    together = line.together(run, u0, u1);
+    whole = together && line.start(run & -kWaves) == u0 && line.start((run & -kWaves) + kWaves) == u1;
+  }
+  const int first = at;
+
+  // The sequence's page numbers page0 .. page0 + 63, one a lane, and the place of
+  // the tile that is fetched next.
+  int page0, page, in_page, numbers;
+  bool bad;  // a page is not one of the cache's, or the sequence is longer than its table
+  auto number_pages = [&]() {
+    numbers = a.table[b * a.table_stride + min(page0 + lane, a.max_pages - 1)];  // no branch: what follows stays uniform
+    asm volatile("" : "+v"(numbers));  // used here, so that the wait for it is here and not in every tile
+  };
+  auto fetch = [&](Tile<T, D> &to) {
+    const uint32_t id = (uint32_t)lane_of(numbers, page - page0);
+    const bool ok = id < a.pages;
+    bad |= !ok;
+    const int64_t place = ((int64_t)(ok ? id : 0) * a.cache.kv_heads + kv) * tpp + in_page;
+    to.load(a.cache.data + place * L::kBytes, lane);
+    __builtin_amdgcn_sched_barrier(0);  // requested before the tile at hand is waited for
+  };
+  auto advance = [&]() {
+    if (++in_page == tpp) {
+      in_page = 0;
+      if (++page == page0 + 64) {
+        page0 = page;
+        number_pages();
       }
-      idx = __builtin_ctzll(more);
-      nx.b = line.c0 + idx;
-      nx.tiles = lane_of(line.tiles, idx);
     }
-    page0 = page = in_page = 0;
-    number_pages();
   };
 
   bf16x8 qf[kB];
   f32x4 o[kC];  // O^T: this lane's head, columns 16 c + 4 g + 0..3
   float m, l;
-  bool bad = false;
-  auto begin = [&](const Unit &u) {
-    const int in = u.chunk * kHeads + r;
-    const __bf16 *p = a.q + u.b * a.sq + (int64_t)(u.kv * a.group + (in < a.group ? in : 0)) * a.hq;
+  auto begin = [&]() {
+    const int in = chunk * kHeads + r;
+    const __bf16 *p = a.q + b * a.sq + (int64_t)(kv * a.group + (in < a.group ? in : 0)) * a.hq;
 #pragma unroll
     for (int b = 0; b < kB; ++b) {
       uint32_t w[4];
@@ -306,10 +371,12 @@ __global__ __launch_bounds__(64 * kWaves, 2) void decode_kernel(const DecodeArgs
     for (int c = 0; c < kC; ++c) o[c] = f32x4{0.f, 0.f, 0.f, 0.f};
     m = -__FLT_MAX__;
     l = 0.f;
-    bad = false;
+    bad = n > a.max_pages * a.cache.page_tokens;
+#pragma unroll
+    for (int b = 0; b < kB; ++b) asm volatile("" : "+v"(qf[b]));  // waited for here, not in every tile
   };
 
-  auto compute = [&](Tile<T, D> &x, const Unit &u) {
+  auto compute = [&](Tile<T, D> &x, int tile) {
     f32x4 s[2];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -335,8 +402,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void decode_kernel(const DecodeArgs
         }
       }
     }
-    if (u.t + 1 == u.tiles) {  // tokens past the sequence's last: no weight, and no value or scale that could make 0 x NaN
-      const int over = min(a.lengths[u.b], a.max_pages * a.cache.page_tokens) - (u.tiles - 1) * kTileTokens;
+    if (tile + 1 == tiles) {  // tokens past the sequence's last: no weight, and no value or scale that could make 0 x NaN
+      const int over = n - (tiles - 1) * kTileTokens;
       uint32_t keep[4] = {0, 0, 0, 0};
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
@@ -399,72 +466,115 @@ __global__ __launch_bounds__(64 * kWaves, 2) void decode_kernel(const DecodeArgs
         }
       }
     }
-    bad |= u.bad;
   };
-  // the end of the run or of a (sequence, head)
-  const int nh = min(a.group, kHeads);
-  auto finish = [&](const Unit &u, int from) {
-    if (bad || a.lengths[u.b] > (int64_t)a.max_pages * a.cache.page_tokens) l = __builtin_nanf("");
+  // the tiles at hand are done: their sums, or the result if they were all
+  auto finish = [&](int from, int count) {
+    if (bad) l = __builtin_nanf("");
     l = column_add(l);
-    const int in = u.chunk * kHeads + r;
-    if (in >= a.group) return;
-    if (u.t + 1 == u.tiles && u.at - from + 1 == u.tiles) {
+    const int in = chunk * kHeads + r;
+    if (together) {
+      shares.put(wave, lane, o, m * a.scale, l);
+    } else if (count == tiles) {
       const float inv = 1.f / l;
-      __bf16 *p = a.out + u.b * a.so + (int64_t)(u.kv * a.group + in) * a.ho + 4 * g;
+      __bf16 *p = a.out + b * a.so + (int64_t)(kv * a.group + in) * a.ho + 4 * g;
+      if (in < a.group)
 #pragma unroll
-      for (int c = 0; c < kC; ++c)
-        *reinterpret_cast<uint2 *>(p + 16 * c) = make_uint2(pack2(o[c][0] * inv, o[c][1] * inv), pack2(o[c][2] * inv, o[c][3] * inv));
-      return;
+        for (int c = 0; c < kC; ++c) store4(p + 16 * c, o[c], inv);
+    } else {
+      float *rec = a.partial + (int64_t)(2 * run + (from != first)) * nh * (D + 4);
+      if (in < a.group) {
+#pragma unroll
+        for (int c = 0; c < kC; ++c) *reinterpret_cast<f32x4 *>(rec + r * D + 16 * c + 4 * g) = o[c];
+        if (g == 0) *reinterpret_cast<float2 *>(rec + nh * D + 2 * r) = make_float2(m * a.scale, l);
+      }
     }
-    float *rec = a.partial + (int64_t)(2 * run + (from != first)) * nh * (D + 4);
-#pragma unroll
-    for (int c = 0; c < kC; ++c)
-      *reinterpret_cast<f32x4 *>(rec + r * D + 16 * c + 4 * g) = o[c];
-    if (g == 0) *reinterpret_cast<float2 *>(rec + nh * D + 2 * r) = make_float2(m * a.scale, l);
   };
 
-  int from = first;  // where the (sequence, head) at hand began in this run
-  Unit cu = nx;
-  Tile<T, D> t0, t1;
-  fetch(t0);
-  cu.bad = nx.bad;
-  begin(cu);
-  // one unit: the next one's tile is requested, this one's taken in
-  auto step = [&](Tile<T, D> &now, Tile<T, D> &then) {
-    advance();
-    fetch(then);
-    compute(now, cu);
-    const bool over = cu.at + 1 == end;
-    if (over || cu.t + 1 == cu.tiles) {
-      finish(cu, from);
-      if (over) return false;
-      from = nx.at;
-      cu = nx;
-      begin(cu);
-    } else {
-      cu = nx;
+  while (at < end) {
+    const int count = min(tiles - t, end - at);
+    page = page0 = scalar(t / tpp);
+    in_page = t - page * tpp;
+    number_pages();
+    begin();
+    Tile<T, D> t0, t1;
+    fetch(t0);
+    // two tiles a turn, each fetched while the one before it is taken in; past the
+    // last the fetch repeats it (a branch there would make every wait one for all loads)
+    for (int i = 0;;) {
+      if (i + 1 < count) advance();
+      fetch(t1);
+      compute(t0, t + i);
+      if (++i == count) break;
+      if (i + 1 < count) advance();
+      fetch(t0);
+      compute(t1, t + i);
+      if (++i == count) break;
     }
-    return true;
-  };
-  while (step(t0, t1) && step(t1, t0)) {
+    finish(at, count);
+    at += count;
+    if constexpr (!kPair) {
+      if (at < end) {  // the sequence's next head unit, or the next sequence with tokens
+        t = 0;
+        if (++chunk == a.chunks) {
+          chunk = 0;
+          ++kv;
+        }
+        if (kv == a.cache.kv_heads) {
+          kv = 0;
+          uint64_t more = __ballot(line.tiles > 0) & ~((2ull << idx) - 1);
+          while (more == 0) {
+            line.before += lane_of(line.upto, 63);
+            line.c0 += 64;
+            line.load(a, lane);
+            more = __ballot(line.tiles > 0);
+          }
+          idx = __builtin_ctzll(more);
+          b = line.c0 + idx;
+          n = lane_of(line.n, idx);
+          tiles = lane_of(line.tiles, idx);
+        }
+      }
+    }
+  }
+  if constexpr (kPair)
+    if (first == end) {  // a share without tiles
+#pragma unroll
+      for (int c = 0; c < kC; ++c) o[c] = f32x4{0.f, 0.f, 0.f, 0.f};
+      shares.put(wave, lane, o, -__builtin_inff(), 0.f);
+    }
+  if (!together) return;
+  __syncthreads();
+  const int count = min(a.group - chunk * kHeads, kHeads);
+  for (int i = threadIdx.x; i < count * (D / 4); i += 64 * kW) {
+    const int head = i / (D / 4), col = i - head * (D / 4);
+    float top, sum;
+    const f32x4 x = shares.add(head, col, top, sum);
+    if (whole) {
+      store4(a.out + b * a.so + (int64_t)(kv * a.group + chunk * kHeads + head) * a.ho + 4 * col, x, 1.f / sum);
+    } else {
+      float *rec = a.partial + (int64_t)(2 * (run & -kWaves)) * nh * (D + 4);
+      *reinterpret_cast<f32x4 *>(rec + head * D + 4 * col) = x;
+      if (col == 0) *reinterpret_cast<float2 *>(rec + nh * D + 2 * head) = make_float2(top, sum);
+    }
   }
 }
 
 // A row's shares, added in the order of the line, each relative to its own
 // maximum; zeros for a sequence without tokens.  A workgroup a row: D / 4 threads
-// take 4 columns of every kLanes-th share.
+// take 4 columns of every kLanes-th share, kBatch loads in flight.
 template <int D>
 __global__ __launch_bounds__(256) void join_kernel(const DecodeArgs a) {
-  constexpr int kCols = D / 4, kLanes = 256 / kCols;
+  constexpr int kCols = D / 4, kLanes = 256 / kCols, kBatch = 4;
   __shared__ float red[kLanes][D + 2];
   const int lane = threadIdx.x & 63;
   const int b = blockIdx.x / a.heads, head = blockIdx.x - b * a.heads;
   const int col = threadIdx.x % kCols, part = threadIdx.x / kCols;
   __bf16 *out = a.out + b * a.so + (int64_t)head * a.ho;
-  Line line(a, lane);
-  const int tiles = Line::tiles_of(a, b);
+  Line line;
+  line.make(a, lane);
+  const int n = a.lengths[b], tiles = Line::tiles_of(a, n);
   if (tiles == 0) {
-    const uint32_t v = a.lengths[b] > 0 ? 0x7FC07FC0u : 0u;  // tokens, but a table without pages
+    const uint32_t v = n > 0 ? 0x7FC07FC0u : 0u;  // tokens, but a table without pages: NaN
     if (part == 0) *reinterpret_cast<uint2 *>(out + 4 * col) = make_uint2(v, v);
     return;
   }
@@ -475,24 +585,44 @@ __global__ __launch_bounds__(256) void join_kernel(const DecodeArgs a) {
   }
   const int kv = head / a.group, in = head - kv * a.group, nh = min(a.group, kHeads);
   const int u0 = (line.before + lane_of(line.upto, b - line.c0) - tiles) * line.heads + (kv * a.chunks + in / kHeads) * tiles;
-  const int run0 = line.run_of(u0), run1 = line.run_of(u0 + tiles - 1);
+  const int u1 = u0 + tiles, run0 = line.run_of(u0), run1 = line.run_of(u1 - 1);
   if (run0 == run1) return;  // stored whole
+  // Its records: those of the runs before the first workgroup that is within it,
+  // of each such workgroup, and of the runs after.
+  int w0 = (run0 + (line.start(run0) < u0) + kWaves - 1) / kWaves;
+  int w1 = min(line.runs, run1 + (line.start(run1 + 1) <= u1)) / kWaves;
+  if (w1 < w0) w0 = w1 = run1 / kWaves + 1;
+  const int before = min(w0 * kWaves, run1 + 1) - run0, groups = w1 - w0;
+  const int count = before + groups + max(0, run1 + 1 - max(w1 * kWaves, run0 + before));
+  if (groups == 1 && count == 1) return;  // stored whole by that workgroup
   const int64_t stride = (int64_t)nh * (D + 4);
-  auto record = [&](int run) { return a.partial + (2 * run + (line.start(run) < u0)) * stride; };
+  auto record = [&](int i) {
+    const int run = i < before ? run0 + i : i < before + groups ? (w0 + i - before) * kWaves : w1 * kWaves + i - before - groups;
+    return a.partial + (2 * run + (line.start(run) < u0)) * stride;
+  };
   const int row = in % kHeads;
   float m = -__builtin_inff(), l = 0.f;
   f32x4 o{0.f, 0.f, 0.f, 0.f};
-  for (int run = run0 + part; run <= run1; run += kLanes) {
-    const float *rec = record(run);
-    const f32x4 v = *reinterpret_cast<const f32x4 *>(rec + row * D + 4 * col);
-    const float2 ml = *reinterpret_cast<const float2 *>(rec + nh * D + 2 * row);
-    const float top = __builtin_fmaxf(m, ml.x);
-    const float f = m == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(m - top);
-    const float e = ml.x == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(ml.x - top);
-    m = top;
-    l = l * f + ml.y * e;
+  for (int i = part; i < count; i += kLanes * kBatch) {
+    f32x4 v[kBatch];
+    float2 ml[kBatch];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) o[i] = o[i] * f + v[i] * e;
+    for (int k = 0; k < kBatch; ++k) {
+      const float *rec = record(min(i + k * kLanes, count - 1));
+      v[k] = *reinterpret_cast<const f32x4 *>(rec + row * D + 4 * col);
+      ml[k] = *reinterpret_cast<const float2 *>(rec + nh * D + 2 * row);
+    }
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k) {
+      if (i + k * kLanes >= count) break;
+      const float top = __builtin_fmaxf(m, ml[k].x);
+      const float f = m == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(m - top);
+      const float e = ml[k].x == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(ml[k].x - top);
+      m = top;
+      l = l * f + ml[k].y * e;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) o[c] = o[c] * f + v[k][c] * e;
+    }
   }
 #pragma unroll
   for (int i = 0; i < 4; ++i) red[part][4 * col + i] = o[i];
@@ -520,6 +650,11 @@ int invalid(const char *msg) { return set_error(MQ_E_INVALID, msg); }
 
 int chunks_of(int heads, int kv_heads) { return (heads / kv_heads + kHeads - 1) / kHeads; }
 
+// Whether a workgroup takes each (sequence, head unit): up to kPairTiles tiles of
+// a sequence, by what its page table can hold, which is all the host knows.
+constexpr int64_t kPairTiles = 32;
+bool by_pairs(const mq_kv_cache *c, int64_t max_pages) { return max_pages * (c->page_tokens / kTileTokens) <= kPairTiles; }
+
 // Waves of a launch over `batch` sequences of up to `tokens` tokens: a run each, and no more than the tiles there can be.
 int waves_of(int64_t batch, int kv_heads, int chunks, int64_t tokens) {
   const int64_t units = batch * kv_heads * chunks * ((tokens + kTileTokens - 1) / kTileTokens);
@@ -532,7 +667,8 @@ int waves_of(int64_t batch, int kv_heads, int chunks, int64_t tokens) {
 
 extern "C" size_t mq_cache_attention_scratch_size(const mq_kv_cache *c, int64_t batch, int heads, int64_t max_pages) {
   using namespace mq;
-  if (cache_fault(c) || batch <= 0 || heads < 1 || heads % c->kv_heads || max_pages <= 0) return 0;
+  if (cache_fault(c) || batch <= 0 || heads < 1 || heads % c->kv_heads || max_pages <= 0 || by_pairs(c, max_pages))
+    return 0;
   const int group = heads / c->kv_heads;
   return (size_t)2 * waves_of(batch, c->kv_heads, chunks_of(heads, c->kv_heads), max_pages * c->page_tokens) *
          (group < kHeads ? group : kHeads) * (c->head_dim + 4) * sizeof(float);
@@ -573,7 +709,8 @@ extern "C" int mq_cache_attention(const mq_kv_cache *c, const void *q, int64_t q
   const uintptr_t q1 = q0 + 2 * (uintptr_t)((batch - 1) * q_batch_stride + (heads - 1) * q_head_stride + dim);
   const uintptr_t o1 = o0 + 2 * (uintptr_t)((batch - 1) * out_batch_stride + (heads - 1) * out_head_stride + dim);
   if (q0 < o1 && o0 < q1) return invalid("mq_cache_attention: out lies over q");
-  if (scratch_bytes < mq_cache_attention_scratch_size(c, batch, heads, max_pages) || (max_pages && !scratch))
+  const size_t need = mq_cache_attention_scratch_size(c, batch, heads, max_pages);
+  if (need && (!scratch || scratch_bytes < need))
     return invalid("mq_cache_attention: scratch below mq_cache_attention_scratch_size");
   const int waves = waves_of(batch, c->kv_heads, chunks, max_pages * c->page_tokens);
   const DecodeArgs a{{static_cast<uint8_t *>(c->data), c->pages * c->page_tokens, c->page_tokens, c->kv_heads}, c->pages,
@@ -582,8 +719,12 @@ extern "C" int mq_cache_attention(const mq_kv_cache *c, const void *q, int64_t q
                      heads, heads / c->kv_heads, chunks, waves, scale * 1.44269504f, static_cast<float *>(scratch)};
   hipStream_t s = static_cast<hipStream_t>(stream);
   with_cache_type(c, [&]<int T, int D>() {
-    if (waves) hipLaunchKernelGGL((decode_kernel<T, D>), dim3((unsigned)(waves / kWaves)), dim3(64 * kWaves), 0, s, a);
-    hipLaunchKernelGGL(join_kernel<D>, dim3((unsigned)(batch * heads)), dim3(256), 0, s, a);
+    if (by_pairs(c, max_pages)) {
+      hipLaunchKernelGGL((decode_kernel<T, D, true>), dim3((unsigned)(batch * c->kv_heads * chunks)), dim3(64 * kPairWaves), 0, s, a);
+    } else {
+      hipLaunchKernelGGL((decode_kernel<T, D, false>), dim3((unsigned)(waves / kWaves)), dim3(64 * kWaves), 0, s, a);
+      hipLaunchKernelGGL(join_kernel<D>, dim3((unsigned)(batch * heads)), dim3(256), 0, s, a);
+    }
   });
   const hipError_t e = hipGetLastError();
   return e == hipSuccess ? MQ_OK : set_error(MQ_E_HIP, hipGetErrorString(e));

@@ -23,19 +23,32 @@ from .fused import recorded
 from .quantized import GgmlDType, _dtype_code, _stream_ptr
 
 _MAX_STRIDE = 1 << 24
+_BF16 = torch.bfloat16
 
 
-def _on(device):
-    """The device made current, unless it is."""
-    return torch.cuda.device(device)
+def _run(device, fn, *args):
+    """fn(*args, torch's current stream) with `device` current, as it mostly is (making it so
+    takes 1.3 us of a 9 us call)."""
+    if torch._C._cuda_getDevice() == device.index:
+        rc = fn(*args, _stream_ptr())
+    else:
+        with torch.cuda.device(device):
+            rc = fn(*args, _stream_ptr())
+    if rc:
+        check(rc)
 
 
-def _heads_view(name, t, heads, dim, device):
-    """t as the library reads it: bf16 [tokens, heads, dim] on `device` with unit stride along
-    the head, 16-byte rows and strides; copied if it is anything else of that shape."""
-    if t.dtype is not torch.bfloat16 or t.dim() != 3 or t.shape[1] != heads or t.shape[2] != dim or t.device != device:
-        raise ValueError(f"{name} must be bf16 [tokens, {heads}, {dim}] on {device}")
-    return t if _readable(t) else t.contiguous()
+def _operand(name, t, shape, device):
+    """t as the library reads it, with its token and head stride: bf16 `shape` = (tokens, heads,
+    dim) on `device`; copied unless it has unit stride along the head and 16-byte rows."""
+    if t.dtype is not _BF16 or t.shape != shape or t.device != device:
+        raise ValueError(f"{name} must be bf16 {list(shape)} on {device}")
+    st, sh, sd = t.stride()
+    if sd != 1 or (st | sh) & 7 or st >= _MAX_STRIDE or sh >= _MAX_STRIDE or t.data_ptr() & 15:
+        if not _readable(t):
+            t = t.contiguous()
+        st, sh = _strides(t)
+    return t, st, sh
 
 
 def _readable(t):
@@ -75,22 +88,23 @@ def _apart(out, t):
 
 
 def _out(name, out, shape, device, inputs):
-    """The tensor to write: `out`, or a temporary where the kernel cannot store into it (another
-    device, unaligned or overlapping rows, over an input that other workgroups still read)."""
-    if out is None:
-        return torch.empty(shape, dtype=torch.bfloat16, device=device)
-    if out.dtype is not torch.bfloat16 or tuple(out.shape) != tuple(shape):
-        raise ValueError(f"{name}: out must be bf16 {list(shape)}")
-    if out.device == device and _writable(out) and all(_apart(out, t) for t in inputs):
-        return out
-    return torch.empty(shape, dtype=torch.bfloat16, device=device)
+    """The tensor to write and its strides: `out`, or a temporary where the kernel cannot store
+    into it (another device, unaligned or overlapping rows, over an input that other workgroups
+    still read)."""
+    if out is not None:
+        if out.dtype is not _BF16 or tuple(out.shape) != tuple(shape):
+            raise ValueError(f"{name}: out must be bf16 {list(shape)}")
+        if out.device == device and _writable(out) and all(_apart(out, t) for t in inputs):
+            return out, *_strides(out)
+    return torch.empty(shape, dtype=_BF16, device=device), shape[1] * shape[2], shape[2]
 
 
 def _given(out, res):
-    if out is None or res is out:
-        if out is not None:
-            torch.autograd.graph.increment_version(out)     # written in place, as a copy_ tells autograd
+    if out is None:
         return res
+    if res is out:
+        torch.autograd.graph.increment_version(out)     # written in place, as a copy_ tells autograd
+        return out
     return out.copy_(res)
 
 
@@ -110,30 +124,29 @@ class PromptPlan:
         check(lib.mq_prompt_plan_make(*args, tiles.ctypes.data_as(ctypes.POINTER(ctypes.c_int32)), len(tiles)))
         self.tiles = torch.from_numpy(tiles).to(device)
         self.device = self.tiles.device
+        if self.device.type != "cuda":
+            raise ValueError(f"PromptPlan: a GPU's, not {self.device}")
         self.tokens = int(self.c.tokens)
         self.heads, self.kv_heads, self.head_dim = int(heads), int(kv_heads), int(head_dim)
-        self._ref = ctypes.byref(self.c)
+        self.q_shape = (self.tokens, self.heads, self.head_dim)
+        self.kv_shape = (self.tokens, self.kv_heads, self.head_dim)
+        self._ref, self._tiles = ctypes.byref(self.c), self.tiles.data_ptr()
 
 
 def prompt_attention(q, k, v, plan: PromptPlan, scale=None, out=None):
     """Causal attention inside each of the plan's prompts: q bf16 [tokens, heads, dim], k and v
     bf16 [tokens, kv_heads, dim] (views of one projection's output are read in place) ->
     bf16 [tokens, heads, dim], `out` if given.  scale defaults to dim ** -0.5."""
-    dim, device = plan.head_dim, plan.device
+    device, n = plan.device, plan.tokens
     if recorded(q, k, v):
         raise ValueError("prompt_attention: inference only, nothing may record the call")
-    q = _heads_view("prompt_attention: q", q, plan.heads, dim, device)
-    k = _heads_view("prompt_attention: k", k, plan.kv_heads, dim, device)
-    v = _heads_view("prompt_attention: v", v, plan.kv_heads, dim, device)
-    n = plan.tokens
-    if not q.shape[0] == k.shape[0] == v.shape[0] == n:
-        raise ValueError(f"prompt_attention: q, k and v must have the plan's {n} tokens")
-    res = _out("prompt_attention", out, q.shape, device, (q, k, v))
+    q, qt, qh = _operand("prompt_attention: q", q, plan.q_shape, device)
+    k, kt, kh = _operand("prompt_attention: k", k, plan.kv_shape, device)
+    v, vt, vh = _operand("prompt_attention: v", v, plan.kv_shape, device)
+    res, ot, oh = _out("prompt_attention", out, plan.q_shape, device, (q, k, v))
     if n:
-        with _on(device):
-            check(_lib.load().mq_prompt_attention(
-                plan._ref, plan.tiles.data_ptr(), q.data_ptr(), *_strides(q), k.data_ptr(), *_strides(k), v.data_ptr(),
-                *_strides(v), dim ** -0.5 if scale is None else scale, res.data_ptr(), *_strides(res), _stream_ptr()))
+        _run(device, _lib.load().mq_prompt_attention, plan._ref, plan._tiles, q.data_ptr(), qt, qh, k.data_ptr(), kt, kh,
+             v.data_ptr(), vt, vh, plan.head_dim ** -0.5 if scale is None else scale, res.data_ptr(), ot, oh)
     return _given(out, res)
 
 
@@ -154,6 +167,8 @@ class KvCache:
         self.data = torch.empty(size, dtype=torch.uint8, device=device)
         self.c.data = self.data.data_ptr()
         self.device = self.data.device
+        if self.device.type != "cuda":
+            raise ValueError(f"KvCache: a GPU's, not {self.device}")
         self.pages, self.kv_heads, self.head_dim, self.page_tokens = int(pages), int(kv_heads), int(head_dim), int(page_tokens)
         self.dtype = GgmlDType(dtype)
 
@@ -176,21 +191,26 @@ class KvCache:
             raise ValueError("KvCache.append: inference only, nothing may record the call")
         slots = self._slots("KvCache.append", slots)
         n = slots.shape[0]
-        parts = []
-        for t in (k, v):
-            if t.dtype not in (torch.bfloat16, torch.float32) or t.dtype != k.dtype or t.device != self.device \
-                    or tuple(t.shape) != (n, self.kv_heads, self.head_dim):
-                raise ValueError("KvCache.append: k and v must be bf16 or f32 "
-                                 f"[{n}, {self.kv_heads}, {self.head_dim}] on {self.device}")
-            unit = 16 // t.element_size()
-            st, sh = _strides(t)
-            parts.append(t if t.stride(2) == 1 and t.data_ptr() % 16 == 0 and st % unit == 0 and sh % unit == 0
-                         else t.contiguous())
-        k, v = parts
+        shape, dtype = (n, self.kv_heads, self.head_dim), k.dtype
+        if dtype not in (_BF16, torch.float32):
+            raise ValueError("KvCache.append: k and v must be bf16 or f32")
+        k, kt, kh = self._rows(k, shape, dtype)
+        v, vt, vh = self._rows(v, shape, dtype)
         if n:
-            with _on(self.device):
-                check(_lib.load().mq_kv_cache_append(self._ref, k.data_ptr(), *_strides(k), v.data_ptr(), *_strides(v),
-                                                     _dtype_code(k.dtype), n, slots.data_ptr(), _stream_ptr()))
+            _run(self.device, _lib.load().mq_kv_cache_append, self._ref, k.data_ptr(), kt, kh, v.data_ptr(), vt, vh,
+                 _dtype_code(dtype), n, slots.data_ptr())
+
+    def _rows(self, t, shape, dtype):
+        if t.dtype is not dtype or t.shape != shape or t.device != self.device:
+            raise ValueError(f"KvCache.append: k and v must be {list(shape)} of one type on {self.device}")
+        st, sh, sd = t.stride()
+        mask = 7 if dtype is _BF16 else 3
+        if sd != 1 or (st | sh) & mask or t.data_ptr() & 15:
+            st, sh = _strides(t)
+            if sd != 1 or (st | sh) & mask or t.data_ptr() & 15:
+                t = t.contiguous()
+                st, sh = _strides(t)
+        return t, st, sh
 
     def read(self, slots, dtype=torch.bfloat16):
         """(k, v) [tokens, kv_heads, head_dim] of `slots`, bf16 or f32; zeros for a slot outside the cache."""
@@ -200,9 +220,8 @@ class KvCache:
         shape = (slots.shape[0], self.kv_heads, self.head_dim)
         k, v = (torch.empty(shape, dtype=dtype, device=self.device) for _ in range(2))
         if shape[0]:
-            with _on(self.device):
-                check(_lib.load().mq_kv_cache_read(self._ref, slots.data_ptr(), shape[0], k.data_ptr(), v.data_ptr(),
-                                                   _dtype_code(dtype), _stream_ptr()))
+            _run(self.device, _lib.load().mq_kv_cache_read, self._ref, slots.data_ptr(), shape[0], k.data_ptr(), v.data_ptr(),
+                 _dtype_code(dtype))
         return k, v
 
     def attend(self, q, page_table, lengths, scale=None, out=None):
@@ -216,23 +235,21 @@ class KvCache:
         if q.dim() != 3 or q.shape[1] == 0 or q.shape[1] % self.kv_heads:
             raise ValueError(f"KvCache.attend: q must be [batch, heads, {dim}] with a multiple of {self.kv_heads} heads")
         n, heads, _ = q.shape
-        q = _heads_view("KvCache.attend: q", q, heads, dim, device)
+        q, qb, qh = _operand("KvCache.attend: q", q, (n, heads, dim), device)
         for name, t, dims in (("page_table", page_table, 2), ("lengths", lengths, 1)):
             if t.dtype is not torch.int32 or t.dim() != dims or t.shape[0] != n or t.device != device:
                 raise ValueError(f"KvCache.attend: {name} must be int32 [{n}{', pages' if dims == 2 else ''}] on {device}")
         pages = page_table.shape[1]
         if n > 1 and page_table.stride(0) < pages or pages > 1 and page_table.stride(1) != 1:
             page_table = page_table.contiguous()
-        lengths = lengths if lengths.is_contiguous() else lengths.contiguous()
-        res = _out("KvCache.attend", out, q.shape, device, (q,))
+        if not lengths.is_contiguous():
+            lengths = lengths.contiguous()
+        res, ob, oh = _out("KvCache.attend", out, (n, heads, dim), device, (q,))
         if n:
             lib = _lib.load()
-            with _on(device):
-                nbytes = lib.mq_cache_attention_scratch_size(self._ref, n, heads, pages)
-                scratch = torch.empty(nbytes, dtype=torch.uint8, device=device)     # freed to this stream
-                check(lib.mq_cache_attention(
-                    self._ref, q.data_ptr(), *_strides(q), n, heads, page_table.data_ptr(),
-                    page_table.stride(0) if n > 1 else pages, pages, lengths.data_ptr(),
-                    dim ** -0.5 if scale is None else scale, res.data_ptr(), *_strides(res), scratch.data_ptr(), nbytes,
-                    _stream_ptr()))
+            nbytes = lib.mq_cache_attention_scratch_size(self._ref, n, heads, pages)
+            scratch = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None     # freed to this stream
+            _run(device, lib.mq_cache_attention, self._ref, q.data_ptr(), qb, qh, n, heads, page_table.data_ptr(),
+                 page_table.stride(0) if n > 1 else pages, pages, lengths.data_ptr(), dim ** -0.5 if scale is None else scale,
+                 res.data_ptr(), ob, oh, scratch.data_ptr() if nbytes else None, nbytes)
         return _given(out, res)

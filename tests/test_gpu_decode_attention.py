@@ -285,20 +285,21 @@ def test_argument_checks():
     for kw in (dict(c=_cache(dtype=12)), dict(c=_cache(data=None)), dict(c=_cache(pages=0)), dict(c=_cache(data=4100)), dict(q=None), dict(q=4100),
                dict(qs=(252, 64)), dict(qs=(-256, 64)), dict(batch=-1), dict(heads=0), dict(heads=5), dict(table=None), dict(ts=3), dict(pages=-1),
                dict(pages=1 << 31, ts=1 << 31), dict(pages=1 << 26, ts=1 << 26), dict(lengths=None), dict(lengths=4098), dict(scale=0.0),
-               dict(scale=float("nan")), dict(out=None), dict(out=4096 + 1024), dict(os=(128, 64)), dict(os=(256, 32)), dict(scratch=None),
-               dict(size=100), dict(batch=1 << 30)):
+               dict(scale=float("nan")), dict(out=None), dict(out=4096 + 1024), dict(os=(128, 64)), dict(os=(256, 32)),
+               dict(scratch=None, pages=64, ts=64), dict(size=100, pages=64, ts=64), dict(batch=1 << 30)):
         assert call(**kw) == -1, kw
     with pytest.raises(MoldqError):
         _lib.check(call(q=None))
     assert call(batch=0, q=None, lengths=None) == 0
     assert lib.mq_cache_attention(None, None, 0, 0, 0, 1, None, 0, 0, None, 1.0, None, 0, 0, None, 0, None) == -1
     size = lib.mq_cache_attention_scratch_size
-    assert size(None, 1, 4, 4) == 0 and size(ctypes.byref(_cache()), 0, 4, 4) == 0 and size(ctypes.byref(_cache()), 1, 4, 4) > 0
+    assert size(None, 1, 4, 4) == 0 and size(ctypes.byref(_cache()), 0, 4, 4) == 0 and size(ctypes.byref(_cache()), 1, 4, 64) > 0
+    assert size(ctypes.byref(_cache()), 1, 4, 4) == 0      # a workgroup takes a whole head: no shares to join
 
 
 @pytest.mark.skipif(HIPCC is None, reason="hipcc not available")
 def test_kernels_do_not_spill(tmp_path):
     funcs = {k: v for k, v in _functions(_asm(tmp_path, "mq_decode.hip")).items() if "_kernel" in k}
-    assert len(funcs) == 8
+    assert len(funcs) == 14
     for name, (_, meta) in funcs.items():
         assert meta.get("ScratchSize", 0) == 0, (name, meta)
