@@ -309,7 +309,7 @@ size_t mq_attention_scratch_size(int64_t batch, int heads, int64_t valid);
  * or 128, lengths >= 0 (a prompt of no tokens has no rows). */
 typedef struct mq_prompt_plan {
     int64_t tokens, tiles;
-    int32_t heads, kv_heads, head_dim, tile_tokens, waves;
+    int32_t heads, kv_heads, head_dim, tile_tokens, parts;
 } mq_prompt_plan;
 int mq_prompt_plan_make(const int64_t *lengths, int64_t count, int heads, int kv_heads, int head_dim,
                         mq_prompt_plan *plan, int32_t *tiles, int64_t capacity);

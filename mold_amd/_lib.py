@@ -29,7 +29,7 @@ MQ_LORA_MAX_PATCHES = 8
 class PromptPlanC(ctypes.Structure):
     """mq_prompt_plan"""
     _fields_ = [("tokens", ctypes.c_int64), ("tiles", ctypes.c_int64)] + [
-        (f, ctypes.c_int32) for f in ("heads", "kv_heads", "head_dim", "tile_tokens", "waves")]
+        (f, ctypes.c_int32) for f in ("heads", "kv_heads", "head_dim", "tile_tokens", "parts")]
 
 
 class KvCacheC(ctypes.Structure):

@@ -64,15 +64,17 @@ __device__ __forceinline__ bool any_not_finite(const uint4 &u) {
   return odd;
 }
 
-template <int D, int W>
+// W waves of 32 queries each; with P = 2 two waves share their queries and take
+// every other 32 keys each.
+template <int D, int W, int P>
 __global__ __launch_bounds__(64 * W, D == 128 ? 2 : 3) void prompt_kernel(const PromptArgs a) {
   constexpr int kRow = 2 * D;              // bytes of a row in LDS
   constexpr int kBlock = kKeys * kRow;     // of a block
   constexpr int kChunks = kRow / 16;       // 16-byte chunks of a row
   constexpr int kDmaRows = 1024 / kRow;    // rows a wave's DMA instruction fills
   constexpr int kDmas = kKeys / kDmaRows / W;
-  __shared__ uint4 lds_k[2][kBlock / 16];
-  __shared__ uint4 lds_v[3][kBlock / 16];
+  __shared__ uint4 lds[5 * kBlock / 16];  // K blocks 0 and 1, V blocks 0 to 2
+  uint4 *const lds_k = lds, *const lds_v = lds + 2 * kBlock / 16;
 
   const int4 tile = a.tiles[blockIdx.x / a.units];
   const int unit = blockIdx.x % a.units;
@@ -82,11 +84,12 @@ __global__ __launch_bounds__(64 * W, D == 128 ? 2 : 3) void prompt_kernel(const 
 
   const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, h = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int head = (unit << a.log_heads) + (wave & ((1 << a.log_heads) - 1));
-  const int tok0 = first + 32 * (wave >> a.log_heads);
-  const int end = min(first + ((32 * W) >> a.log_heads), len);  // past the tile's last token
+  const int slot = wave / P, part = P == 1 ? 0 : wave % P;  // which 32 queries, which keys of theirs
+  const int head = (unit << a.log_heads) + (slot & ((1 << a.log_heads) - 1));
+  const int tok0 = first + 32 * (slot >> a.log_heads);
+  const int end = min(first + ((32 * W / P) >> a.log_heads), len);  // past the tile's last token
   const int nblk = (end + kKeys - 1) / kKeys;
-  const int halves = tok0 < len ? tok0 / 32 + 1 : 0;  // 32-key halves this wave computes; the last is its diagonal
+  const int halves = tok0 < len ? tok0 / 32 + 1 : 0;  // 32-key halves these queries see; the last is their diagonal
   const int row = tok0 + l32;                         // this lane's query
   const int64_t kvhead = (unit << a.log_heads) / a.group;
 
@@ -104,8 +107,8 @@ __global__ __launch_bounds__(64 * W, D == 128 ? 2 : 3) void prompt_kernel(const 
   const int drow = kDmaRows * wave + lane / kChunks, dch = lane % kChunks;
   const int dk = D == 128 ? drow & 15 : (drow >> 1) & 7, dv = D == 128 ? drow & 3 : (drow >> 1) & 1;
   const uint32_t kch = (uint32_t)((dch ^ dk) << 4), vch = (uint32_t)((dch ^ (dv << 2)) << 4);
-  const uint32_t lkw = (uint32_t)(uintptr_t)(&lds_k[0][0]) + 1024 * wave;
-  const uint32_t lvw = (uint32_t)(uintptr_t)(&lds_v[0][0]) + 1024 * wave;
+  const uint32_t lkw = (uint32_t)(uintptr_t)(lds_k) + 1024 * wave;
+  const uint32_t lvw = (uint32_t)(uintptr_t)(lds_v) + 1024 * wave;
   const char *kbase = reinterpret_cast<const char *>(a.k + tile.x * a.sk + kvhead * a.hk);
   const char *vbase = reinterpret_cast<const char *>(a.v + tile.x * a.sv + kvhead * a.hv);
   const uint32_t kstep = (uint32_t)(2 * a.sk), vstep = (uint32_t)(2 * a.sv);
@@ -132,11 +135,12 @@ __global__ __launch_bounds__(64 * W, D == 128 ? 2 : 3) void prompt_kernel(const 
   {
     const int fk = D == 128 ? l32 & 15 : (l32 >> 1) & 7, fv = D == 128 ? i16 >> 2 : i16 >> 3;
 #pragma unroll
-    for (int s = 0; s < D / 16; ++s) ka[s] = (lds_char *)&lds_k[0][0] + (uint32_t)(l32 * kRow + (((2 * s + h) ^ fk) << 4));
+    for (int s = 0; s < D / 16; ++s)
+      ka[s] = (lds_char *)lds_k + (uint32_t)((32 * part + l32) * kRow + (((2 * s + h) ^ fk) << 4));
 #pragma unroll
     for (int d = 0; d < D / 32; ++d)
-      va[d] = (lds_char *)&lds_v[0][0] +
-              (uint32_t)((4 * h + (i16 >> 2)) * kRow + ((d ^ fv) << 6) + 32 * ((lane >> 4) & 1) + 8 * (i16 & 3));
+      va[d] = (lds_char *)lds_v +
+              (uint32_t)((32 * part + 4 * h + (i16 >> 2)) * kRow + ((d ^ fv) << 6) + 32 * ((lane >> 4) & 1) + 8 * (i16 & 3));
   }
 
   // scores of keys 32 kb .. + 31 of the block in K slot `slot`: lane l32's
@@ -150,11 +154,12 @@ __global__ __launch_bounds__(64 * W, D == 128 ? 2 : 3) void prompt_kernel(const 
       s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x, qf[i], s, 0, 0, 0);
     }
   };
-  // the diagonal half: its keys tok0 + 0 .. 31 against rows tok0 + l32
-  auto mask = [&](f32x16 &s) {
+  // a half of which row l32 sees the keys 0 .. seen (l32 on the diagonal, 31 of any
+  // half before it)
+  auto mask = [&](f32x16 &s, int seen) {
 #pragma unroll
     for (int e = 0; e < 16; ++e)
-      if (8 * (e >> 2) + 4 * h + (e & 3) > l32) s[e] = -__builtin_inff();
+      if (8 * (e >> 2) + 4 * h + (e & 3) > seen) s[e] = -__builtin_inff();
   };
   auto max16 = [&](const f32x16 &s) {
     float r = s[0];
@@ -222,7 +227,7 @@ __global__ __launch_bounds__(64 * W, D == 128 ? 2 : 3) void prompt_kernel(const 
   // The diagonal half, whose V holds a value that is not finite: the finite
   // values by their probabilities as ever, and for each row the infinities and
   // NaN (which count as both) that it sees, counted by products with its mask.
-  auto accumulate_seen = [&](int slot, int kb, const bf16x8 *p) {
+  auto accumulate_seen = [&](int slot, int kb, int last, const bf16x8 *p) {
     bf16x8 seen[2];
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
@@ -230,45 +235,48 @@ __global__ __launch_bounds__(64 * W, D == 128 ? 2 : 3) void prompt_kernel(const 
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int key = 16 * t + 8 * (i >> 1) + 4 * h + 2 * (i & 1);
-        u[i] = (key <= l32 ? 0x3F80u : 0u) | (key + 1 <= l32 ? 0x3F800000u : 0u);
+        u[i] = (key <= last ? 0x3F80u : 0u) | (key + 1 <= last ? 0x3F800000u : 0u);
       }
       __builtin_memcpy(&seen[t], u, 16);
     }
+    // pass by pass and one tile of columns at a time, each reading V anew: together
+    // they would spill
+    auto classes = [&](int t, int d, auto pick) {
+      asm volatile("" ::: "memory");
+      const uint4 v4 = values(slot, kb, t, d);
+      const uint32_t w[4] = {v4.x, v4.y, v4.z, v4.w};
+      uint32_t u[4];
 #pragma unroll
-    for (int d = 0; d < D / 32; ++d) {
-      f32x16 up, down;
+      for (int i = 0; i < 4; ++i) u[i] = pick(w[i] & 0xFFFFu) | pick(w[i] >> 16) << 16;
+      return as_bf16(make_uint4(u[0], u[1], u[2], u[3]));
+    };
+    auto finite = [](uint32_t x) { return (x & 0x7F80u) != 0x7F80u; };
 #pragma unroll
-      for (int e = 0; e < 16; ++e) up[e] = down[e] = 0.f;
+    for (int d = 0; d < D / 32; ++d)
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        const uint4 v4 = values(slot, kb, t, d);
-        const uint32_t w[4] = {v4.x, v4.y, v4.z, v4.w};
-        uint32_t fine[4], pos[4], neg[4];
+      for (int t = 0; t < 2; ++t)
+        o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(classes(t, d, [&](uint32_t x) { return finite(x) ? x : 0u; }), p[t], o[d], 0, 0, 0);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          fine[i] = pos[i] = neg[i] = 0;
+    for (int d = 0; d < D / 32; ++d)
 #pragma unroll
-          for (int b = 0; b < 32; b += 16) {
-            const uint32_t x = (w[i] >> b) & 0xFFFFu;
-            const bool ok = (x & 0x7F80u) != 0x7F80u, nan = !ok && (x & 0x7Fu);
-            fine[i] |= ok ? x << b : 0u;
-            pos[i] |= !ok && (nan || !(x & 0x8000u)) ? 0x3F80u << b : 0u;
-            neg[i] |= !ok && (nan || (x & 0x8000u)) ? 0x3F80u << b : 0u;
-          }
-        }
-        o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf16(make_uint4(fine[0], fine[1], fine[2], fine[3])), p[t], o[d], 0, 0, 0);
-        up = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf16(make_uint4(pos[0], pos[1], pos[2], pos[3])), seen[t], up, 0, 0, 0);
-        down = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf16(make_uint4(neg[0], neg[1], neg[2], neg[3])), seen[t], down, 0, 0, 0);
+      for (uint32_t sign = 0; sign <= 0x8000u; sign += 0x8000u) {
+        f32x16 count;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) count[e] = 0.f;
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+          count = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+              classes(t, d, [&](uint32_t x) { return !finite(x) && ((x & 0x7Fu) || (x & 0x8000u) == sign) ? 0x3F80u : 0u; }), seen[t], count,
+              0, 0, 0);
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          if (count[e] > 0.f) o[d][e] += sign ? -__builtin_inff() : __builtin_inff();
+        __builtin_amdgcn_sched_barrier(0);
       }
-#pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        if (up[e] > 0.f) o[d][e] += __builtin_inff();
-        if (down[e] > 0.f) o[d][e] -= __builtin_inff();
-      }
-    }
   };
-  auto diagonal = [&](int slot, int kb, f32x16 &s, bf16x8 *p) {
-    mask(s);
+  auto diagonal = [&](int slot, int kb, int last, f32x16 &s) {
+    bf16x8 p[2];
+    mask(s, last);
     raise_max(max16(s));
     probs(s, p);
     bool odd = false;
@@ -276,7 +284,7 @@ __global__ __launch_bounds__(64 * W, D == 128 ? 2 : 3) void prompt_kernel(const 
     for (int t = 0; t < 2; ++t)
 #pragma unroll
       for (int d = 0; d < D / 32; ++d) odd = any_not_finite(values(slot, kb, t, d)) || odd;
-    if (__any(odd)) accumulate_seen(slot, kb, p);
+    if (__any(odd)) accumulate_seen(slot, kb, last, p);
     else accumulate(slot, kb, p);
   };
 
@@ -284,7 +292,7 @@ __global__ __launch_bounds__(64 * W, D == 128 ? 2 : 3) void prompt_kernel(const 
   block_barrier();
   if (nblk > 1) dma(1, 1, 1);
   f32x16 s0, s1;
-  if (halves) scores(0, 0, s0);
+  if (halves > part) scores(0, 0, s0);
   int vs = 0;  // V slot of block i
   // The barrier in the middle of block i says that block i + 1 has landed and
   // that every wave has read all of K(i) and V(i - 1), whose slots block i + 2
@@ -296,42 +304,73 @@ __global__ __launch_bounds__(64 * W, D == 128 ? 2 : 3) void prompt_kernel(const 
       if (i + 2 < nblk) dma(i + 2, ks, vs == 0 ? 2 : vs - 1);
     }
   };
-  // a block whose keys are all seen and that is not the wave's last; its first half's scores are in s0
-  auto full = [&](int i, auto kslot) {
-    constexpr int ks = decltype(kslot)::v;
-    bf16x8 p[2];
-    raise_max(max16(s0));
-    scores(ks, 1, s1);
-    probs(s0, p);
-    accumulate(vs, 0, p);
-    const float mx = max16(s1);
-    turn(i, ks);
-    raise_max(mx);
-    scores(ks ^ 1, 0, s0);
-    probs(s1, p);
-    accumulate(vs, 1, p);
-    vs = vs == 2 ? 0 : vs + 1;
-  };
   int i = 0;
-  for (; 2 * i + 4 < halves; i += 2) {
-    full(i, Slot<0>{});
-    full(i + 1, Slot<1>{});
-  }
-  if (2 * i + 2 < halves) full(i++, Slot<0>{});
-  if (halves) {
-    bf16x8 p[2];
-    const int ks = i & 1, kb = (halves - 1) & 1;
-    if (kb) {
+  if constexpr (P == 1) {
+    // a block whose keys are all seen and that is not the wave's last; its first half's scores are in s0
+    auto full = [&](int i, auto kslot) {
+      constexpr int ks = decltype(kslot)::v;
+      bf16x8 p[2];
       raise_max(max16(s0));
       scores(ks, 1, s1);
       probs(s0, p);
       accumulate(vs, 0, p);
-      s0 = s1;
+      const float mx = max16(s1);
+      turn(i, ks);
+      raise_max(mx);
+      scores(ks ^ 1, 0, s0);
+      probs(s1, p);
+      accumulate(vs, 1, p);
+      vs = vs == 2 ? 0 : vs + 1;
+    };
+    for (; 2 * i + 4 < halves; i += 2) {
+      full(i, Slot<0>{});
+      full(i + 1, Slot<1>{});
     }
-    turn(i, ks);
-    diagonal(vs, kb, s0, p);
-    vs = vs == 2 ? 0 : vs + 1;
-    ++i;
+    if (2 * i + 2 < halves) full(i++, Slot<0>{});
+    if (halves) {
+      const int ks = i & 1, kb = (halves - 1) & 1;
+      if (kb) {
+        bf16x8 p[2];
+        raise_max(max16(s0));
+        scores(ks, 1, s1);
+        probs(s0, p);
+        accumulate(vs, 0, p);
+        s0 = s1;
+      }
+      turn(i, ks);
+      diagonal(vs, kb, l32, s0);
+      vs = vs == 2 ? 0 : vs + 1;
+      ++i;
+    }
+  } else {
+    // one half of each block, its scores in `now`; the next block's, made after the barrier, in `then`
+    auto half = [&](int i, auto kslot, f32x16 &now, f32x16 &then) {
+      constexpr int ks = decltype(kslot)::v;
+      bf16x8 p[2];
+      const float mx = max16(now);
+      turn(i, ks);
+      raise_max(mx);
+      scores(ks ^ 1, 0, then);
+      probs(now, p);
+      accumulate(vs, 0, p);
+      vs = vs == 2 ? 0 : vs + 1;
+    };
+    const int mine = (halves + 1 - part) / 2;  // blocks of which this wave has a half
+    for (; i + 2 < mine; i += 2) {
+      half(i, Slot<0>{}, s0, s1);
+      half(i + 1, Slot<1>{}, s1, s0);
+    }
+    if (i + 1 < mine) {
+      half(i, Slot<0>{}, s0, s1);
+      s0 = s1;
+      ++i;
+    }
+    if (mine) {
+      turn(i, i & 1);
+      diagonal(vs, 0, ((halves - 1) & 1) == part ? l32 : 31, s0);  // the diagonal is one of the two waves'
+      vs = vs == 2 ? 0 : vs + 1;
+      ++i;
+    }
   }
   for (; i < nblk; ++i) {
     turn(i, i & 1);
@@ -339,11 +378,35 @@ __global__ __launch_bounds__(64 * W, D == 128 ? 2 : 3) void prompt_kernel(const 
   }
 
   l = half_add(l);
+  constexpr int kKept = D / 32 / P;  // 32-column tiles of O that this wave stores
+  if constexpr (P == 2) {
+    // the two waves' sums: each gives the other half of its columns, the maximum and the sum
+    float *const shared = reinterpret_cast<float *>(lds);
+    constexpr int kWave = 64 * (16 * kKept + 2);
+    static_assert(W * kWave * 4 <= 5 * kBlock);
+    block_barrier();  // every wave has read its last K and V
+    float *const give = shared + wave * kWave + lane;
+#pragma unroll
+    for (int d = 0; d < kKept; ++d)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) give[64 * (16 * d + e)] = part ? o[d][e] : o[kKept + d][e];
+    give[64 * 16 * kKept] = m;
+    give[64 * (16 * kKept + 1)] = l;
+    __syncthreads();
+    const float *const take = shared + (wave ^ 1) * kWave + lane;
+    const float m2 = take[64 * 16 * kKept], top = __builtin_fmaxf(m, m2);
+    const float f = __builtin_amdgcn_exp2f((m - top) * a.scale), f2 = __builtin_amdgcn_exp2f((m2 - top) * a.scale);
+    l = l * f + take[64 * (16 * kKept + 1)] * f2;
+#pragma unroll
+    for (int d = 0; d < kKept; ++d)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) o[d][e] = (part ? o[kKept + d][e] : o[d][e]) * f + take[64 * (16 * d + e)] * f2;
+  }
   const float inv = 1.f / l;
   const bool stored = row < len;
-  __bf16 *orow = a.out + (tile.x + (int64_t)row) * a.so + head * a.ho;
+  __bf16 *orow = a.out + (tile.x + (int64_t)row) * a.so + head * a.ho + 32 * kKept * part;
 #pragma unroll
-  for (int d = 0; d < D / 32; ++d)
+  for (int d = 0; d < kKept; ++d)
 #pragma unroll
     for (int g = 0; g < 2; ++g) {
       // columns 32 d + 16 g + 0..15 of this query sit in lanes l32 and l32 + 32
@@ -371,6 +434,19 @@ int unit_log(int group, int waves) {
   return n;
 }
 
+int tile_tokens(int group, int parts) { return (32 * kWaves / parts) >> unit_log(group, kWaves / parts); }
+
+constexpr int64_t kCus = 256;
+// Workgroups that the chip holds at once: two a CU, three with heads of 64.
+int64_t places(int head_dim) { return head_dim == 128 ? 2 * kCus : 3 * kCus; }
+// Up to how many whole tiles they are split over the keys: a wave's half tile runs
+// 0.8 us on its CU alone, so that few long tiles leave the chip waiting for the
+// longest, while split ones fetch each key for half as many queries.  us, whole and
+// split, by tiles: 32 / 8 heads of 128, 64 (500 tokens, 16 / 8) 14.4, 11.3; 256 (1000)
+// 25.5, 20.8; 376 (1500) 36.0, 36.6; 512 (2048) 50.0, 53.4.  Heads of 64, 580 tiles
+// 24.5, 21.5; 632 45.0, 42.4; 768 26.6, 26.9; 1280 18.8, 23.7.
+int64_t split_tiles(int head_dim) { return head_dim == 128 ? 320 : 700; }
+
 // The bytes from a view's first element to past its last.
 struct Span {
   uintptr_t lo, hi;
@@ -395,22 +471,35 @@ extern "C" int mq_prompt_plan_make(const int64_t *lengths, int64_t count, int he
     if (lengths[s] < 0 || lengths[s] >= (int64_t(1) << 31) || (total += lengths[s]) >= (int64_t(1) << 31))
       return invalid("mq_prompt_plan_make: a negative length, or 2^31 tokens or more");
   }
-  const int tile = (32 * kWaves) >> unit_log(heads / kv_heads, kWaves);
+  // parts 2 where whole tiles would leave the chip's places empty or be few enough
+  // that the longest sets the time
   int64_t n = 0, longest = 0;
-  for (int64_t s = 0; s < count; ++s) {
-    n += (lengths[s] + tile - 1) / tile;
-    longest = std::max(longest, lengths[s]);
+  int tile = 0, parts = 1;
+  for (;;) {
+    tile = tile_tokens(heads / kv_heads, parts);
+    n = 0;
+    for (int64_t s = 0; s < count; ++s) {
+      n += (lengths[s] + tile - 1) / tile;
+      longest = std::max(longest, lengths[s]);
+    }
+    if (parts == 2 || n * (heads >> unit_log(heads / kv_heads, kWaves)) > split_tiles(head_dim)) break;
+    parts = 2;
   }
-  *plan = mq_prompt_plan{total, n, heads, kv_heads, head_dim, tile, kWaves};
+  *plan = mq_prompt_plan{total, n, heads, kv_heads, head_dim, tile, parts};
   if (!tiles) return MQ_OK;
   if (capacity < n) return invalid("mq_prompt_plan_make: tiles holds fewer than the plan's tiles");
-  // longest first: the tiles at one distance from their prompts' starts, the furthest first
+  // longest first: the tiles at one distance from their prompts' starts, the furthest
+  // first.  Where all run at once, those after the first of each CU are taken from
+  // the other end, so that a long tile shares its CU with a short one.
+  const int64_t units = heads >> unit_log(heads / kv_heads, kWaves / parts);
+  const int64_t turn = n * units <= places(head_dim) ? std::max<int64_t>(1, kCus / units) : n;
   int64_t at = 0;
   for (int64_t first = (longest - 1) / tile * tile; longest > 0 && first >= 0; first -= tile) {
     int64_t start = 0;
     for (int64_t s = 0; s < count; start += lengths[s++])
       if (lengths[s] > first) {
-        int32_t *t = tiles + 4 * at++;
+        int32_t *t = tiles + 4 * (at < turn ? at : n - 1 - (at - turn));
+        ++at;
         t[0] = (int32_t)start;
         t[1] = (int32_t)lengths[s];
         t[2] = (int32_t)first;
@@ -428,8 +517,8 @@ extern "C" int mq_prompt_attention(const mq_prompt_plan *plan, const int32_t *ti
   if (!plan) return invalid("mq_prompt_attention: NULL plan");
   const int heads = plan->heads, kv = plan->kv_heads, dim = plan->head_dim;
   if ((dim != 64 && dim != 128) || heads < 1 || heads > 65536 || kv < 1 || heads % kv || plan->tokens < 0 ||
-      plan->tokens >= (int64_t(1) << 31) || plan->tiles < 0 || plan->tiles > plan->tokens || plan->waves != kWaves ||
-      plan->tile_tokens != (32 * kWaves) >> unit_log(heads / kv, kWaves))
+      plan->tokens >= (int64_t(1) << 31) || plan->tiles < 0 || plan->tiles > plan->tokens || (plan->parts != 1 && plan->parts != 2) ||
+      plan->tile_tokens != tile_tokens(heads / kv, plan->parts))
     return invalid("mq_prompt_attention: not a plan of mq_prompt_plan_make");
   if (!(scale > 0.f) || scale > 3e38f) return invalid("mq_prompt_attention: scale must be positive and finite");
   if (plan->tokens == 0 || plan->tiles == 0) return MQ_OK;
@@ -452,7 +541,7 @@ extern "C" int mq_prompt_attention(const mq_prompt_plan *plan, const int32_t *ti
                          span(k, plan->tokens, k_token_stride, kv, k_head_stride, dim),
                          span(v, plan->tokens, v_token_stride, kv, v_head_stride, dim)})
     if (o.lo < in.hi && in.lo < o.hi) return invalid("mq_prompt_attention: out lies over q, k or v");
-  const int log_heads = unit_log(heads / kv, kWaves), units = heads >> log_heads;
+  const int log_heads = unit_log(heads / kv, kWaves / plan->parts), units = heads >> log_heads;
   const int64_t grid = plan->tiles * units;
   if (grid >= (int64_t(1) << 31)) return invalid("mq_prompt_attention: 2^31 tiles or more");
   const PromptArgs a{static_cast<const __bf16 *>(q), static_cast<const __bf16 *>(k), static_cast<const __bf16 *>(v),
@@ -460,8 +549,11 @@ extern "C" int mq_prompt_attention(const mq_prompt_plan *plan, const int32_t *ti
                      q_head_stride, k_head_stride, v_head_stride, out_head_stride, reinterpret_cast<const int4 *>(tiles),
                      plan->tokens, units, heads / kv, log_heads, scale * 1.44269504f};
   hipStream_t s = static_cast<hipStream_t>(stream);
-  if (dim == 128) hipLaunchKernelGGL((prompt_kernel<128, kWaves>), dim3((unsigned)grid), dim3(64 * kWaves), 0, s, a);
-  else hipLaunchKernelGGL((prompt_kernel<64, kWaves>), dim3((unsigned)grid), dim3(64 * kWaves), 0, s, a);
+  auto launch = [&]<int D, int P>() {
+    hipLaunchKernelGGL((prompt_kernel<D, kWaves, P>), dim3((unsigned)grid), dim3(64 * kWaves), 0, s, a);
+  };
+  if (dim == 128) plan->parts == 1 ? launch.template operator()<128, 1>() : launch.template operator()<128, 2>();
+  else plan->parts == 1 ? launch.template operator()<64, 1>() : launch.template operator()<64, 2>();
   const hipError_t e = hipGetLastError();
   return e == hipSuccess ? MQ_OK : set_error(MQ_E_HIP, hipGetErrorString(e));
 }

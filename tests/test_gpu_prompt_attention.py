@@ -50,13 +50,26 @@ def _run(q, k, v, lengths, **kw):
     return TA.prompt_attention(q, k, v, TA.PromptPlan(lengths, q.shape[1], k.shape[1], q.shape[2]), **kw)
 
 
+def _run_whole(q, k, v, lengths):
+    """The same rows in a batch of so many tiles that each takes all its keys in one part, before
+    many prompts of zeros."""
+    more = [1000] * 120
+    pad = lambda t: torch.cat([t, torch.zeros((sum(more),) + t.shape[1:], dtype=t.dtype, device="cuda")])
+    plan = TA.PromptPlan(lengths + more, q.shape[1], k.shape[1], q.shape[2])
+    assert plan.c.parts == 1 and TA.PromptPlan(lengths, q.shape[1], k.shape[1], q.shape[2]).c.parts == 2
+    return TA.prompt_attention(pad(q), pad(k), pad(v), plan)[:q.shape[0]]
+
+
 @gpu
 @pytest.mark.parametrize("dim", [64, 128])
 @pytest.mark.parametrize("heads,kv", [(1, 1), (4, 2), (8, 2), (7, 1), (6, 2), (16, 1), (12, 12)])
 def test_lengths_and_groups(heads, kv, dim):
     for n in (1, 2, 31, 32, 33, 63, 64, 65, 95, 96, 97, 127, 128, 129, 160, 193, 257, 320, 577):
         q, k, v = _inputs([n], heads, kv, dim)
-        assert _err(_run(q, k, v, [n]), _ref(q, k, v, [n])) < BOUND, n
+        ref = _ref(q, k, v, [n])
+        assert _err(_run(q, k, v, [n]), ref) < BOUND, n
+        if n in (1, 31, 33, 64, 96, 129, 257, 577):
+            assert _err(_run_whole(q, k, v, [n]), ref) < BOUND, n
 
 
 @gpu
@@ -67,7 +80,8 @@ def test_packed_prompts(heads, kv, dim):
     lengths = [3, 0, 1, 130, 64, 0, 33, 257, 1, 31, 0]
     q, k, v = _inputs(lengths, heads, kv, dim)
     out = _run(q, k, v, lengths)
-    assert _err(out, _ref(q, k, v, lengths)) < BOUND
+    ref = _ref(q, k, v, lengths)
+    assert _err(out, ref) < BOUND and _err(_run_whole(q, k, v, lengths), ref) < BOUND
     at = 0
     for n in lengths:
         if n:
@@ -95,16 +109,17 @@ def test_flat_and_one_hot_rows(sharp, scale):
 @pytest.mark.parametrize("dim", [64, 128])
 @pytest.mark.parametrize("bad", [float("nan"), float("inf"), float("-inf")])
 @pytest.mark.parametrize("which", ["k", "v"])
-def test_unseen_keys_do_not_reach_a_row(which, bad, dim):
+@pytest.mark.parametrize("run", [_run, _run_whole], ids=["parts", "whole"])
+def test_unseen_keys_do_not_reach_a_row(run, which, bad, dim):
     """A non-finite key or value of a later token, or of another prompt, changes no bit of a row;
     rows that see it become what the sum says."""
     lengths = [70, 100, 40]
     q, k, v = _inputs(lengths, 4, 2, dim, seed=9)
-    clean = _run(q, k, v, lengths)
+    clean = run(q, k, v, lengths)
     for at in (0, 31, 32, 50, 63, 64, 90, 99):
         k2, v2 = k.clone(), v.clone()
         (k2 if which == "k" else v2)[70 + at, 1, 5] = bad
-        out = _run(q, k2, v2, lengths)
+        out = run(q, k2, v2, lengths)
         same = torch.cat([out[:70 + at], out[170:]])
         assert torch.equal(same, torch.cat([clean[:70 + at], clean[170:]])), at
         assert torch.equal(out[:, :2], clean[:, :2]), at           # the other group of heads
@@ -170,10 +185,11 @@ def test_offsets_past_32_bits():
 @gpu
 def test_long_prompt_rows():
     """Sampled rows of a prompt whose tiles fill the chip several times."""
-    n = 5001
+    n = 7001
     q, k, v = _inputs([n], 8, 2, 128, seed=4)
     out = _run(q, k, v, [n])
-    for i in (0, 1, 2047, 2048, 4095, 4999, 5000):
+    assert TA.PromptPlan([n], 8, 2, 128).c.parts == 1
+    for i in (0, 1, 2047, 2048, 4095, 6999, 7000):
         kk, vv = (t[:i + 1].double().repeat_interleave(4, 1).transpose(0, 1) for t in (k, v))
         w = torch.softmax((kk @ q[i].double().unsqueeze(2)).squeeze(2) / 128 ** 0.5, -1)
         ref = (w.unsqueeze(1) @ vv.contiguous()).squeeze(1)
@@ -231,11 +247,15 @@ def _plan(lengths, heads=4, kv=2, dim=64, capacity=64):
     return rc, c, [tuple(tiles[4 * i:4 * i + 4]) for i in range(min(capacity, max(0, c.tiles)))]
 
 
-@pytest.mark.parametrize("heads,kv,tile", [(4, 4, 128), (4, 2, 64), (8, 2, 32), (7, 1, 128), (6, 1, 64), (12, 1, 32)])
-def test_plan_covers_every_token_once(heads, kv, tile):
-    lengths = [0, 5, 128, 129, 0, 64, 1, 300]
-    rc, c, tiles = _plan(lengths, heads, kv)
-    assert rc == 0 and c.tokens == sum(lengths) and c.tile_tokens == tile and c.tiles == sum(-(-n // tile) for n in lengths)
+@pytest.mark.parametrize("heads,kv,whole,split", [(4, 4, 128, 64), (4, 2, 64, 32), (8, 2, 32, 32), (7, 1, 128, 64), (6, 1, 64, 32), (12, 1, 32, 32)])
+@pytest.mark.parametrize("parts", [1, 2])
+def test_plan_covers_every_token_once(heads, kv, whole, split, parts):
+    """Few tiles are split over the keys too (two parts), many are not."""
+    lengths = [0, 5, 128, 129, 0, 64, 1, 300] + [50000] * (2 - parts) * 16
+    rc, c, tiles = _plan(lengths, heads, kv, capacity=40000)
+    tile = whole if parts == 1 else split
+    assert rc == 0 and c.parts == parts
+    assert c.tokens == sum(lengths) and c.tile_tokens == tile and c.tiles == sum(-(-n // tile) for n in lengths)
     starts = {}
     for start, n, first, _ in tiles[:c.tiles]:
         starts.setdefault((start, n), []).append(first)
@@ -246,6 +266,13 @@ def test_plan_covers_every_token_once(heads, kv, tile):
         at += n
     assert {key: sorted(f) for key, f in starts.items()} == want
     assert [t[2] for t in tiles[:c.tiles]] == sorted((t[2] for t in tiles[:c.tiles]), reverse=True)     # longest first
+
+
+def test_plan_pairs_long_tiles_with_short_ones():
+    """Where all workgroups run at once, those after a CU's first come from the short end."""
+    rc, c, tiles = _plan([2000], 32, 8, 128)
+    firsts = [t[2] // 32 for t in tiles[:c.tiles]]
+    assert rc == 0 and c.parts == 1 and firsts == list(range(62, 30, -1)) + list(range(0, 31))
 
 
 def test_argument_checks():
@@ -260,7 +287,7 @@ def test_argument_checks():
 
     def call(plan=plan, tiles=4096, q=4096, qs=(256, 64), k=4096, ks=(128, 64), v=4096, vs=(128, 64), scale=0.1, out=far, os=(256, 64)):
         return lib.mq_prompt_attention(plan, tiles, q, *qs, k, *ks, v, *vs, scale, out, *os, None)
-    foreign = _lib.PromptPlanC(40, 3, 4, 2, 64, 128, 4)
+    foreign = _lib.PromptPlanC(40, 3, 4, 2, 64, 128, 1)
     bad = [dict(plan=None), dict(plan=foreign), dict(q=None), dict(tiles=None), dict(q=4100), dict(out=far + 2), dict(qs=(252, 64)),
            dict(ks=(-128, 64)), dict(vs=(1 << 24, 64)), dict(os=(128, 64)), dict(os=(256, 32)), dict(os=(0, 64)), dict(os=(64, 64 * 39)),
            dict(scale=0.0), dict(scale=float("nan")), dict(scale=float("inf")), dict(out=4096), dict(out=4096 + 2 * 128 * 39)]
@@ -275,7 +302,7 @@ def test_argument_checks():
 @pytest.mark.skipif(HIPCC is None, reason="hipcc not available")
 def test_kernel_leaves_m0_alone_and_does_not_spill(tmp_path):
     funcs = {k: v for k, v in _functions(_asm(tmp_path, "mq_prompt.hip")).items() if "prompt_kernel" in k}
-    assert len(funcs) == 2
+    assert len(funcs) == 4
     for name, (lines, meta) in funcs.items():
         assert not _m0_outside_asm(lines), name
         assert meta.get("ScratchSize", 0) == 0, (name, meta)
