@@ -10,10 +10,11 @@
 //           16 u + r and, of each block b of 32 of the head, eight values.  In BF16
 //           and Q8_0 these are 32 b + 8 g + 0..7; in Q4_0, whose byte j of a block
 //           is ggml's (values j and j + 16), bytes 4 g + 0..3.
-//   values  plane of D / 16 operands, O^T = V^T P^T: lane 16 g + r holds value
-//           16 c + r of the eight tokens 16 (j / 4) + 4 g + j % 4 (j = 0..7),
-//           which are the ones whose scores S^T leaves in that lane.  A Q4_0
-//           byte is again the pair (32 b + r, 32 b + 16 + r).
+//   values  plane of D / 16 operands, O^T = V^T P^T, two a block: lane 16 g + r holds
+//           value 32 b + 2 r + c of the eight tokens 16 (j / 4) + 4 g + j % 4 (j =
+//           0..7), which are the ones whose scores S^T leaves in that lane; c = 0 in
+//           the first operand, 1 in the second, so that a lane's eight results of a
+//           block lie next to each other.  A Q4_0 byte is the pair, c = 0 its low half.
 //   scales  of the block types, f16: the keys' as [g][u][b][token 4 g + 0..3 of
 //           u], the values' as [g][b][j].
 // A lane's bytes of one plane are split into pieces of 16 (8 for the keys of Q4_0
@@ -43,11 +44,11 @@ struct CacheTile {
     const int at = b * (kKeyLane / kBlocks) + i;
     return (t >> 4) * (64 * kKeyLane) + at / kKeyPiece * (64 * kKeyPiece) + (16 * g + (t & 15)) * kKeyPiece + at % kKeyPiece;
   }
-  // Value d of token t: its first byte (Q4_0: of the pair, d % 32 < 16).
+  // Value d of token t: its first byte (Q4_0: of the pair, d even).
   __device__ static int value(int t, int d) {
-    const int j = 4 * (t >> 4) + (t & 3);
-    const int at = T == BF16 ? (d >> 4) * 16 + 2 * j : T == Q8_0 ? (d >> 4) * 8 + j : (d >> 5) * 8 + j;
-    return kPlane + at / 16 * 1024 + (16 * ((t >> 2) & 3) + (d & 15)) * 16 + at % 16;
+    const int j = 4 * (t >> 4) + (t & 3), c = 2 * (d >> 5) + (d & 1);
+    const int at = T == BF16 ? c * 16 + 2 * j : T == Q8_0 ? c * 8 + j : (d >> 5) * 8 + j;
+    return kPlane + at / 16 * 1024 + (16 * ((t >> 2) & 3) + ((d >> 1) & 15)) * 16 + at % 16;
   }
   __device__ static int key_scale(int t, int b) {
     return 2 * kPlane + 2 * ((((((t >> 2) & 3) * 2 + (t >> 4)) * kBlocks) + b) * 4 + (t & 3));

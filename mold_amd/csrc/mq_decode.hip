@@ -238,6 +238,12 @@ __device__ __forceinline__ float column_add(float v) {
   return half_add(__uint_as_float(r[0]) + __uint_as_float(r[1]));
 }
 
+// A lane's eight columns of a block, in order, from its two operands' results.
+__device__ __forceinline__ void put8(float *p, const f32x4 *x) {
+  reinterpret_cast<f32x4 *>(p)[0] = f32x4{x[0][0], x[1][0], x[0][1], x[1][1]};
+  reinterpret_cast<f32x4 *>(p)[1] = f32x4{x[0][2], x[1][2], x[0][3], x[1][3]};
+}
+
 // Shares of one (sequence, head unit) that the waves of a workgroup hold, added
 // in the order of the waves, each relative to its own maximum.
 template <int D, int W>
@@ -247,7 +253,7 @@ struct Shares {
   __device__ __forceinline__ void put(int wave, int lane, const f32x4 *x, float ms, float sum) {
     const int g = lane >> 4, r = lane & 15;
 #pragma unroll
-    for (int c = 0; c < D / 16; ++c) *reinterpret_cast<f32x4 *>(&o[wave][r][16 * c + 4 * g]) = x[c];
+    for (int b = 0; b < D / 32; ++b) put8(&o[wave][r][32 * b + 8 * g], x + 2 * b);
     if (g == 0) {
       m[wave][r] = ms;
       l[wave][r] = sum;
@@ -358,7 +364,7 @@ __global__ __launch_bounds__(64 * (kPair ? kPairWaves : kWaves), kPair ? 2 : D =
   };
 
   bf16x8 qf[kB];  // q, the scores' B operand
-  f32x4 o[kC];  // O^T: this lane's head, columns 16 c + 4 g + 0..3
+  f32x4 o[kC];  // O^T: this lane's head, columns 32 b + 8 g + 2 i + c in o[2 b + c][i]
   float m, l;
   auto begin = [&]() {
     const int in = chunk * kHeads + r;
@@ -507,15 +513,19 @@ __global__ __launch_bounds__(64 * (kPair ? kPairWaves : kWaves), kPair ? 2 : D =
       shares.put(wave, lane, o, m * a.scale, l);
     } else if (count == tiles) {
       const float inv = 1.f / l;
-      __bf16 *p = a.out + b * a.so + (int64_t)(kv * a.group + in) * a.ho + 4 * g;
+      __bf16 *p = a.out + b * a.so + (int64_t)(kv * a.group + in) * a.ho + 8 * g;
       if (in < a.group)
 #pragma unroll
-        for (int c = 0; c < kC; ++c) store4(p + 16 * c, o[c], inv);
+        for (int i = 0; i < kB; ++i) {
+          const f32x4 &x = o[2 * i], &y = o[2 * i + 1];
+          *reinterpret_cast<uint4 *>(p + 32 * i) = make_uint4(pack2(x[0] * inv, y[0] * inv), pack2(x[1] * inv, y[1] * inv),
+                                                              pack2(x[2] * inv, y[2] * inv), pack2(x[3] * inv, y[3] * inv));
+        }
     } else {
       float *rec = a.partial + (int64_t)(2 * run + (from != first)) * nh * (D + 4);
       if (in < a.group) {
 #pragma unroll
-        for (int c = 0; c < kC; ++c) *reinterpret_cast<f32x4 *>(rec + r * D + 16 * c + 4 * g) = o[c];
+        for (int i = 0; i < kB; ++i) put8(rec + r * D + 32 * i + 8 * g, o + 2 * i);
         if (g == 0) *reinterpret_cast<float2 *>(rec + nh * D + 2 * r) = make_float2(m * a.scale, l);
       }
     }
