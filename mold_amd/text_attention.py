@@ -205,9 +205,9 @@ class KvCache:
             raise ValueError(f"KvCache.append: k and v must be {list(shape)} of one type on {self.device}")
         st, sh, sd = t.stride()
         mask = 7 if dtype is _BF16 else 3
-        if sd != 1 or (st | sh) & mask or t.data_ptr() & 15:
+        if sd != 1 or (st | sh) & mask or st >= _MAX_STRIDE or sh >= _MAX_STRIDE or t.data_ptr() & 15:
             st, sh = _strides(t)
-            if sd != 1 or (st | sh) & mask or t.data_ptr() & 15:
+            if sd != 1 or (st | sh) & mask or st >= _MAX_STRIDE or sh >= _MAX_STRIDE or t.data_ptr() & 15:
                 t = t.contiguous()
                 st, sh = _strides(t)
         return t, st, sh

@@ -169,6 +169,22 @@ def test_pages_past_32_bits():
 
 
 @gpu
+def test_rows_past_32_bits():
+    """Rows 2^22 elements apart, 1100 of them: 9 GB in bf16; and 2^24 apart, which are copied."""
+    new = _rows(1100, 2, 64, seed=6, dtype=BF)
+    slots = torch.arange(1100, device="cuda")
+    want = TA.KvCache(35, 2, 64, page_tokens=32)
+    want.append(new[0], new[1], slots)
+    for n, step in ((1100, 1 << 22), (40, 1 << 24)):
+        far = torch.empty((n - 1) * step + 256, dtype=BF, device="cuda").as_strided((n, 4, 64), (step, 64, 1))
+        far.copy_(torch.cat([new[0], new[1]], 1)[:n])
+        cache = TA.KvCache(35, 2, 64, page_tokens=32)
+        cache.append(far[:, :2], far[:, 2:], slots[:n])
+        assert all(torch.equal(a, b[:n]) for a, b in zip(cache.read(slots[:n]), want.read(slots)))
+        del far
+
+
+@gpu
 def test_slots_of_positions_and_streams():
     cache = TA.KvCache(6, 2, 64, page_tokens=32)
     table = torch.tensor([[4, 1], [0, 5]], dtype=torch.int32, device="cuda")
@@ -230,7 +246,7 @@ def test_argument_checks():
     def read(c=None, slots=4096, n=3, k=4096, v=4096, dt=30):
         c = c or _cache()
         return lib.mq_kv_cache_read(ctypes.byref(c), slots, n, k, v, dt, None)
-    for kw in (dict(k=None), dict(slots=None), dict(k=4100), dict(slots=4100), dict(ks=(-128, 64)), dict(vs=(128, 60)), dict(dt=1), dict(n=-1),
+    for kw in (dict(k=None), dict(slots=None), dict(k=4100), dict(slots=4100), dict(ks=(-128, 64)), dict(vs=(128, 60)), dict(vs=(1 << 24, 64)), dict(dt=1), dict(n=-1),
                dict(n=1 << 31), dict(c=_cache(page=16)), dict(c=_cache(data=4100)), dict(c=_cache(data=None)), dict(ks=(2, 64), dt=0)):
         assert append(**kw) == -1, kw
     for kw in (dict(k=None), dict(v=4098), dict(slots=None), dict(dt=8), dict(n=-5), dict(c=_cache(dtype=3)), dict(c=_cache(data=4098))):
