@@ -57,11 +57,16 @@ struct Slot {
   static constexpr int v = S;
 };
 
-__device__ __forceinline__ bool any_not_finite(const uint4 &u) {
-  bool odd = false;
-  for (const uint32_t two : {u.x, u.y, u.z, u.w})
-    odd = odd || (two & 0x7F80u) == 0x7F80u || (two & 0x7F800000u) == 0x7F800000u;
-  return odd;
+// The largest magnitudes, as bit patterns, of the even and of the odd values: from
+// 0x7F80 on one is not finite.
+typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ void raise_magnitudes(u16x2 &most, const uint4 &u) {
+  for (const uint32_t two : {u.x, u.y, u.z, u.w}) {
+    const uint32_t bits = two & 0x7FFF7FFFu;
+    u16x2 x;
+    __builtin_memcpy(&x, &bits, 4);
+    most = __builtin_elementwise_max(most, x);
+  }
 }
 
 // W waves of 32 queries each; with P = 2 two waves share their queries and take
@@ -279,12 +284,12 @@ __global__ __launch_bounds__(64 * W, D == 128 ? 2 : 3) void prompt_kernel(const 
     mask(s, last);
     raise_max(max16(s));
     probs(s, p);
-    bool odd = false;
+    u16x2 most{0, 0};
 #pragma unroll
     for (int t = 0; t < 2; ++t)
 #pragma unroll
-      for (int d = 0; d < D / 32; ++d) odd = any_not_finite(values(slot, kb, t, d)) || odd;
-    if (__any(odd)) accumulate_seen(slot, kb, last, p);
+      for (int d = 0; d < D / 32; ++d) raise_magnitudes(most, values(slot, kb, t, d));
+    if (__any(max(most[0], most[1]) >= 0x7F80)) accumulate_seen(slot, kb, last, p);
     else accumulate(slot, kb, p);
   };
 
