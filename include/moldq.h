@@ -340,12 +340,12 @@ typedef struct mq_kv_cache {
 size_t mq_kv_cache_size(const mq_kv_cache *cache);
 /* Write rows t < tokens of k and v (F32 or BF16, head h of row t at t *
  * token_stride + h * head_stride, unit stride inside a head, 16-byte aligned,
- * strides multiples of 16 bytes below 2^24 elements) to slots[t] (device memory).  BF16 rounds to
- * nearest even; a block type's blocks are those of mq_quantize, and a block with
- * a value that is not finite, or whose scale passes float16, reads back as
- * infinities and NaN.  Slots outside the cache are
- * skipped (a padding row's is -1); two rows of one call must not share a slot.
- * Asynchronous on stream. */
+ * strides multiples of 16 bytes below 2^24 elements) to slots[t] (device
+ * memory).  BF16 rounds to nearest even; a block type's blocks are those of
+ * mq_quantize, and a block with a value that is not finite, or whose scale
+ * passes float16, reads back as infinities and NaN.  Slots outside the cache
+ * are skipped (a padding row's is -1); two rows of one call must not share a
+ * slot.  Asynchronous on stream. */
 int mq_kv_cache_append(const mq_kv_cache *cache, const void *k, int64_t k_token_stride, int64_t k_head_stride,
                        const void *v, int64_t v_token_stride, int64_t v_head_stride, int x_dtype, int64_t tokens,
                        const int64_t *slots, void *stream);

@@ -7,12 +7,14 @@
 // 16, the other columns of the matrix instruction are zeros) with a tile of 32
 // tokens are 16 MFMAs, far from their rate, also after a block type's bytes have
 // been widened.  So the kernel is laid out for the loads:
-//   * every wave is on its own: no LDS, no barrier.  The work of the whole batch
-//     is one line of (sequence, k/v head, tile of 32 tokens), cut into equal runs,
-//     one a wave, whatever the lengths are; the lengths stay on the device (each
-//     wave adds them up), so the host neither waits nor plans;
+//   * the work of the whole batch is one line of (sequence, k/v head, tile of 32
+//     tokens), cut into equal runs, one a wave, whatever the lengths are; the
+//     lengths stay on the device (each wave adds them up), so the host neither
+//     waits nor plans;
 //   * a tile is read in the order of the matrix operands (mq_cache.h), 1 KiB a
-//     load instruction, two tiles in flight a wave, eight waves a CU;
+//     load instruction; a wave has one tile in flight, the next one's keys
+//     requested when this one's scores are made and its values when these are
+//     added, and 8 or 12 waves a CU together keep HBM busy;
 //   * the scores are computed transposed, S^T = K Q^T, so that a lane's eight
 //     probabilities are its B operand of O^T = V^T P^T, as they stand;
 //   * the block types' whole numbers enter the products as they are: a key block's
@@ -22,8 +24,13 @@
 //     lacks (relative 2^-16 together): the second product costs matrix time that
 //     the loads leave free, and a step of a few tokens, whose roundings do not
 //     average out, is as exact as its output's type.
-// A run that holds a whole (sequence, head) stores its result; the others store
-// f32 sums, which join_kernel adds in the order of the line.
+// The waves of a workgroup that lie within one (sequence, head unit) join in LDS.
+// What holds a whole one stores its result; the others store f32 sums, which
+// join_kernel adds in the order of the line.  Where page tables are short a
+// workgroup takes a whole (sequence, head unit), and there is no second launch.
+// Reached (32 / 8 heads of 128, us a call, TB/s of the cache's bytes): 64 sequences
+// of 8192 tokens BF16 358 (6.0), one of 65001 54 (4.9), 40 ragged ones up to 6000
+// in Q8_0 51 (3.9: launch, the line and the join are some 10 us of it).
 #include "../../include/moldq.h"
 #include "mq_cache.h"
 
@@ -36,7 +43,6 @@ namespace {
 
 constexpr int kWaves = 4;           // of a workgroup whose waves take runs of the line
 constexpr int kHeads = 16;          // columns of the matrix instruction
-constexpr int kPairWaves = 8;       // of a workgroup that takes one (sequence, head unit)
 
 struct DecodeArgs {
   CacheView cache;
@@ -282,12 +288,13 @@ __device__ __forceinline__ void store4(__bf16 *p, const f32x4 &x, float inv) {
   *reinterpret_cast<uint2 *>(p) = make_uint2(pack2(x[0] * inv, x[1] * inv), pack2(x[2] * inv, x[3] * inv));
 }
 
-// kPair: a workgroup takes a (sequence, head unit), its waves equal shares of its
-// tiles, and stores the result.  Otherwise a wave takes a run of the line.
-template <int T, int D, bool kPair>
-__global__ __launch_bounds__(64 * (kPair ? kPairWaves : kWaves), kPair ? 2 : D == 128 ? 3 : 4) void decode_kernel(const DecodeArgs a) {
+// P > 0: a workgroup of P waves takes a (sequence, head unit), its waves equal shares
+// of its tiles, and stores the result.  P = 0: a wave takes a run of the line.
+template <int T, int D, int P>
+__global__ __launch_bounds__(64 * (P ? P : kWaves), P == 8 ? 2 : D == 128 ? 3 : 4) void decode_kernel(const DecodeArgs a) {
   using L = CacheTile<T, D>;
-  constexpr int kB = L::kBlocks, kC = D / 16, kW = kPair ? kPairWaves : kWaves;
+  constexpr bool kPair = P > 0;
+  constexpr int kB = L::kBlocks, kC = D / 16, kW = kPair ? P : kWaves;
   __shared__ Shares<D, kW> shares;
   const int lane = threadIdx.x & 63, g = lane >> 4, r = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -309,7 +316,7 @@ __global__ __launch_bounds__(64 * (kPair ? kPairWaves : kWaves), kPair ? 2 : D =
     b = blockIdx.x / units;
     kv = head / a.chunks;
     chunk = head - kv * a.chunks;
-    page0 = numbers = 0;  // its table has fewer than 64 pages, or none; it and the length are read together
+    page0 = numbers = 0;  // its table has up to 64 pages, or none; it and the length are read together
     if (a.max_pages > 0) numbers = a.table[b * a.table_stride + min(lane, a.max_pages - 1)];
     n = a.lengths[b];
     tiles = Line::tiles_of(a, n);
@@ -703,10 +710,21 @@ int invalid(const char *msg) { return set_error(MQ_E_INVALID, msg); }
 
 int chunks_of(int heads, int kv_heads) { return (heads / kv_heads + kHeads - 1) / kHeads; }
 
-// Whether a workgroup takes each (sequence, head unit): up to kPairTiles tiles of
-// a sequence, by what its page table can hold, which is all the host knows.
-constexpr int64_t kPairTiles = 32;
-bool by_pairs(const mq_kv_cache *c, int64_t max_pages) { return max_pages * (c->page_tokens / kTileTokens) <= kPairTiles; }
+// (sequence, head unit) pairs.
+int64_t pairs_of(const mq_kv_cache *c, int64_t batch, int heads) { return batch * c->kv_heads * chunks_of(heads, c->kv_heads); }
+
+// Waves of a workgroup that takes a whole pair, 0 where waves take runs of the line: by
+// the tiles that a page table can hold, which is all the host knows of the lengths.  One
+// launch, but the longest pair sets its end, so up to 32 tiles, and 64 where many pairs
+// follow each other on every CU.  us, line and pairs, 32 / 8 heads of 128, up to 1900
+// tokens: 256 sequences 203, 185 (Q8_0, equal), 148, 135 (BF16, ragged); 128 112, 100
+// and 79, 81; 64 57.9, 52.3 and 26.3, 32.3 (Q8_0, ragged).  Eight waves a pair while a
+// CU has not more than two pairs, then four, of which three fit: us with 8 and 4, up to
+// 900 tokens, 16 sequences 12.6, 14.0; 64 30.9, 28.0; 256 112, 97.
+int pair_waves(const mq_kv_cache *c, int64_t pairs, int64_t max_pages) {
+  if (max_pages * (c->page_tokens / kTileTokens) > (pairs < 1024 ? 32 : 64)) return 0;
+  return pairs < 512 ? 8 : 4;
+}
 
 // Waves of the largest launch.  12 a CU where tiles are small; 8 where each has over
 // 8 KiB in flight (64 x 8192 tokens, 32 / 8 heads of 128: BF16 358 us against 371 with
@@ -714,7 +732,8 @@ bool by_pairs(const mq_kv_cache *c, int64_t max_pages) { return max_pages * (c->
 // BF16 22.8 against 24.0).
 int most_waves(const mq_kv_cache *c) { return cache_tile_bytes(c->dtype, c->head_dim) > 8192 ? 2048 : 3072; }
 
-// Waves of a launch over `batch` sequences of up to `tokens` tokens: a run each, and no more than the tiles there can be.
+// Waves of a launch over `batch` sequences of up to `max_pages` pages: a run each, and no
+// more than the tiles there can be.
 int waves_of(const mq_kv_cache *c, int64_t batch, int chunks, int64_t max_pages) {
   const int64_t units = batch * c->kv_heads * chunks * (max_pages * (c->page_tokens / kTileTokens));
   const int64_t w = (units + kWaves - 1) / kWaves * kWaves, most = most_waves(c);
@@ -726,7 +745,8 @@ int waves_of(const mq_kv_cache *c, int64_t batch, int chunks, int64_t max_pages)
 
 extern "C" size_t mq_cache_attention_scratch_size(const mq_kv_cache *c, int64_t batch, int heads, int64_t max_pages) {
   using namespace mq;
-  if (cache_fault(c) || batch <= 0 || heads < 1 || heads % c->kv_heads || max_pages <= 0 || by_pairs(c, max_pages))
+  if (cache_fault(c) || batch <= 0 || heads < 1 || heads % c->kv_heads || max_pages <= 0 ||
+      pair_waves(c, pairs_of(c, batch, heads), max_pages))
     return 0;
   const int group = heads / c->kv_heads;
   return (size_t)2 * waves_of(c, batch, chunks_of(heads, c->kv_heads), max_pages) *
@@ -778,10 +798,12 @@ extern "C" int mq_cache_attention(const mq_kv_cache *c, const void *q, int64_t q
                      heads, heads / c->kv_heads, chunks, waves, scale * 1.44269504f, static_cast<float *>(scratch)};
   hipStream_t s = static_cast<hipStream_t>(stream);
   with_cache_type(c, [&]<int T, int D>() {
-    if (by_pairs(c, max_pages)) {
-      hipLaunchKernelGGL((decode_kernel<T, D, true>), dim3((unsigned)(batch * c->kv_heads * chunks)), dim3(64 * kPairWaves), 0, s, a);
+    const int64_t pairs = pairs_of(c, batch, heads);
+    if (const int w = pair_waves(c, pairs, max_pages)) {
+      if (w == 8) hipLaunchKernelGGL((decode_kernel<T, D, 8>), dim3((unsigned)pairs), dim3(64 * 8), 0, s, a);
+      else hipLaunchKernelGGL((decode_kernel<T, D, 4>), dim3((unsigned)pairs), dim3(64 * 4), 0, s, a);
     } else {
-      hipLaunchKernelGGL((decode_kernel<T, D, false>), dim3((unsigned)(waves / kWaves)), dim3(64 * kWaves), 0, s, a);
+      hipLaunchKernelGGL((decode_kernel<T, D, 0>), dim3((unsigned)(waves / kWaves)), dim3(64 * kWaves), 0, s, a);
       hipLaunchKernelGGL(join_kernel<D>, dim3((unsigned)(batch * heads)), dim3(256), 0, s, a);
     }
   });

@@ -106,6 +106,23 @@ def test_ragged_batches(t):
 
 
 @gpu
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("t", TYPES, ids=lambda t: t.name)
+@pytest.mark.parametrize("count,heads,kv,longest", [(63, 16, 8, 300), (64, 16, 8, 300), (127, 8, 8, 1000), (128, 8, 8, 1000), (128, 8, 8, 2016),
+                                                    (128, 8, 8, 2017), (9, 120, 60, 1984), (31, 51, 17, 100)])
+def test_many_rows(t, dim, count, heads, kv, longest):
+    """About 512 and 1024 rows and tables of 32 and 64 tiles, where the split over workgroups changes."""
+    g = torch.Generator().manual_seed(count + longest)
+    lengths = [longest] + torch.randint(0, min(longest, 400), (count - 1,), generator=g).tolist()
+    b = _Batch(lengths, heads, kv, dim, t, page=32)
+    out = b.run()
+    assert _err(out, b.ref()) < BOUND
+    assert torch.equal(out, b.run())
+    for i, n in enumerate(lengths):
+        assert n or not out[i].any(), i
+
+
+@gpu
 @pytest.mark.parametrize("t", TYPES, ids=lambda t: t.name)
 @pytest.mark.parametrize("lengths,heads,kv", [([40000], 4, 1), ([70001, 3, 20000], 8, 2), ([9000] * 6, 8, 8)])
 def test_long_contexts(lengths, heads, kv, t):
@@ -300,6 +317,6 @@ def test_argument_checks():
 @pytest.mark.skipif(HIPCC is None, reason="hipcc not available")
 def test_kernels_do_not_spill(tmp_path):
     funcs = {k: v for k, v in _functions(_asm(tmp_path, "mq_decode.hip")).items() if "_kernel" in k}
-    assert len(funcs) == 14
+    assert len(funcs) == 20
     for name, (_, meta) in funcs.items():
         assert meta.get("ScratchSize", 0) == 0, (name, meta)
