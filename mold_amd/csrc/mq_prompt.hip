@@ -6,7 +6,7 @@
 //   out[i, h] = sum_{j <= i} p_ij v[j, g],  p_i = softmax_j(scale q[i, h] . k[j, g]),
 //
 // i, j inside one prompt and g = h / (heads / kv_heads), in one pass over the
-// keys with the running maximum and sum of the softmax (f32).
+// keys with a running maximum and sum of the softmax (f32).
 //
 // The wave's inner loop is the joint attention's: transposed scores S^T = K Q^T
 // (v_mfma_f32_32x32x16, a lane holds 16 keys of one query), probabilities as the
@@ -26,7 +26,15 @@
 //     diagonal half, the only one that mixes seen and unseen keys, looks for
 //     non-finite values among its V and, if there are any, adds them row by row
 //     (accumulate_seen).  Rows past a prompt's end are clamped to its last row,
-//     so no neighbour in the pack is ever read.
+//     so no neighbour in the pack is ever read;
+//   * few tiles are split over the keys, two waves a tile (split_tiles below).
+// Bound by the matrix cores and the softmax's VALU under the power limit where
+// prompts are long (32 / 8 heads of 128: one of 8192 tokens 511 us, 1076 TFLOP/s of
+// the pairs i >= j); by the tiles' own costs where they are short: 24 ragged
+// prompts, 7305 tokens, take 65 us (580), of which storing the rows is 13 and
+// reading q 8, as the waves that could hide them are few (two a SIMD: O, q and two
+// blocks of scores fill the registers, K and V half the LDS).  Workgroups that go
+// on to further tiles with the next one's K, V and q requested ahead were 4% slower.
 #include "../../include/moldq.h"
 #include "mq_attn.h"
 
@@ -133,7 +141,7 @@ __global__ __launch_bounds__(64 * W, D == 128 ? 2 : 3) void prompt_kernel(const 
   for (int d = 0; d < D / 32; ++d)
 #pragma unroll
     for (int e = 0; e < 16; ++e) o[d][e] = 0.f;
-  float m = -__FLT_MAX__, l = 0.f;  // running maximum (both halves) and this half's sum
+  float m = -__FLT_MAX__, bar = m, l = 0.f;  // running maximum (both halves) and this half's sum
 
   const int i16 = lane & 15;
   lds_char *ka[D / 16], *va[D / 32];
@@ -172,12 +180,19 @@ __global__ __launch_bounds__(64 * W, D == 128 ? 2 : 3) void prompt_kernel(const 
     for (int e = 1; e < 16; ++e) r = __builtin_fmaxf(r, s[e]);
     return r;
   };
+  // The maximum follows only where a score passes it by 2^8 and more, row by row (what a
+  // row adds up does not depend on the others): O is then rescaled in few of the halves.
+  // Probabilities reach 2^8 instead of 1, whose bf16 rounding is as large relative to them;
+  // only the largest is no longer exact.  Distance to 64 bits 0.0018 to 0.0019 with every
+  // step followed, 0.0018 to 0.0022 so (the result's own rounding alone is 0.0016); 8192
+  // tokens 549 -> 511 us, 24 ragged prompts 67.1 -> 64.5, 8 x 1000 x 12 heads of 64 26.9 -> 24.6.
   auto raise_max = [&](float mx) {
     mx = half_max(mx);
-    if (__any(mx > m)) {
-      const float mn = __builtin_fmaxf(m, mx);
+    if (__any(mx > bar)) {
+      const float mn = mx > bar ? mx : m;
       const float f = __builtin_amdgcn_exp2f((m - mn) * a.scale);
       m = mn;
+      bar = mn + 8.f / a.scale;
       l *= f;
 #pragma unroll
       for (int d = 0; d < D / 32; ++d)
@@ -447,9 +462,9 @@ int64_t places(int head_dim) { return head_dim == 128 ? 2 * kCus : 3 * kCus; }
 // Up to how many whole tiles they are split over the keys: a wave's half tile runs
 // 0.8 us on its CU alone, so that few long tiles leave the chip waiting for the
 // longest, while split ones fetch each key for half as many queries.  us, whole and
-// split, by tiles: 32 / 8 heads of 128, 64 (500 tokens, 16 / 8) 14.4, 11.3; 256 (1000)
-// 25.5, 20.8; 376 (1500) 36.0, 36.6; 512 (2048) 50.0, 53.4.  Heads of 64, 580 tiles
-// 24.5, 21.5; 632 45.0, 42.4; 768 26.6, 26.9; 1280 18.8, 23.7.
+// split, by tiles: 32 / 8 heads of 128, 64 (500 tokens, 16 / 8) 12.5, 10.5; 256 (1000)
+// 22.4, 18.6; 376 (1500) 32.5, 33.1; 512 (2048) 46.1, 49.5.  Heads of 64, 580 tiles
+// 22.6, 20.6; 632 41.2, 40.4; 768 24.7, 26.0; 1280 18.1, 23.5.
 int64_t split_tiles(int head_dim) { return head_dim == 128 ? 320 : 700; }
 
 // The bytes from a view's first element to past its last.

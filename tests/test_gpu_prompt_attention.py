@@ -106,6 +106,21 @@ def test_flat_and_one_hot_rows(sharp, scale):
 
 
 @gpu
+@pytest.mark.parametrize("run", [_run, _run_whole], ids=["parts", "whole"])
+@pytest.mark.parametrize("step", [0.01, 0.2, 0.3, 5.0, -0.2])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_rising_scores(dim, step, run):
+    """Scores that rise or fall from key to key by a little or by much, to maxima that differ by row and head."""
+    n = 700
+    q, k, v = (t.clone() for t in _inputs([n], 4, 2, dim))
+    at = torch.arange(n, device="cuda", dtype=torch.float32)
+    q[:, :, 0] = torch.tensor([1.0, 2.0, 4.0, 0.5], device="cuda", dtype=BF)
+    k[:, :, 0] = (at * step * dim ** 0.5)[:, None].to(BF)
+    k[:, :, 1] = (at % 7 * step * dim ** 0.5)[:, None].to(BF)
+    assert _err(run(q, k, v, [n]), _ref(q, k, v, [n])) < BOUND
+
+
+@gpu
 @pytest.mark.parametrize("dim", [64, 128])
 @pytest.mark.parametrize("bad", [float("nan"), float("inf"), float("-inf")])
 @pytest.mark.parametrize("which", ["k", "v"])
