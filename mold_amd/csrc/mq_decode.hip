@@ -726,11 +726,14 @@ int pair_waves(const mq_kv_cache *c, int64_t pairs, int64_t max_pages) {
   return pairs < 512 ? 8 : 4;
 }
 
-// Waves of the largest launch.  12 a CU where tiles are small; 8 where each has over
-// 8 KiB in flight (64 x 8192 tokens, 32 / 8 heads of 128: BF16 358 us against 371 with
-// 12, Q8_0 210 against 219, but Q4_0 143 against 147; 16 x 3500 x 20 heads of 64 in
-// BF16 22.8 against 24.0).
-int most_waves(const mq_kv_cache *c) { return cache_tile_bytes(c->dtype, c->head_dim) > 8192 ? 2048 : 3072; }
+// Waves of the largest launch: what the registers allow, 16 a CU with heads of 64 and 12
+// with 128, or 8 where each has over 8 KiB in flight.  us with 8, 12 and 16 a CU: 64 x
+// 8192 tokens, 32 / 8 heads of 128 in BF16 358, 371, Q8_0 210, 219, Q4_0 147, 143; heads
+// of 64, 32 x 8192 x 32 in Q8_0 206, 208, 201, Q4_0 181, 158, 148, BF16 373, 382, 383; 16
+// ragged ones up to 3500 x 20 in Q4_0 17.0, 16.2, 15.6, BF16 23.6, 22.4, 22.1.
+int most_waves(const mq_kv_cache *c) {
+  return c->head_dim == 64 ? 4096 : cache_tile_bytes(c->dtype, c->head_dim) > 8192 ? 2048 : 3072;
+}
 
 // Waves of a launch over `batch` sequences of up to `max_pages` pages: a run each, and no
 // more than the tiles there can be.
