@@ -119,7 +119,7 @@ struct Rows {
     const int64_t row = row0 + i, slot = row < count ? slots[row] : -1;
     const int64_t first = ((int64_t)__builtin_amdgcn_readfirstlane((int)(slot >> 32)) << 32) |
                           (uint32_t)__builtin_amdgcn_readfirstlane((int)slot);
-    if (__all(slot == first + i) && first >= 0 && first + kRows <= c.slots && first % kTileTokens == 0) {
+    if (__all((uint64_t)slot - (uint64_t)first == (uint64_t)i) && first >= 0 && first <= c.slots - kRows && first % kTileTokens == 0) {
       int t;
       tile = data + place(c, head, first, t);
     } else if (slot >= 0 && slot < c.slots) {

@@ -129,6 +129,22 @@ def test_slots_outside_the_cache(t):
 
 
 @gpu
+@pytest.mark.parametrize("t", TYPES, ids=lambda t: t.name)
+@pytest.mark.parametrize("first", [64, 1 << 31, 1 << 32, (1 << 63) - 32, -32, -(1 << 63)])
+def test_whole_tiles_outside_the_cache(t, first):
+    """Slots in the order of a tile, just past the cache's end and as far out as slots go."""
+    cache = TA.KvCache(2, 2, 64, page_tokens=32, dtype=t)
+    cache.data.fill_(7)
+    guard = cache.data.clone()
+    slots = torch.arange(32, device="cuda") + first
+    new = _rows(32, 2, 64, seed=2)
+    cache.append(new[0], new[1], slots)
+    assert torch.equal(cache.data, guard)
+    k, v = cache.read(slots)
+    assert not k.any() and not v.any()
+
+
+@gpu
 @pytest.mark.parametrize("dtype", [torch.float32, BF], ids=["f32", "bf16"])
 def test_views(dtype):
     """Views of a stacked projection, head-major rows, one head for all, rows off 16 bytes."""
