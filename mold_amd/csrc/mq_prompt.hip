@@ -187,8 +187,8 @@ __global__ __launch_bounds__(64 * W, D == 128 ? 2 : 3) void prompt_kernel(const 
   // step followed, 0.0018 to 0.0022 so (the result's own rounding alone is 0.0016); 8192
   // tokens 549 -> 511 us, 24 ragged prompts 67.1 -> 64.5, 8 x 1000 x 12 heads of 64 26.9 -> 24.6.
   auto raise_max = [&](float mx) {
-    mx = half_max(mx);
-    if (__any(mx > bar)) {
+    if (__any(mx > bar)) {  // mx: this half's; the row's is looked up only here
+      mx = half_max(mx);
       const float mn = mx > bar ? mx : m;
       const float f = __builtin_amdgcn_exp2f((m - mn) * a.scale);
       m = mn;
