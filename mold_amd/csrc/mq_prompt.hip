@@ -28,13 +28,14 @@
 //     (accumulate_seen).  Rows past a prompt's end are clamped to its last row,
 //     so no neighbour in the pack is ever read;
 //   * few tiles are split over the keys, two waves a tile (split_tiles below).
-// Bound by the waves' chains of scores, softmax and second product where prompts
-// are long (32 / 8 heads of 128: one of 8192 tokens 503 us, 1093 TFLOP/s of the
-// pairs i >= j, the matrix cores 0.57 busy); by the tiles' own costs where they are
-// short: 24 ragged prompts, 7305 tokens, take 64 us (590), of which storing rows is 13 and
-// reading q 8, as the waves that could hide them are few (two a SIMD: O, q and two
-// blocks of scores fill the registers, K and V half the LDS).  Workgroups that go
-// on to further tiles with the next one's K, V and q requested ahead were 4% slower.
+// Bound by the matrix cores and the softmax at the clock that the power limit leaves
+// where prompts are long (32 / 8 heads of 128: one of 8192 tokens 503 us, 1093
+// TFLOP/s of the pairs i >= j, the matrix cores 0.57 busy at 1.8 GHz); by the tiles'
+// own costs where they are short: 24 ragged prompts, 7305 tokens, take 64 us (590),
+// of which storing rows is 13 and reading q 8, as the waves that could hide them are
+// few (two a SIMD: O, q and two blocks of scores fill the registers, K and V half the
+// LDS).  Workgroups that go on to further tiles with the next one's K, V and q
+// requested ahead were 4% slower.
 #include "../../include/moldq.h"
 #include "mq_attn.h"
 
