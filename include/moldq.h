@@ -81,7 +81,10 @@ int mq_version(void);
 int mq_block_size(int dtype);
 int mq_type_size(int dtype);
 
-/* Device context (candle Device::new_cuda(ordinal), device.rs:165). */
+/* Device context (candle Device::new_cuda(ordinal), device.rs:165).  Destroying it
+ * waits for the device and releases its workspaces; its tensors stay to be freed, before
+ * or after, and an arena goes with the last of them.  No other call takes a context, or
+ * a tensor of it, after its destruction. */
 int mq_ctx_create(int device_ordinal, mq_ctx **out);
 void mq_ctx_destroy(mq_ctx *ctx);
 /* Pre-allocate one HBM arena that later uploads are carved from (bump

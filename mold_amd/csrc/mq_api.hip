@@ -25,8 +25,11 @@ static __device__ __align__(256) uint8_t scratch[MQ_NOALLOC_SCRATCH_BYTES];
 
 struct mq_ctx {
   int device = 0;
+  // The context's own (until mq_ctx_destroy) and one of each of its tensors, which need
+  // its device and its arena until they are freed: a collector may free them in any order.
+  std::atomic<int64_t> refs{1};
   int cu_count = 0;
-  // HBM arena: one allocation, bump-allocated by uploads, freed with the ctx.
+  // HBM arena: one allocation, bump-allocated by uploads, freed with the last reference.
   uint8_t *arena = nullptr;
   size_t arena_size = 0;
   size_t arena_used = 0;
@@ -136,6 +139,15 @@ int check_weight_shape(int dtype, int64_t n, int64_t k, size_t nbytes) {
   if (nbytes != want)
     return fail(MQ_E_INVALID, "%s [%lld, %lld] is %zu bytes, got %zu", name, (long long)n, (long long)k, want, nbytes);
   return MQ_OK;
+}
+
+void release(mq_ctx *ctx) {
+  if (ctx->refs.fetch_sub(1, std::memory_order_acq_rel) != 1) return;
+  if (ctx->arena) {
+    DeviceGuard g(ctx->device);
+    (void)hipFree(ctx->arena);
+  }
+  delete ctx;
 }
 
 int alloc_weight(mq_ctx *ctx, mq_qtensor *t) {
@@ -344,6 +356,7 @@ int make_tensor(mq_ctx *ctx, int dtype, int64_t n, int64_t k, mq_qtensor **out) 
     delete t;
     return rc;
   }
+  ctx->refs.fetch_add(1, std::memory_order_relaxed);
   *out = t;
   return MQ_OK;
 }
@@ -554,20 +567,21 @@ int mq_ctx_create(int device_ordinal, mq_ctx **out) {
 
 void mq_ctx_destroy(mq_ctx *ctx) {
   if (!ctx) return;
-  DeviceGuard g(ctx->device);
-  (void)hipDeviceSynchronize();
-  for (auto &w : ctx->ws)
-    if (w.p) (void)hipFree(w.p);
-  for (void *p : ctx->retired) (void)hipFree(p);
-  for (auto *p : ctx->dstage)
-    if (p) (void)hipFree(p);
-  for (auto *p : ctx->pinned)
-    if (p) (void)hipHostFree(p);
-  for (auto s : ctx->copy_streams)
-    if (s) (void)hipStreamDestroy(s);
-  if (ctx->upload_stream) (void)hipStreamDestroy(ctx->upload_stream);
-  if (ctx->arena) (void)hipFree(ctx->arena);
-  delete ctx;
+  {
+    DeviceGuard g(ctx->device);
+    (void)hipDeviceSynchronize();
+    for (auto &w : ctx->ws)
+      if (w.p) (void)hipFree(w.p);
+    for (void *p : ctx->retired) (void)hipFree(p);
+    for (auto *p : ctx->dstage)
+      if (p) (void)hipFree(p);
+    for (auto *p : ctx->pinned)
+      if (p) (void)hipHostFree(p);
+    for (auto s : ctx->copy_streams)
+      if (s) (void)hipStreamDestroy(s);
+    if (ctx->upload_stream) (void)hipStreamDestroy(ctx->upload_stream);
+  }
+  release(ctx);
 }
 
 int mq_ctx_reserve_arena(mq_ctx *ctx, size_t bytes) {
@@ -819,6 +833,7 @@ void mq_qtensor_free(mq_qtensor *w) {
     DeviceGuard g(w->ctx->device);
     (void)hipFree(w->data);
   }
+  release(w->ctx);
   delete w;
 }
 
