@@ -221,6 +221,8 @@ class KvCache:
 
     def read(self, slots, dtype=torch.bfloat16):
         """(k, v) [tokens, kv_heads, head_dim] of `slots`, bf16 or f32; zeros for a slot outside the cache."""
+        if recorded(slots):
+            raise ValueError("KvCache.read: inference only, nothing may record the call")
         slots = self._slots("KvCache.read", slots)
         if dtype not in (torch.bfloat16, torch.float32):
             raise ValueError("KvCache.read: dtype must be bf16 or f32")
