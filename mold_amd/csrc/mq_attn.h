@@ -1,5 +1,5 @@
-// mq_attn.h — what the attention kernels share: the LDS DMA and its barrier,
-// the exchange between a wave's halves, and the rounding of a pair to bf16.
+// mq_attn.h — what the attention kernels share: the scale they take, the LDS DMA and its
+// barrier, the exchange between a wave's halves, and the rounding of a pair to bf16.
 #pragma once
 
 #include "mq_kernels.h"
@@ -9,6 +9,17 @@ namespace {
 
 typedef __attribute__((address_space(3))) char lds_char;
 typedef short s16x4 __attribute__((ext_vector_type(4)));
+
+constexpr float kLog2e = 1.44269504f;
+
+// What a row's running maximum starts at: a score below which scale (times log2(e)) s is no
+// finite f32, so that the maximum times the scale always is one, also while every score
+// seen is minus infinity: each then weighs 2^-inf, and not 2^(-inf + inf).  The last bits
+// are room for the division's and the product's roundings.
+inline float least_score(float scale) {
+  const float s = scale * kLog2e;
+  return s > 1.f ? -__FLT_MAX__ * (1.f - 0x1p-22f) / s : -__FLT_MAX__;
+}
 
 // 16 bytes per lane from base + off straight into LDS (lane i at lds + 16 i);
 // base and lds are wave-uniform.  Read only after block_barrier.

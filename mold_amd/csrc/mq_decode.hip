@@ -55,6 +55,7 @@ struct DecodeArgs {
   int max_pages, batch, heads, group, chunks;  // chunks of 16 heads of a group
   int waves;
   float scale;                 // times log2(e)
+  float least;                 // what the running maximum starts at (least_score)
   float *partial;
 };
 
@@ -397,7 +398,7 @@ __global__ __launch_bounds__(64 * (P ? P : kWaves), P == 8 ? 2 : D == 128 ? 3 : 
     for (int b = 0; b < kB; ++b) qf[b] = operand(w[b]);
 #pragma unroll
     for (int c = 0; c < kC; ++c) o[c] = f32x4{0.f, 0.f, 0.f, 0.f};
-    m = -__FLT_MAX__;
+    m = a.least;
     l = 0.f;
     bad = n > a.max_pages * a.cache.page_tokens;
   };
@@ -798,7 +799,7 @@ extern "C" int mq_cache_attention(const mq_kv_cache *c, const void *q, int64_t q
   const DecodeArgs a{{static_cast<uint8_t *>(c->data), c->pages * c->page_tokens, c->page_tokens, c->kv_heads}, c->pages,
                      static_cast<const __bf16 *>(q), static_cast<__bf16 *>(out), q_batch_stride, q_head_stride,
                      out_batch_stride, out_head_stride, page_table, lengths, table_stride, (int)max_pages, (int)batch,
-                     heads, heads / c->kv_heads, chunks, waves, scale * 1.44269504f, static_cast<float *>(scratch)};
+                     heads, heads / c->kv_heads, chunks, waves, scale * kLog2e, least_score(scale), static_cast<float *>(scratch)};
   hipStream_t s = static_cast<hipStream_t>(stream);
   with_cache_type(c, [&]<int T, int D>() {
     const int64_t pairs = pairs_of(c, batch, heads);

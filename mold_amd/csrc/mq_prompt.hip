@@ -59,6 +59,7 @@ struct PromptArgs {
   int64_t total;           // rows of q
   int units, group, log_heads;  // head units (of 1 << log_heads heads), heads per k/v head
   float scale;             // times log2(e)
+  float least;             // what the running maximum starts at (least_score)
 };
 
 template <int S>
@@ -142,7 +143,7 @@ __global__ __launch_bounds__(64 * W, D == 128 ? 2 : 3) void prompt_kernel(const 
   for (int d = 0; d < D / 32; ++d)
 #pragma unroll
     for (int e = 0; e < 16; ++e) o[d][e] = 0.f;
-  float m = -__FLT_MAX__, bar = m, l = 0.f;  // running maximum (both halves) and this half's sum
+  float m = a.least, bar = m, l = 0.f;  // running maximum (both halves) and this half's sum
 
   const int i16 = lane & 15;
   lds_char *ka[D / 16], *va[D / 32];
@@ -568,7 +569,7 @@ extern "C" int mq_prompt_attention(const mq_prompt_plan *plan, const int32_t *ti
   const PromptArgs a{static_cast<const __bf16 *>(q), static_cast<const __bf16 *>(k), static_cast<const __bf16 *>(v),
                      static_cast<__bf16 *>(out), q_token_stride, k_token_stride, v_token_stride, out_token_stride,
                      q_head_stride, k_head_stride, v_head_stride, out_head_stride, reinterpret_cast<const int4 *>(tiles),
-                     plan->tokens, units, heads / kv, log_heads, scale * 1.44269504f};
+                     plan->tokens, units, heads / kv, log_heads, scale * kLog2e, least_score(scale)};
   hipStream_t s = static_cast<hipStream_t>(stream);
   auto launch = [&]<int D, int P>() {
     hipLaunchKernelGGL((prompt_kernel<D, kWaves, P>), dim3((unsigned)grid), dim3(64 * kWaves), 0, s, a);
