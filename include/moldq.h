@@ -318,7 +318,8 @@ int mq_prompt_plan_make(const int64_t *lengths, int64_t count, int heads, int kv
                         mq_prompt_plan *plan, int32_t *tiles, int64_t capacity);
 /* Causal attention inside each prompt of the pack: row i of a prompt attends to
  * its rows 0 .. i, query head h to k/v head h / (heads / kv_heads);
- * softmax(scale q . k) v with f32 scores, softmax and sums.  q, out: bf16, token
+ * softmax(scale q . k) v with f32 scores, softmax and sums, scale positive and a
+ * finite f32 also when multiplied by log2(e) (up to 2.3e38).  q, out: bf16, token
  * t and head h at t * token_stride + h * head_stride, unit stride inside a head;
  * k, v likewise with kv_heads.  16-byte aligned, strides multiples of 8 elements
  * below 2^24, out apart from q, k and v; tiles: the plan's, on the device.  What
@@ -365,7 +366,7 @@ int mq_kv_cache_read(const mq_kv_cache *cache, const int64_t *slots, int64_t cou
  * head h of sequence b at b * batch_stride + h * head_stride, 16-byte aligned,
  * strides multiples of 8 elements, out apart from q.  page_table and lengths are
  * device memory: the host neither reads them nor waits.  f32 scores, softmax and
- * sums.  A sequence of no tokens gives zeros; one that names a page outside the
+ * sums, scale as in mq_prompt_attention.  A sequence of no tokens gives zeros; one that names a page outside the
  * cache, or is longer than its max_pages pages, gives NaN.  scratch: at least
  * mq_cache_attention_scratch_size bytes (device, 16-byte aligned, of this call
  * alone).  Asynchronous on stream; may be captured in a graph, whose replays

@@ -21,6 +21,9 @@ inline float least_score(float scale) {
   return s > 1.f ? -__FLT_MAX__ * (1.f - 0x1p-22f) / s : -__FLT_MAX__;
 }
 
+// Scales that the kernels take: scale log2(e) is a finite f32 too.
+inline bool takes_scale(float scale) { return scale > 0.f && scale * kLog2e <= __FLT_MAX__; }
+
 // 16 bytes per lane from base + off straight into LDS (lane i at lds + 16 i);
 // base and lds are wave-uniform.  Read only after block_barrier.
 __device__ __forceinline__ void dma16(const char *base, uint32_t off, uint32_t lds) {

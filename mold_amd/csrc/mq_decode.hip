@@ -766,7 +766,7 @@ extern "C" int mq_cache_attention(const mq_kv_cache *c, const void *q, int64_t q
   if (const char *fault = cache_fault(c)) return invalid(fault);
   if (batch < 0 || heads < 1 || heads > 65536 || heads % c->kv_heads)
     return invalid("mq_cache_attention: negative batch, or heads not a multiple of the cache's");
-  if (!(scale > 0.f) || scale > 3e38f) return invalid("mq_cache_attention: scale must be positive and finite");
+  if (!takes_scale(scale)) return invalid("mq_cache_attention: scale must be positive, and finite times log2(e)");
   if (max_pages < 0 || max_pages >= (int64_t(1) << 31) || max_pages * c->page_tokens >= (int64_t(1) << 31))
     return invalid("mq_cache_attention: a page table of 0 to 2^31 tokens");
   if (batch == 0) return MQ_OK;

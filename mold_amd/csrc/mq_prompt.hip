@@ -542,7 +542,7 @@ extern "C" int mq_prompt_attention(const mq_prompt_plan *plan, const int32_t *ti
       plan->tokens >= (int64_t(1) << 31) || plan->tiles < 0 || plan->tiles > plan->tokens || (plan->parts != 1 && plan->parts != 2) ||
       plan->tile_tokens != tile_tokens(heads / kv, plan->parts))
     return invalid("mq_prompt_attention: not a plan of mq_prompt_plan_make");
-  if (!(scale > 0.f) || scale > 3e38f) return invalid("mq_prompt_attention: scale must be positive and finite");
+  if (!takes_scale(scale)) return invalid("mq_prompt_attention: scale must be positive, and finite times log2(e)");
   if (plan->tokens == 0 || plan->tiles == 0) return MQ_OK;
   if (!tiles || !q || !k || !v || !out) return invalid("mq_prompt_attention: NULL pointer");
   if (!aligned16(tiles) || !aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(out))

@@ -5,11 +5,13 @@ has no value (0 / 0).
 
 Against float64; the bound is that of the finite cases (2.4e-3 from the roundings of
 probabilities and output to bf16, 3e-3 asserted over the rows that have a value)."""
+import ctypes
+
 import pytest
 
 torch = pytest.importorskip("torch")
 
-from mold_amd import GgmlDType
+from mold_amd import GgmlDType, _lib
 from mold_amd import text_attention as TA
 from tests.test_gpu_decode_attention import _Batch
 from tests.test_gpu_prompt_attention import _inputs, _ref, _run, _run_whole
@@ -83,3 +85,15 @@ def test_cache(dim, scale):
             ref = b.ref(scale)
             assert torch.isnan(ref).any() == (32 in lengths)
             _check(b.run(scale=scale), ref, (lengths, every))
+
+
+def test_scales_that_pass_float32_in_bits_are_refused():
+    """The kernels work in base 2: scale times log2(e) has to be a float32 too."""
+    lib, plan, n = _lib.load(), _lib.PromptPlanC(), (ctypes.c_int64 * 1)(3)
+    cache = _lib.KvCacheC(4096, 3, 30, 2, 64, 32)
+    assert lib.mq_prompt_plan_make(n, 1, 2, 2, 64, ctypes.byref(plan), None, 0) == 0
+    for scale in (2.4e38, 3e38, float("inf"), float("nan"), 0.0, -1.0):
+        args = (ctypes.byref(plan), 4096) + (4096, 128, 64) * 3 + (scale, 1 << 20, 128, 64, None)
+        assert lib.mq_prompt_attention(*args) == _lib.MQ_E_INVALID, scale
+        assert lib.mq_cache_attention(ctypes.byref(cache), 4096, 128, 64, 2, 2, 4096, 2, 2, 4096, scale, 1 << 20, 128, 64, None, 0,
+                                      None) == _lib.MQ_E_INVALID, scale
