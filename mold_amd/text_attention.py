@@ -47,9 +47,14 @@ def _operand(name, t, shape, device):
     st, sh, sd = t.stride()
     if sd != 1 or (st | sh) & 7 or st >= _MAX_STRIDE or sh >= _MAX_STRIDE or t.data_ptr() & 15:
         if not _readable(t):
-            t = t.contiguous()
+            t = _copied(t)
         st, sh = _strides(t)
     return t, st, sh
+
+
+def _copied(t):
+    """t's values packed and aligned; contiguous() would return a packed t as it is, off 16 bytes too."""
+    return t.clone(memory_format=torch.contiguous_format)
 
 
 def _readable(t):
@@ -215,7 +220,7 @@ class KvCache:
         if sd != 1 or (st | sh) & mask or st >= _MAX_STRIDE or sh >= _MAX_STRIDE or t.data_ptr() & 15:
             st, sh = _strides(t)
             if sd != 1 or (st | sh) & mask or st >= _MAX_STRIDE or sh >= _MAX_STRIDE or t.data_ptr() & 15:
-                t = t.contiguous()
+                t = _copied(t)
                 st, sh = _strides(t)
         return t, st, sh
 

@@ -1,4 +1,5 @@
-"""What the text attention's entry points take and refuse: calls that something records."""
+"""What the text attention's entry points take and refuse: calls that something records, tensors
+that start off 16 bytes."""
 import pytest
 
 torch = pytest.importorskip("torch")
@@ -7,6 +8,7 @@ from mold_amd import GgmlDType
 from mold_amd import text_attention as TA
 
 gpu = pytest.mark.gpu
+BF = torch.bfloat16
 
 
 def _cache(dtype=GgmlDType.BF16, tokens=40):
@@ -18,6 +20,13 @@ def _cache(dtype=GgmlDType.BF16, tokens=40):
     return cache, slots
 
 
+def _off(t):
+    """t's values in a contiguous tensor that starts one element off 16 bytes."""
+    off = torch.empty(t.numel() + 8, dtype=t.dtype, device=t.device)[1:t.numel() + 1].view(t.shape)
+    assert off.is_contiguous() and off.data_ptr() % 16
+    return off.copy_(t)
+
+
 @gpu
 def test_a_read_that_is_recorded_is_refused():
     """A trace would keep the allocations and not the kernel: its replay would return memory as it is."""
@@ -27,3 +36,32 @@ def test_a_read_that_is_recorded_is_refused():
     with torch.autograd.forward_ad.dual_level(), pytest.raises(ValueError):
         cache.read(slots)
     assert cache.read(slots)[0].shape == (40, 2, 64)
+
+
+@gpu
+@pytest.mark.parametrize("dim", [64, 128])
+def test_prompts_off_16_bytes(dim):
+    g = torch.Generator(device="cuda").manual_seed(1)
+    for n, heads, kv in ((50, 4, 2), (1, 1, 1)):
+        plan = TA.PromptPlan([n], heads, kv, dim)
+        q, k, v = (torch.randn((n, h, dim), device="cuda", generator=g).to(BF) for h in (heads, kv, kv))
+        want = TA.prompt_attention(q, k, v, plan)
+        for off in ((_off(q), k, v), (q, _off(k), v), (q, k, _off(v)), (_off(q), _off(k), _off(v))):
+            assert torch.equal(TA.prompt_attention(*off, plan), want), n
+        wide = torch.nn.functional.pad(q, (1, 7))[..., 1:dim + 1]     # of one token and head: contiguous too
+        assert torch.equal(TA.prompt_attention(wide, k, v, plan), want), n
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, BF], ids=["f32", "bf16"])
+def test_cache_calls_off_16_bytes(dtype):
+    g = torch.Generator(device="cuda").manual_seed(2)
+    slots = torch.arange(40, device="cuda")
+    k, v = torch.randn((2, 40, 2, 64), device="cuda", generator=g).to(dtype)
+    caches = [TA.KvCache(2, 2, 64, page_tokens=32, dtype=GgmlDType.Q8_0) for _ in range(4)]
+    for c, (a, b) in zip(caches, ((k, v), (_off(k), v), (k, _off(v)), (_off(k), _off(v)))):
+        c.append(a, b, slots)
+        assert all(torch.equal(x, y) for x, y in zip(c.read(slots), caches[0].read(slots)))
+    q = torch.randn((1, 4, 64), device="cuda", generator=g).to(BF)
+    table, n = torch.tensor([[0, 1]], dtype=torch.int32, device="cuda"), torch.tensor([40], dtype=torch.int32, device="cuda")
+    assert torch.equal(caches[0].attend(_off(q), table, n), caches[0].attend(q, table, n))
