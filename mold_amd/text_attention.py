@@ -150,7 +150,7 @@ def prompt_attention(q, k, v, plan: PromptPlan, scale=None, out=None):
     bf16 [tokens, kv_heads, dim] (views of one projection's output are read in place) ->
     bf16 [tokens, heads, dim], `out` if given.  scale defaults to dim ** -0.5."""
     device, n = plan.device, plan.tokens
-    if recorded(q, k, v):
+    if recorded(q, k, v) if out is None else recorded(q, k, v, out):
         raise ValueError("prompt_attention: inference only, nothing may record the call")
     q, qt, qh = _operand("prompt_attention: q", q, plan.q_shape, device)
     k, kt, kh = _operand("prompt_attention: k", k, plan.kv_shape, device)
@@ -245,7 +245,7 @@ class KvCache:
         page_table[b] (int32 [batch, pages]) -> bf16 [batch, heads, head_dim], `out` if given.
         scale defaults to head_dim ** -0.5.  Table and lengths are read on the device."""
         device, dim = self.device, self.head_dim
-        if recorded(q):
+        if recorded(q) if out is None else recorded(q, out):
             raise ValueError("KvCache.attend: inference only, nothing may record the call")
         if q.dim() != 3 or q.shape[1] == 0 or q.shape[1] % self.kv_heads:
             raise ValueError(f"KvCache.attend: q must be [batch, heads, {dim}] with a multiple of {self.kv_heads} heads")

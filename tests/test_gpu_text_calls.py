@@ -1,5 +1,5 @@
 """What the text attention's entry points take and refuse: calls that something records, tensors
-that start off 16 bytes."""
+that start off 16 bytes, an output that autograd watches."""
 import pytest
 
 torch = pytest.importorskip("torch")
@@ -65,3 +65,22 @@ def test_cache_calls_off_16_bytes(dtype):
     q = torch.randn((1, 4, 64), device="cuda", generator=g).to(BF)
     table, n = torch.tensor([[0, 1]], dtype=torch.int32, device="cuda"), torch.tensor([40], dtype=torch.int32, device="cuda")
     assert torch.equal(caches[0].attend(_off(q), table, n), caches[0].attend(q, table, n))
+
+
+@gpu
+def test_an_out_that_requires_gradients_is_refused():
+    """As any write in place into it; without gradient recording it is written."""
+    q, k, v = (torch.randn((8, 2, 64), device="cuda").to(BF) for _ in range(3))
+    plan = TA.PromptPlan([8], 2, 2, 64)
+    cache, _ = _cache()
+    table = torch.tensor([[0, 1]] * 8, dtype=torch.int32, device="cuda")
+    n = torch.arange(8, dtype=torch.int32, device="cuda")
+    for call in (lambda **kw: TA.prompt_attention(q, k, v, plan, **kw), lambda **kw: cache.attend(q, table, n, **kw)):
+        out = torch.zeros((8, 2, 64), device="cuda", dtype=BF, requires_grad=True)
+        for given in (out, out[:], (out * 1)):
+            with pytest.raises(ValueError):
+                call(out=given)
+        assert not out.detach().any()
+        with torch.no_grad():
+            assert call(out=out) is out
+        assert torch.equal(out.detach(), call())
