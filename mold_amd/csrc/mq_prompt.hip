@@ -551,12 +551,11 @@ extern "C" int mq_prompt_attention(const mq_prompt_plan *plan, const int32_t *ti
                     out_token_stride, out_head_stride})
     if (s < 0 || s % 8 || s >= (int64_t(1) << 24))
       return invalid("mq_prompt_attention: strides must be multiples of 8 elements, 0 to 2^24");
-  // rows and heads of out apart from each other
-  const int64_t small = std::min(heads > 1 ? out_head_stride : out_token_stride, out_token_stride);
-  const bool by_token = heads == 1 || out_token_stride >= out_head_stride;
-  if (small < dim || (heads > 1 && plan->tokens > 1 &&
-                      (by_token ? out_token_stride < (heads - 1) * out_head_stride + dim
-                                : out_head_stride < (plan->tokens - 1) * out_token_stride + dim)))
+  // rows and heads of out apart from each other; the stride of a single one may be anything
+  const bool rows = plan->tokens > 1, several = heads > 1;
+  if ((rows && out_token_stride < dim) || (several && out_head_stride < dim) ||
+      (rows && several && out_token_stride < (heads - 1) * out_head_stride + dim &&
+       out_head_stride < (plan->tokens - 1) * out_token_stride + dim))
     return invalid("mq_prompt_attention: rows or heads of out overlap");
   const Span o = span(out, plan->tokens, out_token_stride, heads, out_head_stride, dim);
   for (const Span &in : {span(q, plan->tokens, q_token_stride, heads, q_head_stride, dim),

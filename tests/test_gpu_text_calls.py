@@ -1,10 +1,12 @@
 """What the text attention's entry points take and refuse: calls that something records, tensors
-that start off 16 bytes, an output that autograd watches."""
+that start off 16 bytes, an output that autograd watches, one token's strides."""
+import ctypes
+
 import pytest
 
 torch = pytest.importorskip("torch")
 
-from mold_amd import GgmlDType
+from mold_amd import GgmlDType, _lib
 from mold_amd import text_attention as TA
 
 gpu = pytest.mark.gpu
@@ -84,3 +86,19 @@ def test_an_out_that_requires_gradients_is_refused():
         with torch.no_grad():
             assert call(out=out) is out
         assert torch.equal(out.detach(), call())
+
+
+@gpu
+def test_one_token_has_any_token_stride():
+    """A single row is not apart from another one: its token stride may be anything, 0 too."""
+    lib, plan, n = _lib.load(), _lib.PromptPlanC(), (ctypes.c_int64 * 1)(1)
+    for heads in (1, 4):
+        q, k, v = (torch.randn((1, heads, 64), device="cuda").to(BF) for _ in range(3))
+        tiles = TA.PromptPlan([1], heads, heads, 64)
+        assert lib.mq_prompt_plan_make(n, 1, heads, heads, 64, ctypes.byref(plan), None, 0) == 0
+        for stride in (0, 8, 64 * heads, 1 << 20):
+            out = torch.zeros_like(q)
+            args = [x for t in (q, k, v) for x in (t.data_ptr(), stride, 64)]
+            assert lib.mq_prompt_attention(ctypes.byref(plan), tiles.tiles.data_ptr(), *args, 0.125, out.data_ptr(), stride, 64,
+                                           torch.cuda.current_stream().cuda_stream) == 0, (heads, stride)
+            assert torch.equal(out, v), (heads, stride)
