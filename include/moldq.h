@@ -335,7 +335,8 @@ int mq_prompt_attention(const mq_prompt_plan *plan, const int32_t *tiles, const 
  * Q4_0 blocks along the head.  Slot s is token s % page_tokens of page s /
  * page_tokens.  `data` is mq_kv_cache_size bytes of device memory (16-byte
  * aligned) of the caller's, in a layout of the library's own; it needs no
- * clearing.  The size is 0 for a description that is not valid. */
+ * clearing.  The size is 0 for a description that is not valid (one of 2^63 bytes or
+ * more among them). */
 typedef struct mq_kv_cache {
     void *data;
     int64_t pages;

@@ -79,6 +79,9 @@ inline const char *cache_fault(const mq_kv_cache *c) {
   if (c->page_tokens < kTileTokens || c->page_tokens % kTileTokens || c->page_tokens > 65536)
     return "a cache's pages hold a multiple of 32 tokens, up to 65536";
   if (c->pages < 0 || c->pages >= (int64_t(1) << 31)) return "a cache has 0 to 2^31 pages";
+  int64_t size;  // a page alone is below 2^38
+  if (__builtin_mul_overflow(c->pages, c->kv_heads * (c->page_tokens / kTileTokens) * cache_tile_bytes(c->dtype, c->head_dim), &size))
+    return "a cache has less than 2^63 bytes";
   return nullptr;
 }
 

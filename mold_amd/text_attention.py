@@ -175,7 +175,8 @@ class KvCache:
         size = lib.mq_kv_cache_size(self._ref)
         if size == 0 and pages != 0:
             raise ValueError("KvCache: BF16, Q8_0 or Q4_0, heads of 64 or 128, pages of a multiple of 32 tokens up to 65536, "
-                             f"1 to 4096 heads; got {GgmlDType(dtype).name}, {head_dim}, {page_tokens}, {kv_heads}")
+                             f"1 to 4096 heads, less than 2^63 bytes; got {GgmlDType(dtype).name}, {head_dim}, {page_tokens}, "
+                             f"{kv_heads}, {pages} pages")
         self.data = torch.empty(size, dtype=torch.uint8, device=device)
         self.c.data = self.data.data_ptr()
         self.device = self.data.device
