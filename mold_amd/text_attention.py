@@ -187,10 +187,13 @@ class KvCache:
 
     def slots(self, page_table, positions):
         """The slots of `positions` [batch, n] of the sequences whose pages are page_table
-        [batch, pages]; -1 (skipped by append) for a negative position."""
+        [batch, pages]; -1 (skipped by append) for a negative position and one past the table."""
         at = positions.clamp(min=0).long()
-        page = torch.gather(page_table.long(), 1, at // self.page_tokens)
-        return torch.where(positions < 0, -1, page * self.page_tokens + at % self.page_tokens)
+        column, pages = at // self.page_tokens, page_table.shape[1]
+        if pages == 0:
+            return torch.full_like(at, -1)
+        page = torch.gather(page_table.long(), 1, column.clamp(max=pages - 1))
+        return torch.where((positions < 0) | (column >= pages), -1, page * self.page_tokens + at % self.page_tokens)
 
     def _slots(self, name, slots):
         if slots.dtype is not torch.int64 or slots.dim() != 1 or slots.device != self.device:
