@@ -9,7 +9,9 @@ block type) that `step` attends over.  Norms, rotations and the activation are t
 in float32; projections are QMatMul, attention and cache text_attention.
 
 `step` makes no host synchronization: lengths and page table stay on the device, so it can be
-captured in a graph.
+captured in a graph.  The graph goes on to a later prefill's sequences if there are as many and
+their page table is as wide; otherwise its replays write nothing and give NaN, and a step has to
+be captured anew.
 """
 from __future__ import annotations
 
@@ -59,6 +61,7 @@ class TextDecoder:
         self.caches = [KvCache(pages, config.kv_heads, config.head_dim, page_tokens, cache_dtype, device)
                        for _ in range(config.layers)]
         self.table = self.lengths = None
+        self._captured, self._retired = False, []     # what graphs of earlier batches hold
         half = config.head_dim // 2
         self._inv_freq = config.rope_theta ** (-torch.arange(half, device=device, dtype=torch.float32) / half)
 
@@ -122,13 +125,27 @@ class TextDecoder:
         pos = torch.cat([torch.arange(n) for n in lengths])
         seq = torch.repeat_interleave(torch.arange(len(lengths)), torch.tensor(lengths))
         slots = table.long()[seq, pos // self.page_tokens] * self.page_tokens + pos % self.page_tokens
-        self.table, slots, pos = (t.to(self.device) for t in (table, slots, pos))
-        self.lengths = torch.tensor(lengths, dtype=torch.int32, device=self.device)
+        self._begin(table, torch.tensor(lengths, dtype=torch.int32))
+        slots, pos = slots.to(self.device), pos.to(self.device)
         plan = PromptPlan(lengths, self.config.heads, self.config.kv_heads, self.config.head_dim, self.device)
         tokens = torch.tensor([t for p in prompts for t in p], device=self.device)
         x = self._forward(tokens, pos, slots, lambda layer, q, k, v: prompt_attention(q, k, v, plan))
         last = torch.cumsum(torch.tensor(lengths), 0) - 1
         return self._logits(x[last.to(self.device)])
+
+    def _begin(self, table, lengths):
+        """The sequences to step from here on, in the buffers of those before them if they fit, which a
+        captured step reads and writes.  Buffers that do not fit are kept for such a step, with
+        lengths past their table: it then writes nowhere and gives NaN."""
+        if self.table is not None and self.table.shape == table.shape:
+            self.table.copy_(table)
+            self.lengths.copy_(lengths)
+            return
+        if self._captured:
+            self.lengths.fill_(self.table.shape[1] * self.page_tokens)
+            self._retired.append((self.table, self.lengths))
+            self._captured = False
+        self.table, self.lengths = table.to(self.device), lengths.to(self.device)
 
     @torch.no_grad()
     def step(self, tokens):
@@ -136,6 +153,7 @@ class TextDecoder:
         A sequence past its pages has none left: its logits are NaN."""
         if self.lengths is None:
             raise ValueError("TextDecoder.step: prefill first")
+        self._captured |= torch.cuda.is_current_stream_capturing()
         pos = self.lengths.long()
         held = torch.full_like(pos, self.table.shape[1] * self.page_tokens)
         # past the table: written nowhere, and longer than its pages, which attention answers with NaN

@@ -1,0 +1,68 @@
+"""What a text decoder keeps between calls: the buffers that a captured step reads and writes."""
+import pytest
+
+torch = pytest.importorskip("torch")
+
+from mold_amd import GgmlDType
+from tests.test_gpu_text_decoder import PROMPTS, _decoder, model  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+OTHERS = [[9, 8], list(range(500, 566)), [1, 2, 3, 4, 5, 6, 7, 8, 9], [700] * 4]      # as wide a page table as PROMPTS'
+
+
+def _capture(dec, token):
+    """A step of dec in a graph, and its logits; dec stays where it is."""
+    start = dec.lengths.clone()
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        dec.step(token)                                      # workspaces of this stream
+        dec.lengths.copy_(start)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=s):
+            logits = dec.step(token)
+    torch.cuda.current_stream().wait_stream(s)
+    dec.lengths.copy_(start)
+    return graph, logits
+
+
+def _replay_beside(graph, logits, dec, eager, token, count):
+    for t in range(count):
+        want = eager.step(token)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(logits, want), t
+        assert dec.lengths.tolist() == eager.lengths.tolist()
+        token.copy_(want.argmax(-1))
+
+
+def test_captured_step_after_another_prefill(model):
+    eager, graphed = _decoder(model, GgmlDType.Q8_0), _decoder(model, GgmlDType.Q8_0)
+    token = eager.prefill(PROMPTS, room=20).argmax(-1)
+    graphed.prefill(PROMPTS, room=20)
+    graph, logits = _capture(graphed, token)
+    for prompts in (PROMPTS, OTHERS, PROMPTS[::-1]):
+        token.copy_(eager.prefill(prompts, room=20).argmax(-1))
+        graphed.prefill(prompts, room=20)
+        junk = [torch.full((4, 3), 12345, dtype=torch.int32, device="cuda") for _ in range(8)]
+        _replay_beside(graph, logits, graphed, eager, token, 6)
+        del junk
+
+
+def test_captured_step_after_a_prefill_of_another_shape(model):
+    """More sequences, or a wider table: the graph of before writes nothing and says so."""
+    for prompts, room in ((PROMPTS + [[1, 2]], 20), (PROMPTS, 90)):
+        eager, graphed = _decoder(model, GgmlDType.Q8_0), _decoder(model, GgmlDType.Q8_0)
+        token = eager.prefill(PROMPTS, room=20).argmax(-1)
+        graphed.prefill(PROMPTS, room=20)
+        graph, logits = _capture(graphed, token)
+        first = eager.prefill(prompts, room=room).argmax(-1)
+        graphed.prefill(prompts, room=room)
+        held = [c.data.clone() for c in graphed.caches]
+        for _ in range(3):
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.isnan(logits).all()
+        assert all(torch.equal(c.data, h) for c, h in zip(graphed.caches, held))
+        again, more = _capture(graphed, first)               # captured anew, it goes on
+        _replay_beside(again, more, graphed, eager, first, 4)
