@@ -153,15 +153,17 @@ class TextDecoder:
         A sequence past its pages has none left: its logits are NaN."""
         if self.lengths is None:
             raise ValueError("TextDecoder.step: prefill first")
+        if tokens.shape != self.lengths.shape or tokens.dtype not in (torch.int64, torch.int32) or tokens.device != self.lengths.device:
+            raise ValueError(f"TextDecoder.step: tokens must be int64 {list(self.lengths.shape)} on {self.lengths.device}")
         self._captured |= torch.cuda.is_current_stream_capturing()
-        pos = self.lengths.long()
+        pos, lengths = self.lengths.long(), self.lengths + 1
         held = torch.full_like(pos, self.table.shape[1] * self.page_tokens)
         # past the table: written nowhere, and longer than its pages, which attention answers with NaN
         slots = torch.where(pos < held, self.caches[0].slots(self.table, torch.minimum(pos, held - 1)[:, None])[:, 0], -1)
-        self.lengths += 1
-        x = self._forward(tokens, pos, slots,
-                          lambda layer, q, k, v: self.caches[layer].attend(q, self.table, self.lengths))
-        return self._logits(x)
+        x = self._forward(tokens, pos, slots, lambda layer, q, k, v: self.caches[layer].attend(q, self.table, lengths))
+        logits = self._logits(x)
+        self.lengths.copy_(lengths)      # last: a step that fails has not moved the sequences on
+        return logits
 
     def generate(self, prompts: Sequence[Sequence[int]], count: int, stop: Optional[int] = None):
         """The `count` most likely next tokens of each prompt, one after another, [n, count]; a

@@ -1,4 +1,5 @@
-"""What a text decoder keeps between calls: the buffers that a captured step reads and writes."""
+"""What a text decoder keeps between calls: the buffers that a captured step reads and writes, and
+its sequences after a call that failed."""
 import pytest
 
 torch = pytest.importorskip("torch")
@@ -66,3 +67,24 @@ def test_captured_step_after_a_prefill_of_another_shape(model):
         assert all(torch.equal(c.data, h) for c, h in zip(graphed.caches, held))
         again, more = _capture(graphed, first)               # captured anew, it goes on
         _replay_beside(again, more, graphed, eager, first, 4)
+
+
+def test_a_refused_step_moves_nothing_on(model, monkeypatch):
+    """Wrong tokens, and a failure in the middle of a step: the next one gives what it would have."""
+    eager, dec = _decoder(model, GgmlDType.BF16), _decoder(model, GgmlDType.BF16)
+    token = eager.prefill(PROMPTS, room=20).argmax(-1)
+    dec.prefill(PROMPTS, room=20)
+    lengths = dec.lengths.tolist()
+    for bad in (token[:3], torch.cat([token, token[:1]]), token[:1], token[None], token[:, None], token[0], token.cpu(), token.float(), token > 3):
+        with pytest.raises(ValueError):
+            dec.step(bad)
+        assert dec.lengths.tolist() == lengths
+    with monkeypatch.context() as m:
+        m.setattr(dec, "_logits", lambda x: 1 / 0)
+        with pytest.raises(ZeroDivisionError):
+            dec.step(token)
+    assert dec.lengths.tolist() == lengths
+    for _ in range(3):
+        want = eager.step(token)
+        assert torch.equal(dec.step(token.int()), want)
+        token = want.argmax(-1)
