@@ -60,7 +60,7 @@ class TextDecoder:
         self.page_tokens, self.pages = page_tokens, pages
         self.caches = [KvCache(pages, config.kv_heads, config.head_dim, page_tokens, cache_dtype, device)
                        for _ in range(config.layers)]
-        self.table = self.lengths = None
+        self.table = self.lengths = self._buffers = None
         self._captured, self._retired = False, []     # what graphs of earlier batches hold
         half = config.head_dim // 2
         self._inv_freq = config.rope_theta ** (-torch.arange(half, device=device, dtype=torch.float32) / half)
@@ -110,7 +110,8 @@ class TextDecoder:
     @torch.no_grad()
     def prefill(self, prompts: Sequence[Sequence[int]], room: int = 0):
         """Start sequences from `prompts` (at least a token each), with pages for `room` more tokens
-        of each; returns the logits after each prompt's last token [n, vocab]."""
+        of each; returns the logits after each prompt's last token [n, vocab].  The sequences before
+        them end, also where it fails in the middle."""
         lengths = [len(p) for p in prompts]
         if not lengths or min(lengths) == 0:
             raise ValueError("TextDecoder.prefill: at least one prompt, of at least one token each")
@@ -125,25 +126,31 @@ class TextDecoder:
         pos = torch.cat([torch.arange(n) for n in lengths])
         seq = torch.repeat_interleave(torch.arange(len(lengths)), torch.tensor(lengths))
         slots = table.long()[seq, pos // self.page_tokens] * self.page_tokens + pos % self.page_tokens
-        self._begin(table, torch.tensor(lengths, dtype=torch.int32))
         slots, pos = slots.to(self.device), pos.to(self.device)
         plan = PromptPlan(lengths, self.config.heads, self.config.kv_heads, self.config.head_dim, self.device)
         tokens = torch.tensor([t for p in prompts for t in p], device=self.device)
-        x = self._forward(tokens, pos, slots, lambda layer, q, k, v: prompt_attention(q, k, v, plan))
         last = torch.cumsum(torch.tensor(lengths), 0) - 1
-        return self._logits(x[last.to(self.device)])
+        self._end()
+        x = self._forward(tokens, pos, slots, lambda layer, q, k, v: prompt_attention(q, k, v, plan))
+        logits = self._logits(x[last.to(self.device)])
+        self._begin(table, torch.tensor(lengths, dtype=torch.int32))
+        return logits
+
+    def _end(self):
+        """The sequences end, their pages are free.  A captured step that still reads their buffers
+        finds lengths past the table: it writes nowhere and gives NaN."""
+        if self.lengths is not None:
+            self.lengths.fill_(self.table.shape[1] * self.page_tokens)
+            self._buffers, self.table, self.lengths = (self.table, self.lengths), None, None
 
     def _begin(self, table, lengths):
         """The sequences to step from here on, in the buffers of those before them if they fit, which a
-        captured step reads and writes.  Buffers that do not fit are kept for such a step, with
-        lengths past their table: it then writes nowhere and gives NaN."""
-        if self.table is not None and self.table.shape == table.shape:
-            self.table.copy_(table)
-            self.lengths.copy_(lengths)
+        captured step reads and writes; buffers that do not fit are kept for such a step."""
+        if self._buffers is not None and self._buffers[0].shape == table.shape:
+            self.table, self.lengths = self._buffers[0].copy_(table), self._buffers[1].copy_(lengths)
             return
         if self._captured:
-            self.lengths.fill_(self.table.shape[1] * self.page_tokens)
-            self._retired.append((self.table, self.lengths))
+            self._retired.append(self._buffers)
             self._captured = False
         self.table, self.lengths = table.to(self.device), lengths.to(self.device)
 

@@ -88,3 +88,29 @@ def test_a_refused_step_moves_nothing_on(model, monkeypatch):
         want = eager.step(token)
         assert torch.equal(dec.step(token.int()), want)
         token = want.argmax(-1)
+
+
+def test_a_failed_prefill_ends_the_sequences_before(model, monkeypatch):
+    """Their pages may hold the new prompts' keys by then: a step is refused, a captured one writes
+    nothing; the next prefill starts anew.  A prefill that is refused at once changes nothing."""
+    eager, dec = _decoder(model, GgmlDType.Q8_0), _decoder(model, GgmlDType.Q8_0)
+    token = eager.prefill(PROMPTS, room=20).argmax(-1)
+    dec.prefill(PROMPTS, room=20)
+    graph, logits = _capture(dec, token)
+    for bad in ([], [[1], []], [[1] * 64] * 30):
+        with pytest.raises(ValueError):
+            dec.prefill(bad)
+    _replay_beside(graph, logits, dec, eager, token, 2)
+    with monkeypatch.context() as m:
+        m.setattr(dec, "_logits", lambda x: 1 / 0)
+        with pytest.raises(ZeroDivisionError):
+            dec.prefill(OTHERS, room=20)
+    with pytest.raises(ValueError):
+        dec.step(token)
+    held = [c.data.clone() for c in dec.caches]
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.isnan(logits).all() and all(torch.equal(c.data, h) for c, h in zip(dec.caches, held))
+    token.copy_(eager.prefill(OTHERS, room=20).argmax(-1))
+    dec.prefill(OTHERS, room=20)
+    _replay_beside(graph, logits, dec, eager, token, 3)
