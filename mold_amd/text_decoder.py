@@ -128,7 +128,11 @@ class TextDecoder:
         slots = table.long()[seq, pos // self.page_tokens] * self.page_tokens + pos % self.page_tokens
         slots, pos = slots.to(self.device), pos.to(self.device)
         plan = PromptPlan(lengths, self.config.heads, self.config.kv_heads, self.config.head_dim, self.device)
-        tokens = torch.tensor([t for p in prompts for t in p], device=self.device)
+        tokens = torch.tensor([t for p in prompts for t in p])
+        vocab = self.weights["token_embd.weight"].shape[0]
+        if tokens.min() < 0 or tokens.max() >= vocab:
+            raise ValueError(f"TextDecoder.prefill: a token outside 0 .. {vocab - 1}")
+        tokens = tokens.to(self.device)
         last = torch.cumsum(torch.tensor(lengths), 0) - 1
         self._end()
         x = self._forward(tokens, pos, slots, lambda layer, q, k, v: prompt_attention(q, k, v, plan))
@@ -156,7 +160,7 @@ class TextDecoder:
 
     @torch.no_grad()
     def step(self, tokens):
-        """Append `tokens` (int64 [n], on the device) to the sequences; returns the logits after them.
+        """Append `tokens` (int64 [n], on the device, of the vocabulary) to the sequences; returns the logits after them.
         A sequence past its pages has none left: its logits are NaN."""
         if self.lengths is None:
             raise ValueError("TextDecoder.step: prefill first")

@@ -5,7 +5,7 @@ import pytest
 torch = pytest.importorskip("torch")
 
 from mold_amd import GgmlDType
-from tests.test_gpu_text_decoder import PROMPTS, _decoder, model  # noqa: F401
+from tests.test_gpu_text_decoder import PROMPTS, VOCAB, _decoder, model  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 OTHERS = [[9, 8], list(range(500, 566)), [1, 2, 3, 4, 5, 6, 7, 8, 9], [700] * 4]      # as wide a page table as PROMPTS'
@@ -114,3 +114,15 @@ def test_a_failed_prefill_ends_the_sequences_before(model, monkeypatch):
     token.copy_(eager.prefill(OTHERS, room=20).argmax(-1))
     dec.prefill(OTHERS, room=20)
     _replay_beside(graph, logits, dec, eager, token, 3)
+
+
+def test_tokens_outside_the_vocabulary_are_refused(model):
+    """On the host: on the GPU an index past the embedding is a device assertion, and -1 its last row."""
+    dec = _decoder(model, GgmlDType.BF16)
+    want = dec.prefill(PROMPTS, room=3)
+    for bad in (VOCAB, -1, 1 << 40):
+        with pytest.raises(ValueError):
+            dec.prefill([[1, 2], [3, bad, 4]])
+    assert dec.lengths.tolist() == [len(p) for p in PROMPTS]
+    assert torch.equal(dec.prefill(PROMPTS, room=3), want)
+    dec.prefill([[0, VOCAB - 1]])
