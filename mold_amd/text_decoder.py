@@ -115,6 +115,8 @@ class TextDecoder:
         lengths = [len(p) for p in prompts]
         if not lengths or min(lengths) == 0:
             raise ValueError("TextDecoder.prefill: at least one prompt, of at least one token each")
+        if room < 0:
+            raise ValueError(f"TextDecoder.prefill: room for {room} tokens")
         per = -(-(max(lengths) + room) // self.page_tokens)
         need = [-(-(n + room) // self.page_tokens) for n in lengths]
         if sum(need) > self.pages:
@@ -179,10 +181,12 @@ class TextDecoder:
     def generate(self, prompts: Sequence[Sequence[int]], count: int, stop: Optional[int] = None):
         """The `count` most likely next tokens of each prompt, one after another, [n, count]; a
         sequence repeats `stop` once it has given it."""
+        if count < 0:
+            raise ValueError(f"TextDecoder.generate: {count} tokens")
         token = self.prefill(prompts, room=count).argmax(-1)
         out = [token]
         for _ in range(count - 1):
             nxt = self.step(token).argmax(-1)
             token = nxt if stop is None else torch.where(token == stop, token, nxt)
             out.append(token)
-        return torch.stack(out, 1)
+        return torch.stack(out, 1)[:, :count]

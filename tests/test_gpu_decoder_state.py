@@ -126,3 +126,12 @@ def test_tokens_outside_the_vocabulary_are_refused(model):
     assert dec.lengths.tolist() == [len(p) for p in PROMPTS]
     assert torch.equal(dec.prefill(PROMPTS, room=3), want)
     dec.prefill([[0, VOCAB - 1]])
+
+
+def test_no_tokens_and_negative_counts(model):
+    dec = _decoder(model, GgmlDType.BF16)
+    for count in (0, 1, 2):
+        assert dec.generate(PROMPTS, count).shape == (len(PROMPTS), count)
+    for call in (lambda: dec.generate(PROMPTS, -1), lambda: dec.prefill(PROMPTS, room=-1), lambda: dec.prefill([[1] * 33], room=-2)):
+        with pytest.raises(ValueError):
+            call()
