@@ -3,7 +3,7 @@
 What mold's prompt expansion runs through candle's quantized_qwen3::ModelWeights
 (crates/mold-inference/src/expand.rs:200-203): RmsNorm, grouped-head attention with rotary
 halves and optional q/k head norms, and a SwiGLU MLP, with tensor names as GGUF files give
-them.  `prefill` takes a batch of prompts packed without padding, `step` one new token of each
+them (TextConfig.from_metadata and gguf.Content.var_builder make one of a file).  `prefill` takes a batch of prompts packed without padding, `step` one new token of each
 sequence; both write their keys and values into one paged cache (quantized where its type is a
 block type) that `step` attends over.  Norms, rotations and the activation are torch operations
 in float32; projections are QMatMul, attention and cache text_attention.
@@ -34,6 +34,18 @@ class TextConfig:
     rope_theta: float = 1e6
     eps: float = 1e-6
 
+    @classmethod
+    def from_metadata(cls, metadata: Dict[str, object]) -> "TextConfig":
+        """A GGUF file's (Content.metadata), by the keys of its architecture."""
+        arch = metadata["general.architecture"]
+        get = lambda key, default=None: metadata.get(f"{arch}.{key}", default)
+        sizes = {key: get(key) for key in ("embedding_length", "attention.head_count", "block_count")}
+        if None in sizes.values():
+            raise ValueError(f"TextConfig: the metadata has no {', '.join(f'{arch}.{k}' for k, v in sizes.items() if v is None)}")
+        hidden, heads, layers = sizes.values()
+        return cls(hidden, heads, get("attention.head_count_kv", heads), get("attention.key_length", hidden // heads), layers,
+                   get("rope.freq_base", cls.rope_theta), get("attention.layer_norm_rms_epsilon", cls.eps))
+
 
 def rms_norm(x, weight, eps: float):
     """float32 RmsNorm over the last axis."""
@@ -49,13 +61,17 @@ def rotate(x, cos, sin):
 
 
 class TextDecoder:
-    """weights: {GGUF name: QTensor for the projections, float32 tensor for token_embd.weight and
-    the norms}; `output.weight` falls back to the embedding, `attn_{q,k}_norm` and biases are
-    optional.  One layer's cache each, `pages` pages of `page_tokens` tokens."""
+    """weights: {GGUF name: QTensor (as Content.var_builder gives them all) or float32 tensor};
+    `output.weight` falls back to the embedding, `attn_{q,k}_norm` and biases are optional.
+    Projections of a block type stay as they are; the embedding, norms, biases and whatever is
+    stored dense are held in float32.  One layer's cache each, `pages` pages of `page_tokens` tokens."""
 
     def __init__(self, config: TextConfig, weights: Dict[str, object], pages: int, page_tokens: int = 64,
                  cache_dtype: GgmlDType = GgmlDType.Q8_0, device="cuda"):
-        self.config, self.weights = config, weights
+        self.config = config
+        self.weights = {name: self._dense(name, w) if isinstance(w, QTensor) else w for name, w in weights.items()}
+        if self._blocks(weights["token_embd.weight"]):
+            self.weights.setdefault("output.weight", weights["token_embd.weight"])
         self.device = torch.device(device)
         self.page_tokens, self.pages = page_tokens, pages
         self.caches = [KvCache(pages, config.kv_heads, config.head_dim, page_tokens, cache_dtype, device)
@@ -64,6 +80,16 @@ class TextDecoder:
         self._captured, self._retired = False, []     # what graphs of earlier batches hold
         half = config.head_dim // 2
         self._inv_freq = config.rope_theta ** (-torch.arange(half, device=device, dtype=torch.float32) / half)
+
+    @staticmethod
+    def _blocks(w) -> bool:
+        return isinstance(w, QTensor) and w.dtype().is_quantized
+
+    def _dense(self, name: str, w: QTensor):
+        """w as it is used: a projection in blocks as it is, anything else in float32, a vector as one."""
+        if name.endswith("norm.weight") or name.endswith(".bias"):
+            return w.dequantize().reshape(-1)
+        return w if self._blocks(w) and name != "token_embd.weight" else w.dequantize()
 
     def _linear(self, name: str, x, out_dtype=torch.float32):
         bias = self.weights.get(name + ".bias")
