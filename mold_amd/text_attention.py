@@ -20,23 +20,34 @@ import torch
 from . import _lib
 from ._lib import check
 from .fused import recorded
-from .quantized import GgmlDType, _dtype_code, _stream_ptr
+from .quantized import GgmlDType, _dtype_code
 
 _MAX_STRIDE = 1 << 24
 _BF16 = torch.bfloat16
 
 
-def _run(device, fn, *args):
-    """fn(*args, torch's current stream) with `device` current, as it mostly is (making it so
-    takes 1.3 us of a 9 us call)."""
-    current = torch._C._cuda_getDevice()
-    if current == device.index:
-        rc = fn(*args, torch._C._cuda_getCurrentRawStream(current))
-    else:
-        with torch.cuda.device(device):
-            rc = fn(*args, _stream_ptr())
-    if rc:
-        check(rc)
+class _OnStreams:
+    """Device memory that an object keeps for its calls, told to the allocator for each stream that
+    they run on: memory of an object that is dropped is given out again only after them."""
+
+    def __init__(self, t):
+        self.t, self.device = t, t.device
+        self.streams = {torch._C._cuda_getCurrentRawStream(t.device.index)}
+
+    def run(self, fn, *args):
+        """fn(*args, torch's current stream) with the device current, as it mostly is (making it so
+        takes 1.3 us of a 9 us call)."""
+        current = torch._C._cuda_getDevice()
+        if current != self.device.index:
+            with torch.cuda.device(self.device):
+                return self.run(fn, *args)
+        stream = torch._C._cuda_getCurrentRawStream(current)
+        if stream not in self.streams:
+            self.t.record_stream(torch.cuda.current_stream())
+            self.streams.add(stream)
+        rc = fn(*args, stream)
+        if rc:
+            check(rc)
 
 
 def _operand(name, t, shape, device):
@@ -143,6 +154,7 @@ class PromptPlan:
         self.q_shape = (self.tokens, self.heads, self.head_dim)
         self.kv_shape = (self.tokens, self.kv_heads, self.head_dim)
         self._ref, self._tiles = ctypes.byref(self.c), self.tiles.data_ptr()
+        self._run = _OnStreams(self.tiles).run
 
 
 def prompt_attention(q, k, v, plan: PromptPlan, scale=None, out=None):
@@ -157,8 +169,8 @@ def prompt_attention(q, k, v, plan: PromptPlan, scale=None, out=None):
     v, vt, vh = _operand("prompt_attention: v", v, plan.kv_shape, device)
     res, ot, oh = _out("prompt_attention", out, plan.q_shape, device, (q, k, v))
     if n:
-        _run(device, _lib.load().mq_prompt_attention, plan._ref, plan._tiles, q.data_ptr(), qt, qh, k.data_ptr(), kt, kh,
-             v.data_ptr(), vt, vh, plan.head_dim ** -0.5 if scale is None else scale, res.data_ptr(), ot, oh)
+        plan._run(_lib.load().mq_prompt_attention, plan._ref, plan._tiles, q.data_ptr(), qt, qh, k.data_ptr(), kt, kh,
+                  v.data_ptr(), vt, vh, plan.head_dim ** -0.5 if scale is None else scale, res.data_ptr(), ot, oh)
     return _given(out, res)
 
 
@@ -184,6 +196,7 @@ class KvCache:
             raise ValueError(f"KvCache: a GPU's, not {self.device}")
         self.pages, self.kv_heads, self.head_dim, self.page_tokens = int(pages), int(kv_heads), int(head_dim), int(page_tokens)
         self.dtype = GgmlDType(dtype)
+        self._run = _OnStreams(self.data).run
 
     def slots(self, page_table, positions):
         """The slots of `positions` [batch, n] of the sequences whose pages are page_table
@@ -213,8 +226,8 @@ class KvCache:
         k, kt, kh = self._rows(k, shape, dtype)
         v, vt, vh = self._rows(v, shape, dtype)
         if n:
-            _run(self.device, _lib.load().mq_kv_cache_append, self._ref, k.data_ptr(), kt, kh, v.data_ptr(), vt, vh,
-                 _dtype_code(dtype), n, slots.data_ptr())
+            self._run(_lib.load().mq_kv_cache_append, self._ref, k.data_ptr(), kt, kh, v.data_ptr(), vt, vh,
+                      _dtype_code(dtype), n, slots.data_ptr())
 
     def _rows(self, t, shape, dtype):
         if t.dtype is not dtype or t.shape != shape or t.device != self.device:
@@ -239,8 +252,8 @@ class KvCache:
         k = torch.empty(shape, dtype=dtype, device=self.device)
         v = torch.empty_like(k)
         if shape[0]:
-            _run(self.device, _lib.load().mq_kv_cache_read, self._ref, slots.data_ptr(), shape[0], k.data_ptr(), v.data_ptr(),
-                 _dtype_code(dtype))
+            self._run(_lib.load().mq_kv_cache_read, self._ref, slots.data_ptr(), shape[0], k.data_ptr(), v.data_ptr(),
+                      _dtype_code(dtype))
         return k, v
 
     def attend(self, q, page_table, lengths, scale=None, out=None):
@@ -268,7 +281,8 @@ class KvCache:
             lib = _lib.load()
             nbytes = lib.mq_cache_attention_scratch_size(self._ref, n, heads, pages)
             scratch = self.data.new_empty(nbytes) if nbytes else None     # freed to this stream
-            _run(device, lib.mq_cache_attention, self._ref, q.data_ptr(), qb, qh, n, heads, page_table.data_ptr(),
-                 page_table.stride(0) if n > 1 else pages, pages, lengths.data_ptr(), dim ** -0.5 if scale is None else scale,
-                 res.data_ptr(), ob, oh, scratch.data_ptr() if nbytes else None, nbytes)
+            self._run(lib.mq_cache_attention, self._ref, q.data_ptr(), qb, qh, n, heads, page_table.data_ptr(),
+                      page_table.stride(0) if n > 1 else pages, pages, lengths.data_ptr(),
+                      dim ** -0.5 if scale is None else scale, res.data_ptr(), ob, oh, scratch.data_ptr() if nbytes else None,
+                      nbytes)
         return _given(out, res)
