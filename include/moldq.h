@@ -299,9 +299,9 @@ int mq_attention_bf16(const void *q, const void *k, const void *v, int64_t batch
  * it needs none.  With less, or NULL, it runs without. */
 size_t mq_attention_scratch_size(int64_t batch, int heads, int64_t valid);
 
-/* --- Text attention: the layers between a GGUF text model's linears (the text
- *     encoders of crates/mold-inference/src/encoders and the prompt-expansion
- *     model of src/expand.rs:200-203, whose attention candle composes of
+/* --- Text attention: the layers between a GGUF text model's linears (the Qwen
+ *     text encoders, crates/mold-inference/src/encoders/qwen3_gguf.rs and
+ *     qwen2_text_gguf.rs, and the prompt-expansion model of src/expand.rs:200-203, whose attention candle composes of
  *     matmul, mask and softmax and whose cache grows by concatenation). ------ */
 
 /* How packed prompts of given lengths are attended: made once per batch, used

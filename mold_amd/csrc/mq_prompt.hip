@@ -1,7 +1,8 @@
 // mq_prompt.hip — causal attention of whole prompts: packed sequences of
-// different lengths, grouped heads, what a text encoder's or a decoder's layer
-// runs between its projections (the GGUF text encoders and the prompt-expansion
-// model of crates/mold-inference/src/encoders and src/expand.rs:200-203).
+// different lengths, grouped heads, what a decoder's layer runs between its
+// projections, or an encoder's that is one (the Qwen text encoders,
+// crates/mold-inference/src/encoders/qwen3_gguf.rs and qwen2_text_gguf.rs, and the
+// prompt-expansion model, src/expand.rs:200-203; T5 attends both ways, with a bias).
 //
 //   out[i, h] = sum_{j <= i} p_ij v[j, g],  p_i = softmax_j(scale q[i, h] . k[j, g]),
 //
@@ -29,10 +30,10 @@
 //     so no neighbour in the pack is ever read;
 //   * few tiles are split over the keys, two waves a tile (split_tiles below).
 // Bound by the matrix cores and the softmax at the clock that the power limit leaves
-// where prompts are long (32 / 8 heads of 128: one of 8192 tokens 503 us, 1093
-// TFLOP/s of the pairs i >= j, the matrix cores 0.57 busy at 1.8 GHz); by the tiles'
-// own costs where they are short: 24 ragged prompts, 7305 tokens, take 64 us (590),
-// of which storing rows is 13 and reading q 8, as the waves that could hide them are
+// where prompts are long (32 / 8 heads of 128: one of 8192 tokens 499 to 544 us by box,
+// 1010 to 1102 TFLOP/s of the pairs i >= j, the matrix cores 0.57 busy at 1.8 GHz); by the
+// tiles' own costs where they are short: 24 ragged prompts, 7305 tokens, take 62 to 70 us
+// (538 to 607), of which storing rows is 13 and reading q 8, as the waves that could hide them are
 // few (two a SIMD: O, q and two blocks of scores fill the registers, K and V half the
 // LDS).  Workgroups that go on to further tiles with the next one's K, V and q
 // requested ahead were 4% slower.
@@ -464,9 +465,14 @@ int64_t places(int head_dim) { return head_dim == 128 ? 2 * kCus : 3 * kCus; }
 // Up to how many whole tiles they are split over the keys: a wave's half tile runs
 // 0.8 us on its CU alone, so that few long tiles leave the chip waiting for the
 // longest, while split ones fetch each key for half as many queries.  us, whole and
-// split, by tiles: 32 / 8 heads of 128, 64 (500 tokens, 16 / 8) 12.5, 10.5; 256 (1000)
-// 22.4, 18.6; 376 (1500) 32.5, 33.1; 512 (2048) 46.1, 49.5.  Heads of 64, 580 tiles
-// 22.6, 20.6; 632 41.2, 40.4; 768 24.7, 26.0; 1280 18.1, 23.5.
+// split, by tiles and whatever the lengths are.  Heads of 128, 32 / 8: 56 (200 tokens) 9.4,
+// 9.5; 64 (500, 16 / 8) 12.1, 10.1; 256 (1000) 22.0, 18.2; 264 (three of up to 600) 16.3,
+// 14.1; 376 (1500) 31.0, 31.4; 512 (2048) 44.0, 47.8; 512 (4096, 16 / 8) 81.0, 85.5; 1936
+// (24 of up to 1000) 62, 87.  Heads of 64: 144 (four of up to 600, 12 / 12) 10.1, 9.6; 228
+// (eight) 10.7, 9.7; 580 (eight of up to 1500, 20 / 20) 21.1, 18.9; 632 (2500, 32 / 8) 39.1,
+// 38.5; 640 (4000, 20 / 20) 60.8, 57.5; 640 (2 x 2000) 33.8, 32.5; 768 (8 x 1000, 12 / 12)
+// 22.3, 23.9; 768 (16 x 512) 16.0, 17.9; 768 (64 x 77) 9.5, 11.7; 1024 (4096, 32 / 8) 83.1,
+// 89.1; 1280 (32 x 200, 20 / 20) 18.0, 23.6.
 int64_t split_tiles(int head_dim) { return head_dim == 128 ? 320 : 700; }
 
 // The bytes from a view's first element to past its last.

@@ -1,5 +1,5 @@
-"""Attention of the GGUF text models (text encoders, prompt expansion): whole prompts, and new
-tokens over a paged key/value cache, run by libmoldq (mq_prompt_attention, mq_kv_cache_* and
+"""Causal attention of the GGUF text models (the Qwen text encoders, prompt expansion): whole
+prompts, and new tokens over a paged key/value cache, run by libmoldq (mq_prompt_attention, mq_kv_cache_* and
 mq_cache_attention in include/moldq.h).
 
 candle composes both of matmul, mask and softmax and grows its cache by concatenation

@@ -3,10 +3,11 @@
 What mold's prompt expansion runs through candle's quantized_qwen3::ModelWeights
 (crates/mold-inference/src/expand.rs:200-203): RmsNorm, grouped-head attention with rotary
 halves and optional q/k head norms, and a SwiGLU MLP, with tensor names as GGUF files give
-them (TextConfig.from_metadata and gguf.Content.var_builder make one of a file).  `prefill` takes a batch of prompts packed without padding, `step` one new token of each
-sequence; both write their keys and values into one paged cache (quantized where its type is a
-block type) that `step` attends over.  Norms, rotations and the activation are torch operations
-in float32; projections are QMatMul, attention and cache text_attention.
+them (TextConfig.from_metadata and gguf.Content.var_builder make one of a file).  `prefill`
+takes a batch of prompts packed without padding, `step` one new token of each sequence; both
+write their keys and values into one paged cache (quantized where its type is a block type)
+that `step` attends over.  Norms, rotations and the activation are torch operations in float32;
+projections are QMatMul, attention and cache text_attention.
 
 `step` makes no host synchronization: lengths and page table stay on the device, so it can be
 captured in a graph.  The graph goes on to a later prefill's sequences if there are as many and
@@ -188,8 +189,8 @@ class TextDecoder:
 
     @torch.no_grad()
     def step(self, tokens):
-        """Append `tokens` (int64 [n], on the device, of the vocabulary) to the sequences; returns the logits after them.
-        A sequence past its pages has none left: its logits are NaN."""
+        """Append `tokens` (int64 [n], on the device, of the vocabulary) to the sequences; returns the
+        logits after them.  A sequence past its pages has none left: its logits are NaN."""
         if self.lengths is None:
             raise ValueError("TextDecoder.step: prefill first")
         if tokens.shape != self.lengths.shape or tokens.dtype not in (torch.int64, torch.int32) or tokens.device != self.lengths.device:
