@@ -234,6 +234,8 @@ def _prepare_reorder(case, seed):
             state["caches"][-1].data.copy_(x)
         else:
             state["pools"].append(x)
+    if own:
+        state["states"] = _beams().BeamStates(state["caches"])
     return state
 
 
@@ -361,7 +363,7 @@ def run(state):
         return state["cache"].place(state["counts"], state["tokens"], state["width"], room=state["room"], beams=state["beams"], pages=state["pages"])
     if op == "select":
         return _beams().select_beams(state["logits"], state["scores"], count=state["count"], last=state["last"], stop=state["stop"])
-    _beams().reorder_beams(state["caches"], state["table"], state["lengths"], state["parents"])
+    state["states"].reorder(state["table"], state["lengths"], state["parents"])
     return (state["table"], *(c.data for c in state["caches"]))
 
 
