@@ -378,6 +378,32 @@ int mq_cache_attention(const mq_kv_cache *cache, const void *q, int64_t q_batch_
                        int64_t out_head_stride, void *scratch, size_t scratch_bytes, void *stream);
 size_t mq_cache_attention_scratch_size(const mq_kv_cache *cache, int64_t batch, int heads, int64_t max_pages);
 
+/* --- The same models' steps between their projections and their attention.
+ *     candle's quantized_qwen3 (crates/mold-inference/src/expand.rs:200-203) composes them of
+ *     separate norms, rotations and concatenations. ---------------------------- */
+
+/* Every head of q and k [tokens, heads / kv_heads, head_dim], RmsNormed where its weight
+ * (f32 [head_dim]) is not NULL, x / sqrt(mean(x^2) + eps) * weight, and then its halves
+ * rotated by the token's position: with a = positions[t] * inv_freq[i], value i becomes
+ * x_i cos a - x_(i+D/2) sin a and value i + D/2 becomes x_(i+D/2) cos a + x_i sin a (f32;
+ * angles in 64 bits; rounded once to bf16).  q, k: F32 or BF16, head h of token t at t *
+ * token_stride + h * head_stride, unit stride inside a head, 16-byte aligned, strides
+ * multiples of 16 bytes below 2^24 elements; positions int64 and inv_freq f32
+ * [head_dim / 2] in device memory; head_dim 64 or 128.  q_out, k_out: bf16, contiguous,
+ * 16-byte aligned, apart from the inputs.  Asynchronous on stream. */
+int mq_rotate_heads(const void *q, int64_t q_token_stride, int64_t q_head_stride, int heads, const void *k,
+                    int64_t k_token_stride, int64_t k_head_stride, int kv_heads, int x_dtype, int head_dim, int64_t tokens,
+                    const int64_t *positions, const float *inv_freq, const float *q_weight, const float *k_weight, float eps,
+                    void *q_out, void *k_out, void *stream);
+/* mq_rotate_heads, and its k (as rounded to bf16) together with v written to the cache's
+ * slots, as mq_kv_cache_append would write them.  k_out may be NULL where the rotated keys
+ * are wanted in the cache only.  Asynchronous on stream. */
+int mq_kv_cache_append_rotated(const mq_kv_cache *cache, const int64_t *slots, const void *q, int64_t q_token_stride,
+                               int64_t q_head_stride, int heads, const void *k, int64_t k_token_stride, int64_t k_head_stride,
+                               const void *v, int64_t v_token_stride, int64_t v_head_stride, int x_dtype, int64_t tokens,
+                               const int64_t *positions, const float *inv_freq, const float *q_weight, const float *k_weight,
+                               float eps, void *q_out, void *k_out, void *stream);
+
 /* Quantize activations once for several Q4_K GEMVs: x [m, k] (F32 or BF16,
  * row stride ldx, 16-byte aligned rows) -> m * k / 256 blocks of
  * MQ_X_Q8K_BLOCK_BYTES at dst (16-byte aligned), by the Q8_K quantization

@@ -86,6 +86,9 @@ SIGNATURES = {
     "mq_cache_attention": (_int, [ctypes.POINTER(KvCacheC), _vp, _i64, _i64, _i64, _int, _vp, _i64, _i64, _vp,
                                   ctypes.c_float, _vp, _i64, _i64, _vp, _sz, _vp]),
     "mq_cache_attention_scratch_size": (_sz, [ctypes.POINTER(KvCacheC), _i64, _int, _i64]),
+    "mq_rotate_heads": (_int, [_vp, _i64, _i64, _int] * 2 + [_int, _int, _i64] + [_vp] * 4 + [ctypes.c_float] + [_vp] * 3),
+    "mq_kv_cache_append_rotated": (_int, [ctypes.POINTER(KvCacheC), _vp, _vp, _i64, _i64, _int] + [_vp, _i64, _i64] * 2
+                                   + [_int, _i64] + [_vp] * 4 + [ctypes.c_float] + [_vp] * 3),
     "mq_gguf_open": (_int, [ctypes.c_char_p, _pp]),
     "mq_gguf_close": (None, [_vp]),
     "mq_gguf_tensor_count": (_i64, [_vp]),

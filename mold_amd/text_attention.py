@@ -1,6 +1,7 @@
 """Causal attention of the GGUF text models (the Qwen text encoders, prompt expansion): whole
-prompts, and new tokens over a paged key/value cache, run by libmoldq (mq_prompt_attention, mq_kv_cache_* and
-mq_cache_attention in include/moldq.h).
+prompts, and new tokens over a paged key/value cache, with what goes before it, the norms and rotation
+of q and k.  Run by libmoldq (mq_prompt_attention,
+mq_rotate_heads, mq_kv_cache_* and mq_cache_attention in include/moldq.h).
 
 candle composes both of matmul, mask and softmax and grows its cache by concatenation
 (quantized_qwen3's attention, used at crates/mold-inference/src/expand.rs:200-203).  Here the
@@ -34,6 +35,12 @@ class _OnStreams:
         self.t, self.device = t, t.device
         self.streams = {torch._C._cuda_getCurrentRawStream(t.device.index)}
 
+    def seen(self, stream):
+        """The current stream of the memory's device, `stream`, has calls that use it."""
+        if stream not in self.streams:
+            self.t.record_stream(torch.cuda.current_stream(self.device))
+            self.streams.add(stream)
+
     def run(self, fn, *args):
         """fn(*args, torch's current stream) with the device current, as it mostly is (making it so
         takes 1.3 us of a 9 us call)."""
@@ -42,12 +49,21 @@ class _OnStreams:
             with torch.cuda.device(self.device):
                 return self.run(fn, *args)
         stream = torch._C._cuda_getCurrentRawStream(current)
-        if stream not in self.streams:
-            self.t.record_stream(torch.cuda.current_stream())
-            self.streams.add(stream)
+        self.seen(stream)
         rc = fn(*args, stream)
         if rc:
             check(rc)
+
+
+def _run_on(device, fn, *args):
+    """fn(*args, torch's current stream of `device`) with the device current."""
+    current = torch._C._cuda_getDevice()
+    if current != device.index:
+        with torch.cuda.device(device):
+            return _run_on(device, fn, *args)
+    rc = fn(*args, torch._C._cuda_getCurrentRawStream(current))
+    if rc:
+        check(rc)
 
 
 def _operand(name, t, shape, device):
@@ -61,6 +77,71 @@ def _operand(name, t, shape, device):
             t = _copied(t)
         st, sh = _strides(t)
     return t, st, sh
+
+
+def _head_rows(name, t, shape, dtype, device):
+    """t as the library reads rows of one type, bf16 or f32, with its token and head stride; copied
+    unless it has unit stride along the head and 16-byte rows."""
+    if t.dtype is not dtype or t.shape != shape or t.device != device:
+        raise ValueError(f"{name} must be {list(shape)} of one type on {device}")
+    st, sh, sd = t.stride()
+    mask = 7 if dtype is _BF16 else 3
+    if sd != 1 or (st | sh) & mask or st >= _MAX_STRIDE or sh >= _MAX_STRIDE or t.data_ptr() & 15:
+        st, sh = _strides(t)
+        if sd != 1 or (st | sh) & mask or st >= _MAX_STRIDE or sh >= _MAX_STRIDE or t.data_ptr() & 15:
+            t = _copied(t)
+            st, sh = _strides(t)
+    return t, st, sh
+
+
+def _vector(name, t, dtype, size, device):
+    """t, contiguous and 16-byte aligned, of `size` elements."""
+    if t.dtype is not dtype or t.shape != (size,) or t.device != device:
+        raise ValueError(f"{name} must be {str(dtype)[6:]} [{size}] on {device}")
+    return t if t.is_contiguous() and not t.data_ptr() & 15 else _copied(t)
+
+
+def _rotation(name, tokens, dim, positions, inv_freq, q_weight, k_weight, device):
+    """The rotation's operands as the library reads them; a weight that is None stays None."""
+    if positions.dtype is not torch.int64 or positions.shape != (tokens,) or positions.device != device:
+        raise ValueError(f"{name}: positions must be int64 [{tokens}] on {device}")
+    if not positions.is_contiguous():
+        positions = positions.contiguous()
+    inv_freq = _vector(f"{name}: inv_freq", inv_freq, torch.float32, dim // 2, device)
+    q_weight, k_weight = (w if w is None else _vector(f"{name}: norm weights", w, torch.float32, dim, device) for w in (q_weight, k_weight))
+    return positions, inv_freq, q_weight, k_weight
+
+
+def _address(t):
+    return None if t is None else t.data_ptr()
+
+
+def _float_rows(name, q, k):
+    if q.dim() != 3 or k.dim() != 3 or q.dtype not in (_BF16, torch.float32) or q.device.type != "cuda" or q.shape[1] == 0 or k.shape[1] == 0:
+        raise ValueError(f"{name}: q and k must be bf16 or f32 [tokens, heads, dim] on a GPU")
+
+
+def rotate_heads(q, k, positions, inv_freq, q_weight=None, k_weight=None, eps: float = 1e-6):
+    """Each head of q [tokens, heads, dim] and k [tokens, kv_heads, dim] (bf16 or f32, both the same;
+    dim 64 or 128) RmsNormed with its weight (f32 [dim]; None: as it is) and its halves rotated by
+    positions[t] * inv_freq[i] (int64 [tokens], f32 [dim / 2]) -> (q, k) in bf16."""
+    if recorded(*(t for t in (q, k, inv_freq, q_weight, k_weight) if t is not None)):
+        raise ValueError("rotate_heads: inference only, nothing may record the call")
+    _float_rows("rotate_heads", q, k)
+    (n, heads, dim), device, dtype = q.shape, q.device, q.dtype
+    if dim not in (64, 128):
+        raise ValueError("rotate_heads: heads of 64 or 128")
+    kv_heads = k.shape[1]
+    q, qt, qh = _head_rows("rotate_heads: q and k", q, (n, heads, dim), dtype, device)
+    k, kt, kh = _head_rows("rotate_heads: q and k", k, (n, kv_heads, dim), dtype, device)
+    positions, inv_freq, q_weight, k_weight = _rotation("rotate_heads", n, dim, positions, inv_freq, q_weight, k_weight, device)
+    q_out = torch.empty((n, heads, dim), dtype=_BF16, device=device)
+    k_out = torch.empty((n, kv_heads, dim), dtype=_BF16, device=device)
+    if n:
+        _run_on(device, _lib.load().mq_rotate_heads, q.data_ptr(), qt, qh, heads, k.data_ptr(), kt, kh, kv_heads, _dtype_code(dtype),
+                dim, n, positions.data_ptr(), inv_freq.data_ptr(), _address(q_weight), _address(k_weight), eps, q_out.data_ptr(),
+                k_out.data_ptr())
+    return q_out, k_out
 
 
 def _copied(t):
@@ -196,7 +277,8 @@ class KvCache:
             raise ValueError(f"KvCache: a GPU's, not {self.device}")
         self.pages, self.kv_heads, self.head_dim, self.page_tokens = int(pages), int(kv_heads), int(head_dim), int(page_tokens)
         self.dtype = GgmlDType(dtype)
-        self._run = _OnStreams(self.data).run
+        self._on = _OnStreams(self.data)
+        self._run = self._on.run
 
     def slots(self, page_table, positions):
         """The slots of `positions` [batch, n] of the sequences whose pages are page_table
@@ -230,16 +312,31 @@ class KvCache:
                       _dtype_code(dtype), n, slots.data_ptr())
 
     def _rows(self, t, shape, dtype):
-        if t.dtype is not dtype or t.shape != shape or t.device != self.device:
-            raise ValueError(f"KvCache.append: k and v must be {list(shape)} of one type on {self.device}")
-        st, sh, sd = t.stride()
-        mask = 7 if dtype is _BF16 else 3
-        if sd != 1 or (st | sh) & mask or st >= _MAX_STRIDE or sh >= _MAX_STRIDE or t.data_ptr() & 15:
-            st, sh = _strides(t)
-            if sd != 1 or (st | sh) & mask or st >= _MAX_STRIDE or sh >= _MAX_STRIDE or t.data_ptr() & 15:
-                t = _copied(t)
-                st, sh = _strides(t)
-        return t, st, sh
+        return _head_rows("KvCache.append: k and v", t, shape, dtype, self.device)
+
+    def append_rotated(self, q, k, v, slots, positions, inv_freq, q_weight=None, k_weight=None, eps: float = 1e-6,
+                       keys: bool = False):
+        """rotate_heads of q and k (k and v [tokens, kv_heads, head_dim], all of one type), with the
+        rotated keys and v appended to `slots` in the same pass -> (q, k) in bf16, k None unless
+        `keys` asks for it (a prompt's attention reads it, a step's reads the cache)."""
+        name = "KvCache.append_rotated"
+        if recorded(*(t for t in (q, k, v, inv_freq, q_weight, k_weight) if t is not None)):
+            raise ValueError(f"{name}: inference only, nothing may record the call")
+        _float_rows(name, q, k)
+        slots = self._slots(name, slots)
+        n, heads, device, dtype = slots.shape[0], q.shape[1], self.device, q.dtype
+        shape = (n, self.kv_heads, self.head_dim)
+        q, qt, qh = _head_rows(f"{name}: q", q, (n, heads, self.head_dim), dtype, device)
+        k, kt, kh = _head_rows(f"{name}: q, k and v", k, shape, dtype, device)
+        v, vt, vh = _head_rows(f"{name}: q, k and v", v, shape, dtype, device)
+        positions, inv_freq, q_weight, k_weight = _rotation(name, n, self.head_dim, positions, inv_freq, q_weight, k_weight, device)
+        q_out = torch.empty((n, heads, self.head_dim), dtype=_BF16, device=device)
+        k_out = torch.empty(shape, dtype=_BF16, device=device) if keys else None
+        if n:
+            self._run(_lib.load().mq_kv_cache_append_rotated, self._ref, slots.data_ptr(), q.data_ptr(), qt, qh, heads, k.data_ptr(), kt,
+                      kh, v.data_ptr(), vt, vh, _dtype_code(dtype), n, positions.data_ptr(), inv_freq.data_ptr(), _address(q_weight),
+                      _address(k_weight), eps, q_out.data_ptr(), _address(k_out))
+        return q_out, k_out
 
     def read(self, slots, dtype=torch.bfloat16):
         """(k, v) [tokens, kv_heads, head_dim] of `slots`, bf16 or f32; zeros for a slot outside the cache."""
