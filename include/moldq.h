@@ -404,6 +404,32 @@ int mq_kv_cache_append_rotated(const mq_kv_cache *cache, const int64_t *slots, c
                                const int64_t *positions, const float *inv_freq, const float *q_weight, const float *k_weight,
                                float eps, void *q_out, void *k_out, void *stream);
 
+/* Pages for `sequences` (up to 65536) prompts of counts[i] tokens (int32, device memory; below
+ * 0 counts as 0) with room for `room` more each, and where their tokens go.  With
+ * beams > 1 a sequence has so many rows of the page table, which share the pages that
+ * its tokens fill and have the others each to itself.  Pages are taken in the order of
+ * `pages` (int32 [page_count], device memory; NULL: 0 .. page_count - 1), sequence by
+ * sequence, shared pages first, then beam by beam:
+ *   table[i * beams + j]   max_pages entries, -1 where it has no page (past its room, no
+ *                          pages left, or a page outside the cache)
+ *   slots, positions       int64 [tokens]: of the packed tokens, sequence by sequence, in
+ *                          beam 0's pages (-1 where the table has none); rows past the
+ *                          last sequence have slot -1, position 0
+ *   lengths                int32 [sequences * beams]
+ *   last                   int64 [sequences]: the row of each one's last token, -1 if none
+ * Asynchronous on stream; one launch, no scratch. */
+#define MQ_MAX_BEAMS 64
+int mq_cache_place(const mq_kv_cache *cache, const int32_t *counts, int64_t sequences, int beams, int64_t room, const int32_t *pages,
+                   int64_t page_count, int32_t *table, int64_t table_stride, int64_t max_pages, int64_t tokens, int64_t *slots,
+                   int64_t *positions, int32_t *lengths, int64_t *last, void *stream);
+/* Where counts[i] more tokens (NULL: one) of sequences that hold held[i] go over the pages
+ * they have: slots and positions as above, -1 past the table or where it names no page of
+ * the cache; lengths[i] = held[i] + counts[i], which may not be `held` itself.  Asynchronous
+ * on stream; one launch, no scratch. */
+int mq_cache_extend(const mq_kv_cache *cache, const int32_t *held, const int32_t *counts, int64_t sequences, const int32_t *table,
+                    int64_t table_stride, int64_t max_pages, int64_t tokens, int64_t *slots, int64_t *positions, int32_t *lengths,
+                    void *stream);
+
 /* Quantize activations once for several Q4_K GEMVs: x [m, k] (F32 or BF16,
  * row stride ldx, 16-byte aligned rows) -> m * k / 256 blocks of
  * MQ_X_Q8K_BLOCK_BYTES at dst (16-byte aligned), by the Q8_K quantization

@@ -24,6 +24,7 @@ class LoraPatchC(ctypes.Structure):
 
 
 MQ_LORA_MAX_PATCHES = 8
+MQ_MAX_BEAMS = 64
 
 
 class PromptPlanC(ctypes.Structure):
@@ -89,6 +90,9 @@ SIGNATURES = {
     "mq_rotate_heads": (_int, [_vp, _i64, _i64, _int] * 2 + [_int, _int, _i64] + [_vp] * 4 + [ctypes.c_float] + [_vp] * 3),
     "mq_kv_cache_append_rotated": (_int, [ctypes.POINTER(KvCacheC), _vp, _vp, _i64, _i64, _int] + [_vp, _i64, _i64] * 2
                                    + [_int, _i64] + [_vp] * 4 + [ctypes.c_float] + [_vp] * 3),
+    "mq_cache_place": (_int, [ctypes.POINTER(KvCacheC), _vp, _i64, _int, _i64, _vp, _i64, _vp, _i64, _i64, _i64]
+                       + [_vp] * 5),
+    "mq_cache_extend": (_int, [ctypes.POINTER(KvCacheC), _vp, _vp, _i64, _vp, _i64, _i64, _i64] + [_vp] * 4),
     "mq_gguf_open": (_int, [ctypes.c_char_p, _pp]),
     "mq_gguf_close": (None, [_vp]),
     "mq_gguf_tensor_count": (_i64, [_vp]),

@@ -1,0 +1,238 @@
+// mq_place.hip — page tables, slots and positions of packed sequences, made on the GPU from
+// their lengths: mq_cache_place for prompts that start, mq_cache_extend for sequences
+// that go on over the pages they have.
+//
+//   shared_i = beams > 1 ? floor(count_i / page) : 0       pages of i that all its beams read
+//   columns_i = min(ceil((count_i + room) / page), width)  pages of each beam
+//   need_i = shared_i + beams (columns_i - shared_i)        first_i = need_0 + .. + need_(i-1)
+//   table[i beams + j, c] = pages[first_i + (c < shared_i ? c : shared_i + j (columns_i - shared_i) + c - shared_i)]
+//   token at offset p of i: position p, slot table[i beams, p / page] page + p % page
+//
+// There is next to nothing to move (16 bytes a token, 4 a table entry) and nothing to
+// compute but two prefix sums over the sequences, so the launch is the cost, and there is
+// one: every workgroup takes the sums over all sequences itself (a window of 1024 at a
+// time, of which a batch has one), rather than wait for another launch or workgroup that
+// did.  A slot comes from the formula and not from the table, which is being written.
+#include "../../include/moldq.h"
+#include "mq_cache_write.h"
+
+namespace mq {
+int set_error(int code, const char *msg);
+}
+
+namespace mq {
+namespace {
+
+constexpr int kPlaceThreads = 256, kPer = 4, kWindow = kPlaceThreads * kPer;
+constexpr int kBlockTokens = 1024;  // tokens of a workgroup
+constexpr int kBlockRows = 4;       // sequences whose table rows a workgroup writes
+constexpr uint32_t kMost = 0x7FFFFFFFu;
+
+struct PlaceArgs {
+  const int32_t *counts, *held;  // counts NULL: one token each; held NULL: prompts that start
+  const int32_t *pages;          // NULL: 0, 1, ..
+  int32_t *table;
+  int64_t n, tokens, width, stride, page_count, cache_pages;
+  int64_t *slots, *positions, *last;
+  int32_t *lengths;
+  uint32_t room, page;
+  int beams;
+};
+
+// Sums stop at kMost, so that counts that mean nothing cannot wrap them.
+__device__ __forceinline__ uint32_t add_capped(uint32_t a, uint32_t b) { return min(a + b, kMost); }
+
+struct Need {
+  uint32_t count, shared, columns, pages;
+  __device__ Need(const PlaceArgs &a, int64_t i) : count(0), shared(0), columns(0), pages(0) {
+    if (i >= a.n) return;
+    count = a.counts ? (uint32_t)max(a.counts[i], 0) : 1;
+    if (a.held) return;
+    const uint32_t most = (uint32_t)min(a.width, (int64_t)kMost);
+    columns = min((count + a.room) / a.page + ((count + a.room) % a.page != 0), most);
+    shared = a.beams > 1 ? min(count / a.page, columns) : 0;
+    const uint64_t need = shared + (uint64_t)a.beams * (columns - shared);
+    pages = (uint32_t)min(need, (uint64_t)kMost);
+  }
+};
+
+// Before each sequence of the window that starts at `from`: the tokens and pages of all
+// sequences before it, given those before the window; after it those of the window's too.
+struct Window {
+  uint32_t tokens[kWindow + 1], pages[kWindow];
+};
+__device__ __forceinline__ void scan_window(const PlaceArgs &a, int64_t from, uint32_t &tokens, uint32_t &pages, Window &w, uint32_t (*sums)[2]) {
+  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+  uint32_t t[kPer], p[kPer], at = 0, ap = 0;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const Need need(a, from + tid * kPer + i);
+    t[i] = at, p[i] = ap;
+    at = add_capped(at, need.count), ap = add_capped(ap, need.pages);
+  }
+  uint32_t st = at, sp = ap;  // over the lanes up to this one
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) {
+    const uint32_t ut = __shfl_up(st, off), up = __shfl_up(sp, off);
+    if (lane >= off) st = add_capped(st, ut), sp = add_capped(sp, up);
+  }
+  __syncthreads();  // the window before has been read
+  if (lane == 63) sums[wave][0] = st, sums[wave][1] = sp;
+  uint32_t bt = __shfl_up(st, 1), bp = __shfl_up(sp, 1);
+  if (lane == 0) bt = bp = 0;
+  __syncthreads();
+  uint32_t all_t = tokens, all_p = pages;
+  bt = add_capped(tokens, bt), bp = add_capped(pages, bp);
+#pragma unroll
+  for (int i = 0; i < kPlaceThreads / 64; ++i) {
+    if (i < wave) bt = add_capped(bt, sums[i][0]), bp = add_capped(bp, sums[i][1]);
+    all_t = add_capped(all_t, sums[i][0]), all_p = add_capped(all_p, sums[i][1]);
+  }
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    w.tokens[tid * kPer + i] = add_capped(bt, t[i]);
+    w.pages[tid * kPer + i] = add_capped(bp, p[i]);
+  }
+  if (tid == 0) w.tokens[kWindow] = all_t;
+  tokens = all_t, pages = all_p;
+  __syncthreads();
+}
+
+// Page `at` of those to take, or -1.
+__device__ __forceinline__ int32_t page_at(const PlaceArgs &a, int64_t at) {
+  if (at >= a.page_count) return -1;
+  const int32_t page = a.pages ? a.pages[at] : (int32_t)at;
+  return page >= 0 && page < a.cache_pages ? page : -1;
+}
+
+// A token's slot and position: offset `in` of sequence i, whose first page is `first`.
+__device__ __forceinline__ void put_token(const PlaceArgs &a, int64_t t, int64_t i, uint32_t in, uint32_t first) {
+  const int64_t position = in + (a.held ? (int64_t)a.held[i] : 0);  // below 2^32
+  const uint32_t column = (uint32_t)position / a.page;
+  int32_t page = -1;
+  if (position >= 0 && column < a.width) {
+    page = a.held ? a.table[i * a.stride + column] : page_at(a, (int64_t)first + column);  // beam 0's, whose own pages follow the shared ones
+    if (page >= a.cache_pages) page = -1;
+  }
+  a.positions[t] = position;
+  a.slots[t] = page < 0 ? -1 : (int64_t)page * a.page + ((uint32_t)position - column * a.page);
+}
+
+// Workgroups 0 .. rows - 1 write kBlockRows sequences' table rows, lengths and last rows
+// each, the others kBlockTokens tokens' slots and positions.
+__global__ __launch_bounds__(kPlaceThreads) void place_kernel(PlaceArgs a, uint32_t rows) {
+  __shared__ Window w;
+  __shared__ uint32_t sums[kPlaceThreads / 64][2];
+  const int tid = threadIdx.x;
+  uint32_t tokens = 0, pages = 0;
+  if (blockIdx.x < rows) {
+    const int64_t first = (int64_t)blockIdx.x * kBlockRows, end = min(a.n, first + kBlockRows);
+    int64_t from = 0;
+    if (!a.held)
+      for (;; from += kWindow) {  // kWindow is a multiple of kBlockRows: the sequences lie in one window
+        scan_window(a, from, tokens, pages, w, sums);
+        if (first < from + kWindow) break;
+      }
+    if (tid < end - first) {
+      const int64_t i = first + tid;
+      const Need need(a, i);
+      const int64_t length = a.held ? min((int64_t)a.held[i] + need.count, (int64_t)kMost) : need.count;
+      for (int j = 0; j < a.beams; ++j) a.lengths[i * a.beams + j] = (int32_t)length;
+      if (!a.held) {
+        const int64_t at = (int64_t)w.tokens[i - from] + need.count - 1;
+        a.last[i] = need.count == 0 || at >= a.tokens ? -1 : at;
+      }
+    }
+    if (a.held || a.width == 0) return;
+    const uint32_t width = (uint32_t)a.width, beams = (uint32_t)a.beams;
+    const uint64_t entries = (uint64_t)(end - first) * beams * width;
+#pragma unroll 4
+    for (uint64_t e = tid; e < entries; e += kPlaceThreads) {
+      const uint32_t row = entries >> 32 ? (uint32_t)(e / width) : (uint32_t)e / width, c = (uint32_t)(e - (uint64_t)row * width);
+      const uint32_t i = row / beams, j = row - i * beams;
+      const Need need(a, first + i);
+      const int64_t own = need.columns - need.shared;
+      a.table[((first + i) * beams + j) * a.stride + c] =
+          c < need.columns ? page_at(a, w.pages[first + i - from] + (c < need.shared ? c : c + j * own)) : -1;
+    }
+    return;
+  }
+  const int64_t t0 = (int64_t)(blockIdx.x - rows) * kBlockTokens, t1 = min(a.tokens, t0 + kBlockTokens);
+  if (!a.counts) {  // a token each
+    for (int64_t t = t0 + tid; t < t1; t += kPlaceThreads) {
+      if (t < a.n) put_token(a, t, t, 0, 0);
+      else a.slots[t] = -1, a.positions[t] = 0;
+    }
+    return;
+  }
+  for (int64_t from = 0; from < a.n; from += kWindow) {
+    const uint32_t before = tokens;
+    scan_window(a, from, tokens, pages, w, sums);
+    const int64_t lo = max(t0, (int64_t)before), hi = min(t1, (int64_t)tokens);
+    for (int64_t t = lo + tid; t < hi; t += kPlaceThreads) {
+      int at = 0;  // the last sequence of the window that starts at or before t and, as t < tokens, holds it
+#pragma unroll
+      for (int step = kWindow / 2; step; step >>= 1)
+        if (w.tokens[at + step] <= t) at += step;
+      put_token(a, t, from + at, (uint32_t)(t - w.tokens[at]), w.pages[at]);
+    }
+    if (tokens >= t1) return;
+  }
+  for (int64_t t = max(t0, (int64_t)tokens) + tid; t < t1; t += kPlaceThreads) a.slots[t] = -1, a.positions[t] = 0;
+}
+
+int invalid(const char *msg) { return set_error(MQ_E_INVALID, msg); }
+bool aligned_to(const void *p, uintptr_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0; }
+
+int launch_place(const PlaceArgs &a, void *stream) {
+  const int64_t rows = (a.n + kBlockRows - 1) / kBlockRows, blocks = rows + (a.tokens + kBlockTokens - 1) / kBlockTokens;
+  if (blocks == 0) return MQ_OK;
+  hipLaunchKernelGGL(place_kernel, dim3((unsigned)blocks), dim3(kPlaceThreads), 0, static_cast<hipStream_t>(stream), a, (uint32_t)rows);
+  const hipError_t e = hipGetLastError();
+  return e == hipSuccess ? MQ_OK : set_error(MQ_E_HIP, hipGetErrorString(e));
+}
+
+const char *place_fault(const mq_kv_cache *c, int64_t n, int64_t tokens, int64_t width, int64_t stride, int64_t rows) {
+  if (const char *fault = cache_fault(c)) return fault;
+  if (n < 0 || n > 65536) return "placing tokens: 0 to 65536 sequences";
+  if (tokens < 0 || tokens >= (int64_t(1) << 31)) return "placing tokens: tokens outside 0 .. 2^31";
+  if (width < 0 || width >= (int64_t(1) << 31) || stride < (rows > 1 ? width : 0) || stride >= (int64_t(1) << 40))
+    return "placing tokens: a table's rows are apart, of 0 to 2^31 pages";
+  return nullptr;
+}
+
+}  // namespace
+}  // namespace mq
+
+extern "C" int mq_cache_place(const mq_kv_cache *c, const int32_t *counts, int64_t sequences, int beams, int64_t room,
+                              const int32_t *pages, int64_t page_count, int32_t *table, int64_t table_stride, int64_t max_pages,
+                              int64_t tokens, int64_t *slots, int64_t *positions, int32_t *lengths, int64_t *last, void *stream) {
+  using namespace mq;
+  if (beams < 1 || beams > MQ_MAX_BEAMS) return invalid("mq_cache_place: 1 to 64 beams");
+  if (const char *fault = place_fault(c, sequences, tokens, max_pages, table_stride, sequences * beams)) return invalid(fault);
+  if (room < 0 || room >= (int64_t(1) << 31)) return invalid("mq_cache_place: room outside 0 .. 2^31");
+  if (page_count < 0 || page_count >= (int64_t(1) << 31)) return invalid("mq_cache_place: 0 to 2^31 pages");
+  if ((sequences && (!counts || !lengths || !last || (!table && max_pages))) || (tokens && (!slots || !positions)))
+    return invalid("mq_cache_place: NULL pointer");
+  if (!aligned_to(counts, 4) || !aligned_to(pages, 4) || !aligned_to(table, 4) || !aligned_to(lengths, 4) || !aligned_to(slots, 8) ||
+      !aligned_to(positions, 8) || !aligned_to(last, 8))
+    return invalid("mq_cache_place: misaligned buffer");
+  return launch_place({counts, nullptr, pages, table, sequences, tokens, max_pages, table_stride, page_count, c->pages, slots,
+                       positions, last, lengths, (uint32_t)room, (uint32_t)c->page_tokens, beams},
+                      stream);
+}
+
+extern "C" int mq_cache_extend(const mq_kv_cache *c, const int32_t *held, const int32_t *counts, int64_t sequences, const int32_t *table,
+                               int64_t table_stride, int64_t max_pages, int64_t tokens, int64_t *slots, int64_t *positions, int32_t *lengths,
+                               void *stream) {
+  using namespace mq;
+  if (const char *fault = place_fault(c, sequences, tokens, max_pages, table_stride, sequences)) return invalid(fault);
+  if ((sequences && (!held || !lengths || (!table && max_pages))) || (tokens && (!slots || !positions)))
+    return invalid("mq_cache_extend: NULL pointer");
+  if (!aligned_to(counts, 4) || !aligned_to(held, 4) || !aligned_to(table, 4) || !aligned_to(lengths, 4) || !aligned_to(slots, 8) ||
+      !aligned_to(positions, 8))
+    return invalid("mq_cache_extend: misaligned buffer");
+  return launch_place({counts, held, nullptr, const_cast<int32_t *>(table), sequences, tokens, max_pages, table_stride, 0, c->pages, slots,
+                       positions, nullptr, lengths, 0, (uint32_t)c->page_tokens, 1},
+                      stream);
+}

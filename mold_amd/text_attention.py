@@ -1,7 +1,7 @@
 """Causal attention of the GGUF text models (the Qwen text encoders, prompt expansion): whole
-prompts, and new tokens over a paged key/value cache, with what goes before it, the norms and rotation
-of q and k.  Run by libmoldq (mq_prompt_attention,
-mq_rotate_heads, mq_kv_cache_* and mq_cache_attention in include/moldq.h).
+prompts, and new tokens over a paged key/value cache, with what goes before it: the norms and rotation
+of q and k, and the pages and slots of a batch's tokens.  Run by libmoldq (mq_prompt_attention,
+mq_rotate_heads, mq_kv_cache_*, mq_cache_place, mq_cache_extend and mq_cache_attention in include/moldq.h).
 
 candle composes both of matmul, mask and softmax and grows its cache by concatenation
 (quantized_qwen3's attention, used at crates/mold-inference/src/expand.rs:200-203).  Here the
@@ -14,6 +14,7 @@ and scratch.  Inference only: calls that autograd or a tracer would record are r
 from __future__ import annotations
 
 import ctypes
+from typing import NamedTuple, Optional
 
 import numpy as np
 import torch
@@ -255,6 +256,17 @@ def prompt_attention(q, k, v, plan: PromptPlan, scale=None, out=None):
     return _given(out, res)
 
 
+class Placed(NamedTuple):
+    """Where a batch's prompts lie: the page table int32 [n * beams, width], their packed tokens'
+    slots and positions int64 [tokens], the lengths int32 [n * beams], and the row of each one's last
+    token, int64 [n] (-1: no token)."""
+    table: torch.Tensor
+    slots: torch.Tensor
+    positions: torch.Tensor
+    lengths: torch.Tensor
+    last: torch.Tensor
+
+
 class KvCache:
     """A paged key/value cache on the device, of `pages` pages of `page_tokens` tokens (a multiple
     of 32), BF16 or in Q8_0 / Q4_0 blocks along the head; head_dim 64 or 128.  Slot s is token
@@ -337,6 +349,64 @@ class KvCache:
                       kh, v.data_ptr(), vt, vh, _dtype_code(dtype), n, positions.data_ptr(), inv_freq.data_ptr(), _address(q_weight),
                       _address(k_weight), eps, q_out.data_ptr(), _address(k_out))
         return q_out, k_out
+
+    def place(self, counts, tokens: int, width: int, room: int = 0, beams: int = 1, pages=None) -> "Placed":
+        """Pages for prompts of `counts` tokens (int32 [n], on the device) with room for `room` more
+        each, and the slots of their packed `tokens` tokens (rows past the last prompt's have
+        none).  A prompt has `beams` rows of the page table, of `width` pages, which share the
+        pages that its tokens fill and have the others each to itself.  `pages` (int32, on the
+        device) are the pages to take, in order; None: the cache's from 0.  Where they end,
+        the table says -1, and attention gives NaN."""
+        if recorded(counts):
+            raise ValueError("KvCache.place: inference only, nothing may record the call")
+        counts = self._whole("KvCache.place: counts", counts)
+        if pages is not None:
+            pages = self._whole("KvCache.place: pages", pages)
+        if tokens < 0 or width < 0 or beams < 1:
+            raise ValueError(f"KvCache.place: {tokens} tokens, {width} pages, {beams} beams")
+        n, device = counts.shape[0], self.device
+        table = torch.empty((n * beams, width), dtype=torch.int32, device=device)
+        slots = torch.empty(tokens, dtype=torch.int64, device=device)
+        positions = torch.empty(tokens, dtype=torch.int64, device=device)
+        lengths = torch.empty(n * beams, dtype=torch.int32, device=device)
+        last = torch.empty(n, dtype=torch.int64, device=device)
+        _run_on(device, _lib.load().mq_cache_place, self._ref, counts.data_ptr(), n, beams, room, _address(pages),
+                self.pages if pages is None else pages.shape[0], table.data_ptr(), width, width, tokens, slots.data_ptr(), positions.data_ptr(),
+                lengths.data_ptr(), last.data_ptr())
+        return Placed(table, slots, positions, lengths, last)
+
+    def extend(self, page_table, held, counts=None, tokens: Optional[int] = None):
+        """(slots, positions, lengths) of more tokens of the sequences that hold `held` (int32 [n])
+        over the pages page_table [n, pages] (int32): one each, or `counts` of them (int32 [n]),
+        packed in `tokens` rows.  A token past the table, or on a page that is not the cache's,
+        has slot -1; rows past the last sequence's have slot -1 and position 0."""
+        if recorded(held):
+            raise ValueError("KvCache.extend: inference only, nothing may record the call")
+        held = self._whole("KvCache.extend: held", held)
+        n, device = held.shape[0], self.device
+        if page_table.dtype is not torch.int32 or page_table.dim() != 2 or page_table.shape[0] != n or page_table.device != device:
+            raise ValueError(f"KvCache.extend: page_table must be int32 [{n}, pages] on {device}")
+        if counts is not None:
+            counts = self._whole("KvCache.extend: counts", counts)
+            if counts.shape[0] != n or tokens is None:
+                raise ValueError(f"KvCache.extend: counts must be int32 [{n}], and tokens says how many rows they fill")
+        tokens = n if tokens is None else tokens
+        if tokens < 0:
+            raise ValueError(f"KvCache.extend: {tokens} tokens")
+        width = page_table.shape[1]
+        if n > 1 and page_table.stride(0) < width or width > 1 and page_table.stride(1) != 1:
+            page_table = page_table.contiguous()
+        slots = torch.empty(tokens, dtype=torch.int64, device=device)
+        positions = torch.empty(tokens, dtype=torch.int64, device=device)
+        lengths = torch.empty(n, dtype=torch.int32, device=device)
+        _run_on(device, _lib.load().mq_cache_extend, self._ref, held.data_ptr(), _address(counts), n, page_table.data_ptr(),
+                page_table.stride(0) if n > 1 else width, width, tokens, slots.data_ptr(), positions.data_ptr(), lengths.data_ptr())
+        return slots, positions, lengths
+
+    def _whole(self, name, t):
+        if t.dtype is not torch.int32 or t.dim() != 1 or t.device != self.device:
+            raise ValueError(f"{name} must be int32, of one dimension, on {self.device}")
+        return t if t.is_contiguous() else t.contiguous()
 
     def read(self, slots, dtype=torch.bfloat16):
         """(k, v) [tokens, kv_heads, head_dim] of `slots`, bf16 or f32; zeros for a slot outside the cache."""
