@@ -378,9 +378,10 @@ int mq_cache_attention(const mq_kv_cache *cache, const void *q, int64_t q_batch_
                        int64_t out_head_stride, void *scratch, size_t scratch_bytes, void *stream);
 size_t mq_cache_attention_scratch_size(const mq_kv_cache *cache, int64_t batch, int heads, int64_t max_pages);
 
-/* --- The same models' steps between their projections and their attention.
- *     candle's quantized_qwen3 (crates/mold-inference/src/expand.rs:200-203) composes them of
- *     separate norms, rotations and concatenations. ---------------------------- */
+/* --- The same models' steps between their projections and their attention, and beam
+ *     search.  candle's quantized_qwen3 (crates/mold-inference/src/expand.rs:200-203) composes
+ *     the first of separate norms, rotations and concatenations; it decodes by
+ *     sampling one sequence, so the rest has no counterpart. ----------------- */
 
 /* Every head of q and k [tokens, heads / kv_heads, head_dim], RmsNormed where its weight
  * (f32 [head_dim]) is not NULL, x / sqrt(mean(x^2) + eps) * weight, and then its halves
@@ -429,6 +430,36 @@ int mq_cache_place(const mq_kv_cache *cache, const int32_t *counts, int64_t sequ
 int mq_cache_extend(const mq_kv_cache *cache, const int32_t *held, const int32_t *counts, int64_t sequences, const int32_t *table,
                     int64_t table_stride, int64_t max_pages, int64_t tokens, int64_t *slots, int64_t *positions, int32_t *lengths,
                     void *stream);
+
+/* The `count` best continuations of each request's beams (both up to MQ_MAX_BEAMS): of all
+ * (beam, token) those with the largest scores[beam] + log softmax(logits of beam)[token],
+ * in order.  Within a beam logits decide, then the lower token; between beams the totals in
+ * 64 bits, then the lower beam.  logits F32 or BF16, row of beam b of request n at n *
+ * request_stride + b * beam_stride (elements, any alignment), unit stride inside; scores
+ * f32 [requests, beams].  A beam whose last[n, b] (int64; NULL: no beam has) is `stop` has
+ * ended: it has one continuation, `stop` at its score, and its logits are not read.  A beam
+ * whose score is not finite, or among whose logits is a NaN or plus infinity, has none, nor
+ * has a logit of minus infinity; places left over have score minus infinity, parent 0,
+ * token -1.  out_scores f32, parents int32 and tokens int64 [requests, count]; scratch: at
+ * least mq_beam_select_scratch_size bytes (device, 16-byte aligned, of this call alone).
+ * Asynchronous on stream. */
+int mq_beam_select(const void *logits, int dtype, int64_t requests, int beams, int64_t vocab, int64_t request_stride,
+                   int64_t beam_stride, const float *scores, const int64_t *last, int64_t stop, int count, float *out_scores,
+                   int32_t *parents, int64_t *tokens, void *scratch, size_t scratch_bytes, void *stream);
+size_t mq_beam_select_scratch_size(int64_t requests, int beams, int64_t vocab, int count);
+/* Beam j of each request goes on from beam parents[n, j] (int32; itself if outside 0 ..
+ * beams - 1), whose tokens so far become its own: in the page table (row n * beams + j,
+ * changed in place) whole pages are shared, the last, partial page is passed on to one child
+ * of each beam and copied, in each of the `count` caches (a model's layers, alike), for the
+ * others, into the pages of beams without a child.  lengths int32 [requests, beams]: the
+ * tokens so far, of which a request's beams have the same number (its first entry is
+ * read).  From the partial page on, no two rows share a page.  scratch: at least
+ * mq_beam_reorder_scratch_size bytes (device, 16-byte aligned, of this call alone).
+ * Asynchronous on stream. */
+int mq_beam_reorder(const mq_kv_cache *caches, int count, int32_t *table, int64_t table_stride, int64_t max_pages,
+                    const int32_t *lengths, const int32_t *parents, int64_t requests, int beams, void *scratch,
+                    size_t scratch_bytes, void *stream);
+size_t mq_beam_reorder_scratch_size(int64_t requests, int beams);
 
 /* Quantize activations once for several Q4_K GEMVs: x [m, k] (F32 or BF16,
  * row stride ldx, 16-byte aligned rows) -> m * k / 256 blocks of
