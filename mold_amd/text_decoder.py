@@ -6,8 +6,10 @@ halves and optional q/k head norms, and a SwiGLU MLP, with tensor names as GGUF 
 them (TextConfig.from_metadata and gguf.Content.var_builder make one of a file).  `prefill`
 takes a batch of prompts packed without padding, `step` one new token of each sequence; both
 write their keys and values into one paged cache (quantized where its type is a block type)
-that `step` attends over.  Norms, rotations and the activation are torch operations in float32;
-projections are QMatMul, attention and cache text_attention.
+that `step` attends over.  Projections are QMatMul; the norms and rotation of q and k, their way
+into the cache, pages and slots, and attention are text_attention; the other norms and the activation are
+torch operations in float32.  `generate` takes the likeliest token each time, `beam_search` keeps
+several hypotheses of each prompt (beams), whose cached prompts share their whole pages.
 
 `step` makes no host synchronization: lengths and page table stay on the device, so it can be
 captured in a graph.  The graph goes on to a later prefill's sequences if there are as many and
@@ -21,6 +23,8 @@ from typing import Dict, Optional, Sequence
 
 import torch
 
+from ._lib import MQ_MAX_BEAMS
+from .beams import BeamStates, select_beams
 from .quantized import GgmlDType, QMatMul, QTensor
 from .text_attention import KvCache, PromptPlan, prompt_attention
 
@@ -54,13 +58,6 @@ def rms_norm(x, weight, eps: float):
     return x * torch.rsqrt(x.square().mean(-1, keepdim=True) + eps) * weight
 
 
-def rotate(x, cos, sin):
-    """Rotary embedding of the halves of each head: x [tokens, heads, dim], cos and sin [tokens, dim / 2]."""
-    a, b = x.float().chunk(2, -1)
-    c, s = cos[:, None], sin[:, None]
-    return torch.cat([a * c - b * s, b * c + a * s], -1)
-
-
 class TextDecoder:
     """weights: {GGUF name: QTensor (as Content.var_builder gives them all) or float32 tensor};
     `output.weight` falls back to the embedding, `attn_{q,k}_norm` and biases are optional.
@@ -80,6 +77,7 @@ class TextDecoder:
         self.table = self.lengths = self._buffers = None
         self._captured, self._retired = False, []     # what graphs of earlier batches hold
         half = config.head_dim // 2
+        self._states = BeamStates(self.caches)
         self._inv_freq = config.rope_theta ** (-torch.arange(half, device=device, dtype=torch.float32) / half)
 
     @staticmethod
@@ -100,27 +98,22 @@ class TextDecoder:
         y = x.float() @ w.t()
         return (y if bias is None else y + bias).to(out_dtype)
 
-    def _heads(self, blk: str, which: str, x, heads: int, cos, sin):
-        y = self._linear(f"{blk}.attn_{which}", x, torch.bfloat16).unflatten(-1, (heads, self.config.head_dim))
-        if which == "v":
-            return y
-        weight = self.weights.get(f"{blk}.attn_{which}_norm.weight")
-        if weight is not None:
-            y = rms_norm(y, weight, self.config.eps)
-        return rotate(y, cos, sin).bfloat16()
+    def _norm(self, name: str):
+        weight = self.weights.get(name)
+        return weight if weight is None else weight.reshape(-1)
 
-    def _forward(self, tokens, positions, slots, attention):
+    def _forward(self, tokens, positions, slots, attention, keys: bool):
         """Hidden states of `tokens` [n] at `positions`, their keys and values written to `slots`;
-        attention(layer, q, k, v) -> [n, heads, dim]."""
+        attention(layer, q, k, v) -> [n, heads, dim], k only if it needs the `keys`."""
         c = self.config
-        angle = positions.float()[:, None] * self._inv_freq
-        cos, sin = angle.cos(), angle.sin()
         x = self.weights["token_embd.weight"][tokens].float()
         for layer in range(c.layers):
             blk = f"blk.{layer}"
             h = rms_norm(x, self.weights[f"{blk}.attn_norm.weight"], c.eps).bfloat16()
-            q, k, v = (self._heads(blk, w, h, n, cos, sin) for w, n in (("q", c.heads), ("k", c.kv_heads), ("v", c.kv_heads)))
-            self.caches[layer].append(k, v, slots)
+            q, k, v = (self._linear(f"{blk}.attn_{w}", h, torch.bfloat16).unflatten(-1, (n, c.head_dim))
+                       for w, n in (("q", c.heads), ("k", c.kv_heads), ("v", c.kv_heads)))
+            q, k = self.caches[layer].append_rotated(q, k, v, slots, positions, self._inv_freq, self._norm(f"{blk}.attn_q_norm.weight"),
+                                                     self._norm(f"{blk}.attn_k_norm.weight"), c.eps, keys)
             a = attention(layer, q, k, v)
             x = x + self._linear(f"{blk}.attn_output", a.flatten(1))
             h = rms_norm(x, self.weights[f"{blk}.ffn_norm.weight"], c.eps).bfloat16()
@@ -135,38 +128,35 @@ class TextDecoder:
         return x @ self.weights["token_embd.weight"].t()
 
     @torch.no_grad()
-    def prefill(self, prompts: Sequence[Sequence[int]], room: int = 0):
+    def prefill(self, prompts: Sequence[Sequence[int]], room: int = 0, beams: int = 1):
         """Start sequences from `prompts` (at least a token each), with pages for `room` more tokens
-        of each; returns the logits after each prompt's last token [n, vocab].  The sequences before
+        of each; returns the logits after each prompt's last token [n, vocab].  With beams, each
+        prompt is so many sequences from here on, one after another.  The sequences before
         them end, also where it fails in the middle."""
         lengths = [len(p) for p in prompts]
         if not lengths or min(lengths) == 0:
             raise ValueError("TextDecoder.prefill: at least one prompt, of at least one token each")
-        if room < 0:
-            raise ValueError(f"TextDecoder.prefill: room for {room} tokens")
-        per = -(-(max(lengths) + room) // self.page_tokens)
-        need = [-(-(n + room) // self.page_tokens) for n in lengths]
-        if sum(need) > self.pages:
-            raise ValueError(f"TextDecoder.prefill: {sum(need)} pages needed, the cache has {self.pages}")
-        table, at = torch.full((len(lengths), per), -1, dtype=torch.int32), 0
-        for b, n in enumerate(need):
-            table[b, :n] = torch.arange(at, at + n)
-            at += n
-        pos = torch.cat([torch.arange(n) for n in lengths])
-        seq = torch.repeat_interleave(torch.arange(len(lengths)), torch.tensor(lengths))
-        slots = table.long()[seq, pos // self.page_tokens] * self.page_tokens + pos % self.page_tokens
-        slots, pos = slots.to(self.device), pos.to(self.device)
+        if room < 0 or not 1 <= beams <= MQ_MAX_BEAMS:
+            raise ValueError(f"TextDecoder.prefill: room for {room} tokens, {beams} beams")
+        page = self.page_tokens
+        per = -(-(max(lengths) + room) // page)
+        shared = [n // page if beams > 1 else 0 for n in lengths]
+        need = sum(s + beams * (-(-(n + room) // page) - s) for s, n in zip(shared, lengths))
+        if need > self.pages:
+            raise ValueError(f"TextDecoder.prefill: {need} pages needed, the cache has {self.pages}")
         plan = PromptPlan(lengths, self.config.heads, self.config.kv_heads, self.config.head_dim, self.device)
         tokens = torch.tensor([t for p in prompts for t in p])
         vocab = self.weights["token_embd.weight"].shape[0]
         if tokens.min() < 0 or tokens.max() >= vocab:
             raise ValueError(f"TextDecoder.prefill: a token outside 0 .. {vocab - 1}")
+        at = self.caches[0].place(torch.tensor(lengths, dtype=torch.int32).to(self.device), sum(lengths), per, room, beams)
         tokens = tokens.to(self.device)
-        last = torch.cumsum(torch.tensor(lengths), 0) - 1
         self._end()
-        x = self._forward(tokens, pos, slots, lambda layer, q, k, v: prompt_attention(q, k, v, plan))
-        logits = self._logits(x[last.to(self.device)])
-        self._begin(table, torch.tensor(lengths, dtype=torch.int32))
+        x = self._forward(tokens, at.positions, at.slots, lambda layer, q, k, v: prompt_attention(q, k, v, plan), keys=True)
+        logits = self._logits(x[at.last])
+        if beams > 1:                # the partial page of each prompt, of which the first beam has the tokens
+            self._states.reorder(at.table, at.lengths, torch.zeros((len(lengths), beams), dtype=torch.int32, device=self.device))
+        self._begin(at.table, at.lengths)
         return logits
 
     def _end(self):
@@ -185,7 +175,7 @@ class TextDecoder:
         if self._captured:
             self._retired.append(self._buffers)
             self._captured = False
-        self.table, self.lengths = table.to(self.device), lengths.to(self.device)
+        self.table, self.lengths = table, lengths
 
     @torch.no_grad()
     def step(self, tokens):
@@ -196,11 +186,9 @@ class TextDecoder:
         if tokens.shape != self.lengths.shape or tokens.dtype not in (torch.int64, torch.int32) or tokens.device != self.lengths.device:
             raise ValueError(f"TextDecoder.step: tokens must be int64 {list(self.lengths.shape)} on {self.lengths.device}")
         self._captured |= torch.cuda.is_current_stream_capturing()
-        pos, lengths = self.lengths.long(), self.lengths + 1
-        held = torch.full_like(pos, self.table.shape[1] * self.page_tokens)
         # past the table: written nowhere, and longer than its pages, which attention answers with NaN
-        slots = torch.where(pos < held, self.caches[0].slots(self.table, torch.minimum(pos, held - 1)[:, None])[:, 0], -1)
-        x = self._forward(tokens, pos, slots, lambda layer, q, k, v: self.caches[layer].attend(q, self.table, lengths))
+        slots, pos, lengths = self.caches[0].extend(self.table, self.lengths)
+        x = self._forward(tokens, pos, slots, lambda layer, q, k, v: self.caches[layer].attend(q, self.table, lengths), keys=False)
         logits = self._logits(x)
         self.lengths.copy_(lengths)      # last: a step that fails has not moved the sequences on
         return logits
@@ -217,3 +205,30 @@ class TextDecoder:
             token = nxt if stop is None else torch.where(token == stop, token, nxt)
             out.append(token)
         return torch.stack(out, 1)[:, :count]
+
+    @torch.no_grad()
+    def beam_search(self, prompts: Sequence[Sequence[int]], beams: int, count: int, stop: Optional[int] = None):
+        """The continuations of `count` tokens of each prompt that a search with `beams` hypotheses
+        finds the most probable, best first -> (tokens [n, beams, count], their log probabilities
+        [n, beams]).  A continuation that has given `stop` repeats it and keeps its probability;
+        where there are fewer continuations than beams, the rest have tokens -1, probability 0."""
+        if count < 0:
+            raise ValueError(f"TextDecoder.beam_search: {count} tokens")
+        logits, chosen = self.prefill(prompts, room=count, beams=beams)[:, None], []
+        n, last = len(prompts), None
+        scores = torch.zeros((n, 1), device=self.device)
+        for at in range(count):
+            if at:
+                logits = self.step(last.reshape(-1)).view(n, beams, -1)
+            ended = {} if stop is None or last is None else {"last": last, "stop": stop}
+            scores, parents, last = select_beams(logits, scores, beams, **ended)
+            if at:
+                self._states.reorder(self.table, self.lengths, parents)
+            chosen.append((parents, last))
+        if not chosen:
+            return torch.empty((n, beams, 0), dtype=torch.int64, device=self.device), scores.expand(n, beams).contiguous()
+        row, out = torch.arange(beams, device=self.device).expand(n, beams), []
+        for parents, tokens in reversed(chosen):
+            out.append(torch.gather(tokens, 1, row))
+            row = torch.gather(parents.long(), 1, row)
+        return torch.stack(out[::-1], 2), scores
