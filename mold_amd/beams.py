@@ -44,11 +44,17 @@ def select_beams(logits, scores, count=None, last=None, stop=None):
         raise ValueError("select_beams: last and stop go together")
     if stop is not None and not 0 <= stop < vocab:
         raise ValueError(f"select_beams: stop {stop} is not one of {vocab} tokens")
-    for name, t, dtype in (("scores", scores, torch.float32), ("last", last, torch.int64)):
-        if t is not None and (t.dtype is not dtype or t.shape != (n, beams) or t.device != device):
-            raise ValueError(f"select_beams: {name} must be {str(dtype)[6:]} [{n}, {beams}] on {device}")
-    scores = scores if scores.is_contiguous() else scores.contiguous()
-    last = last if last is None or last.is_contiguous() else last.contiguous()
+    if scores.dtype is not torch.float32 or scores.shape != (n, beams) or scores.device != device:
+        raise ValueError(f"select_beams: scores must be float32 [{n}, {beams}] on {device}")
+    if not scores.is_contiguous():
+        scores = scores.contiguous()
+    last_at = None
+    if last is not None:
+        if last.dtype is not torch.int64 or last.shape != (n, beams) or last.device != device:
+            raise ValueError(f"select_beams: last must be int64 [{n}, {beams}] on {device}")
+        if not last.is_contiguous():
+            last = last.contiguous()
+        last_at = last.data_ptr()
     sn, sb, sv = logits.stride()
     if sv != 1 and vocab > 1 or sn >= _MAX_STRIDE or sb >= _MAX_STRIDE:
         logits = logits.contiguous()
@@ -61,7 +67,7 @@ def select_beams(logits, scores, count=None, last=None, stop=None):
         nbytes = lib.mq_beam_select_scratch_size(n, beams, vocab, count)
         scratch = torch.empty(nbytes, dtype=torch.uint8, device=device)     # freed to this stream
         _run_on(device, lib.mq_beam_select, logits.data_ptr(), _dtype_code(logits.dtype), n, beams, vocab, sn, sb, scores.data_ptr(),
-                None if last is None else last.data_ptr(), 0 if stop is None else stop, count, totals.data_ptr(), parents.data_ptr(),
+                last_at, 0 if stop is None else stop, count, totals.data_ptr(), parents.data_ptr(),
                 tokens.data_ptr(), scratch.data_ptr(), nbytes)
     return totals, parents, tokens
 
@@ -71,8 +77,8 @@ class BeamStates:
 
     def __init__(self, caches: Sequence[KvCache]):
         self.caches = list(caches)
-        if not self.caches:
-            raise ValueError("BeamStates: no caches")
+        if not 1 <= len(self.caches) <= 256:
+            raise ValueError(f"BeamStates: 1 to 256 caches, got {len(self.caches)}")
         first = self.caches[0]
         like = lambda c: (c.device, c.dtype, c.pages, c.kv_heads, c.head_dim, c.page_tokens)
         if any(like(c) != like(first) for c in self.caches):

@@ -19,7 +19,7 @@
 // of each parent (to the parent's own row if it is one, else the first); every other child
 // takes the page of a row without children, as many as there are, and has the tokens so far
 // copied into it, in every layer's cache.  plan_kernel does the tables, copy_kernel moves the
-// bytes: those of the used tiles (32 tokens) and no others, which bound it.
+// bytes, which bound it: those of the tiles (32 tokens) that the tokens reach, and no others.
 #include "../../include/moldq.h"
 #include "mq_cache_write.h"
 
@@ -31,7 +31,7 @@ namespace mq {
 namespace {
 
 constexpr int kScanThreads = 256, kScanWaves = kScanThreads / 64;
-constexpr int kMergeThreads = 256, kMergeWaves = kMergeThreads / 64;
+constexpr int kMergeThreads = 512, kMergeWaves = kMergeThreads / 64;
 
 // A logit and its token as one key: larger logits first, of equal ones the lower token.  0 is
 // none.  Adding 0 makes the two zeros one.
@@ -46,57 +46,94 @@ __device__ __forceinline__ float logit_of(uint64_t key) {
 }
 __device__ __forceinline__ uint32_t token_of(uint64_t key) { return 0xFFFFFFFFu - (uint32_t)key; }
 
-__device__ __forceinline__ uint64_t xor_lane(uint64_t v, int with) {
-  return ((uint64_t)__shfl_xor((uint32_t)(v >> 32), with) << 32) | __shfl_xor((uint32_t)v, with);
+// Lane i ^ kWith's value, by vector instructions alone (an LDS permutation takes ten times as long).
+template <int kWith>
+__device__ __forceinline__ uint32_t lane_xor(uint32_t x) {
+  if constexpr (kWith == 1) return dpp<0xB1>(x);                 // quad_perm 1 0 3 2
+  else if constexpr (kWith == 2) return dpp<0x4E>(x);            // quad_perm 2 3 0 1
+  else if constexpr (kWith == 4) return dpp<0x1B>(dpp<0x141>(x));  // row_half_mirror, quad_perm 3 2 1 0
+  else if constexpr (kWith == 8) return dpp<0x128>(x);           // row_ror 8
+  else if constexpr (kWith == 16) {
+    const auto r = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+    return threadIdx.x & 16 ? r[0] : r[1];
+  } else {
+    const auto r = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+    return threadIdx.x & 32 ? r[0] : r[1];
+  }
+}
+template <int kWith>
+__device__ __forceinline__ uint64_t lane_xor(uint64_t v) {
+  return ((uint64_t)lane_xor<kWith>((uint32_t)(v >> 32)) << 32) | lane_xor<kWith>((uint32_t)v);
+}
+template <int kWith>
+__device__ __forceinline__ float lane_xor(float v) {
+  return __uint_as_float(lane_xor<kWith>(__float_as_uint(v)));
+}
+template <int kWith>
+__device__ __forceinline__ double lane_xor(double v) {
+  return __longlong_as_double((int64_t)lane_xor<kWith>((uint64_t)__double_as_longlong(v)));
+}
+// The lane before's; lane 0's own is undefined.
+__device__ __forceinline__ uint64_t lane_before(uint64_t v) {
+  return ((uint64_t)dpp<0x138>((uint32_t)(v >> 32)) << 32) | dpp<0x138>((uint32_t)v);  // wave_shr 1
 }
 __device__ __forceinline__ uint64_t lane_of(uint64_t v, int lane) {
   return ((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), lane) << 32) | (uint32_t)__builtin_amdgcn_readlane((int)v, lane);
 }
-// Lane i takes the larger (where `high`) or the smaller of its own and lane i ^ with's.
-template <typename K>
-__device__ __forceinline__ K exchange(K v, int with, bool high) {
-  K other;
-  if constexpr (sizeof(K) == 8) other = xor_lane(v, with);
-  else other = __shfl_xor(v, with);
+// Lane i takes the larger (where `high`) or the smaller of its own and lane i ^ kWith's.
+template <int kWith, typename K>
+__device__ __forceinline__ K exchange(K v, bool high) {
+  const K other = lane_xor<kWith>(v);
   return high == (v > other) ? v : other;
+}
+// A bitonic sequence sorted over runs of 2 kWith lanes, the largest first where `down`.
+template <int kWith, typename K>
+__device__ __forceinline__ K merged(K v, bool down) {
+  v = exchange<kWith>(v, down == !(threadIdx.x & kWith));
+  if constexpr (kWith > 1) return merged<kWith / 2>(v, down);
+  return v;
 }
 // Sorted over the wave, the largest in lane 0.
 template <typename K>
 __device__ __forceinline__ K sorted(K v) {
-  const int lane = threadIdx.x & 63;
-#pragma unroll
-  for (int size = 2; size <= 64; size <<= 1)
-#pragma unroll
-    for (int with = size >> 1; with; with >>= 1) v = exchange(v, with, ((lane & size) == 0) == ((lane & with) == 0));
-  return v;
+  v = merged<1>(v, !(threadIdx.x & 2));
+  v = merged<2>(v, !(threadIdx.x & 4));
+  v = merged<4>(v, !(threadIdx.x & 8));
+  v = merged<8>(v, !(threadIdx.x & 16));
+  v = merged<16>(v, !(threadIdx.x & 32));
+  return merged<32>(v, true);
 }
 
 // The largest keys that a wave has seen, one a lane, the largest in lane 0.
 struct Largest {
-  uint64_t key, least;  // `least`: the count-th, below which nothing enters
+  uint64_t key, least;  // `least`: nothing of it and below enters
   int count;
+  bool any;
 
-  __device__ explicit Largest(int n) : key(0), least(0), count(n) {}
+  __device__ explicit Largest(int n) : key(0), least(0), count(n), any(false) {}
   // A key of each lane, or 0.  All lanes join.
   __device__ void offer(uint64_t k) {
     uint64_t in = __ballot(k > least);
     if (!in) return;
-    if (__popcll(in) <= 6) {
+    if (any && __popcll(in) <= 4) {
       const int lane = threadIdx.x & 63;
       do {
         const int from = __builtin_ctzll(in);
         in &= in - 1;
         const uint64_t one = lane_of(k, from);
         const int at = __popcll(__ballot(key > one));
-        const uint64_t before = ((uint64_t)__shfl_up((uint32_t)(key >> 32), 1) << 32) | __shfl_up((uint32_t)key, 1);
+        const uint64_t before = lane_before(key);
         key = lane < at ? key : lane == at ? one : before;
       } while (in);
     } else {
       k = sorted(k > least ? k : 0);
-      const uint64_t turned = xor_lane(k, 63);  // ascending: with the list one bitonic sequence
-      key = key > turned ? key : turned;
-#pragma unroll
-      for (int with = 32; with; with >>= 1) key = exchange(key, with, (threadIdx.x & with) == 0);
+      if (any) {
+        // ascending, so that with the list it makes one bitonic sequence
+        k = lane_xor<32>(lane_xor<16>(((uint64_t)dpp<0x140>((uint32_t)(k >> 32)) << 32) | dpp<0x140>((uint32_t)k)));  // row_mirror
+        k = merged<32>(key > k ? key : k, true);
+      }
+      key = k;
+      any = true;
     }
     const uint64_t last = lane_of(key, count - 1);
     if (last > least) least = last;
@@ -126,14 +163,16 @@ struct Vec<__bf16> {
   }
 };
 
+template <int kWith = 32>
 __device__ __forceinline__ float wave_max(float v) {
-#pragma unroll
-  for (int off = 32; off; off >>= 1) v = fmaxf(v, __shfl_xor(v, off));
+  v = fmaxf(v, lane_xor<kWith>(v));
+  if constexpr (kWith > 1) return wave_max<kWith / 2>(v);
   return v;
 }
+template <int kWith = 32>
 __device__ __forceinline__ double wave_sum(double v) {
-#pragma unroll
-  for (int off = 32; off; off >>= 1) v += __shfl_xor(v, off);
+  v += lane_xor<kWith>(v);
+  if constexpr (kWith > 1) return wave_sum<kWith / 2>(v);
   return v;
 }
 
@@ -160,15 +199,44 @@ struct SelectArgs {
 
 __device__ __forceinline__ bool ended(const SelectArgs &a, int64_t row) { return a.last && a.last[row] == a.stop; }
 
-// Reads part `part` of `parts` of a row by one wave.
-template <typename X>
+constexpr int kBuffer = 128;
+
+// What a wave keeps of the logits that it has seen.  Those that may be among the largest are
+// put down in `buffer` and sorted 64 at a time, most often only once, with the other waves'
+// at the end: putting each in its place at once is a chain of some 15 instructions that
+// depend on each other (80 rows of 151111, the ten largest: 30 us, 22 now).
 struct Scan {
   Largest top;
+  uint64_t *buffer;
+  int held;            // in the buffer
   double sum;
-  float ref, enter;  // `enter`: what a logit has to reach to enter the list or to move the reference
+  float ref, least;  // `least`: what a logit has to reach to be put down
+  float enter;       // ..: for that or to move the reference
+  float lane_most;
 
-  __device__ explicit Scan(int count) : top(count), sum(0.), ref(-__FLT_MAX__), enter(-__FLT_MAX__) {}
+  __device__ Scan(int count, uint64_t *b)
+      : top(count), buffer(b), held(0), sum(0.), ref(-__FLT_MAX__), least(-__FLT_MAX__), enter(-__FLT_MAX__), lane_most(-__FLT_MAX__) {}
 
+  __device__ static void fence() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+  }
+  // A logit of each lane.
+  __device__ void put(float x, uint32_t token) {
+    const uint64_t k = x >= -__FLT_MAX__ ? key_of_logit(x, token) : 0, in = __ballot(k > top.least);
+    if (!in) return;
+    if (k > top.least) buffer[held + __builtin_amdgcn_mbcnt_hi((uint32_t)(in >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)in, 0))] = k;
+    held += (int)__popcll(in);
+    if (held < 64) return;
+    const int lane = threadIdx.x & 63;
+    fence();
+    const uint64_t first = buffer[lane], then = buffer[64 + lane];
+    fence();
+    held -= 64;
+    if (lane < held) buffer[lane] = then;
+    fence();
+    top.offer(first);
+  }
   // The reference follows the largest of the lanes' logits; the sums so far with it.
   __device__ void follow(float most) {
     const float to = wave_max(most);
@@ -177,11 +245,37 @@ struct Scan {
     ref = to;
   }
   __device__ void bounds() {
-    const float least = top.least ? logit_of(top.least) : -__FLT_MAX__;
+    least = top.least ? logit_of(top.least + 1) : -__FLT_MAX__;  // the least logit of a larger key
     enter = fminf(least, ref + 1.f);
   }
+  // The bar below which a logit need not enter: the count-th largest of the lanes' maxima so
+  // far, which as many logits reach.  In the order of ordered().
+  __device__ uint32_t bar() const {
+    return __builtin_amdgcn_readlane((int)sorted(ordered(lane_most >= -__FLT_MAX__ ? lane_most : -__FLT_MAX__)), top.count - 1);
+  }
+  __device__ void raise(uint32_t to) {
+    const uint64_t below = to > ordered(-__FLT_MAX__) ? ((uint64_t)to << 32) - 1 : 0;  // the key that all of it pass
+    if (below > top.least) top.least = below;
+    bounds();
+  }
   template <int N>
-  __device__ void add(const float *x) {
+  __device__ static float most_of(const float *x) {
+    float m = x[0];
+#pragma unroll
+    for (int i = 1; i < N; ++i) m = fmaxf(m, x[i]);
+    return m;
+  }
+  // N logits of each lane, the largest of them `most`, tokens token .. token + N - 1; minus
+  // infinity for none.
+  template <int N>
+  __device__ void take(const float *x, float most, uint32_t token) {
+    if (__any(most >= enter)) {
+      follow(most);
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        if (__any(x[i] >= least)) put(x[i], token + i);
+      bounds();
+    }
     float s[N];
 #pragma unroll
     for (int i = 0; i < N; ++i) s[i] = __builtin_amdgcn_exp2f((x[i] - ref) * kLog2e);
@@ -191,98 +285,100 @@ struct Scan {
       for (int i = 0; i < w; ++i) s[i] += s[i + w];
     sum += (double)s[0];
   }
-  template <int N>
-  __device__ static float most_of(const float *x) {
-    float m = x[0];
-#pragma unroll
-    for (int i = 1; i < N; ++i) m = fmaxf(m, x[i]);
-    return m;
-  }
-  // N logits of each lane, tokens token .. token + N - 1; minus infinity for none.
-  template <int N>
-  __device__ void take(const float *x, uint32_t token) {
-    const float most = most_of<N>(x);
-    if (__any(most >= enter)) {
-      follow(most);
-#pragma unroll
-      for (int i = 0; i < N; ++i) top.offer(x[i] >= -__FLT_MAX__ ? key_of_logit(x[i], token + i) : 0);
-      bounds();
-    }
-    add<N>(x);
-  }
-
-  __device__ void row(const X *p, int64_t vocab, int64_t part, int64_t parts) {
-    constexpr int N = Vec<X>::kN;
-    typedef typename Vec<X>::raw raw;
-    const int lane = threadIdx.x & 63;
-    const int64_t vectors = vocab / N, rest = vocab - vectors * N;
-    const raw *const body = reinterpret_cast<const raw *>(p);
-    const int64_t from = vectors * part / parts, to = vectors * (part + 1) / parts;
-    constexpr int U = 4;
-    for (int64_t v = from; v < to; v += 64 * U) {
-      float x[U][N];
-      raw r[U];
-#pragma unroll
-      for (int u = 0; u < U; ++u) r[u] = body[min(v + 64 * u + lane, to - 1)];
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        Vec<X>::get(r[u], x[u]);
-        if (v + 64 * u + lane >= to) {
-#pragma unroll
-          for (int i = 0; i < N; ++i) x[u][i] = -__builtin_inff();
-        }
-      }
-      if (v == from) {  // the count-th largest of the lanes' maxima: as many logits reach it, so what lies below need not enter
-        float most = most_of<N>(x[0]);
-#pragma unroll
-        for (int u = 1; u < U; ++u) most = fmaxf(most, most_of<N>(x[u]));
-        follow(most);
-        most = most >= -__FLT_MAX__ ? most : -__FLT_MAX__;
-        const uint32_t least = __builtin_amdgcn_readlane((int)sorted(ordered(most)), top.count - 1);
-        // a key that every logit of that value passes, and none below it
-        top.least = least > ordered(-__FLT_MAX__) ? ((uint64_t)least << 32) - 1 : 0;
-        enter = fminf(logit_of((uint64_t)least << 32), ref + 1.f);
-      }
-#pragma unroll
-      for (int u = 0; u < U; ++u)
-        if (v + 64 * u < to) take<N>(x[u], (uint32_t)((v + 64 * u + lane) * N));
-    }
-    if (part == parts - 1 && rest) {
-      const int64_t at = vectors * N + lane;
-      const float x = lane < rest ? (float)p[at] : -__builtin_inff();
-      take<1>(&x, (uint32_t)at);
-    }
-  }
 };
 
 template <typename X>
 __global__ __launch_bounds__(kScanThreads) void scan_kernel(SelectArgs a) {
+  constexpr int N = Vec<X>::kN, U = 4;
+  typedef typename Vec<X>::raw raw;
   __shared__ Run runs[kScanWaves];
-  __shared__ uint64_t lists[kScanWaves][64];
-  const int64_t row = blockIdx.x / (uint32_t)a.splits, split = blockIdx.x - row * a.splits;
-  if (ended(a, row) || !(fabsf(a.scores[row]) <= __FLT_MAX__)) return;  // has no logits to look at
-  const int64_t n = row / a.beams;
+  __shared__ uint64_t buffers[kScanWaves][kBuffer];
+  __shared__ uint32_t bars[kScanWaves], helds[kScanWaves];
+  const int64_t row = blockIdx.x / (uint32_t)a.splits, split = blockIdx.x - row * a.splits, n = row / a.beams;
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  Scan<X> scan(a.count);
-  scan.row(static_cast<const X *>(a.logits) + n * a.request + (row - n * a.beams) * a.beam, a.vocab, split * kScanWaves + wave,
-           (int64_t)a.splits * kScanWaves);
+  const X *const p = static_cast<const X *>(a.logits) + n * a.request + (row - n * a.beams) * a.beam;
+  const raw *const body = reinterpret_cast<const raw *>(p);
+  const int64_t vectors = a.vocab / N, rest = a.vocab - vectors * N, part = split * kScanWaves + wave, parts = (int64_t)a.splits * kScanWaves;
+  const int64_t to = vectors * (part + 1) / parts;
+  int64_t v = vectors * part / parts;
+  raw next[U];
+  float x[U][N], most[U];
+  auto fetch = [&](int64_t at) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) next[u] = body[min(at + 64 * u + lane, to - 1)];
+  };
+  Scan scan(a.count, buffers[wave]);
+  auto unpack = [&] {  // and what comes after it on its way
+#pragma unroll
+    for (int u = 0; u < U; ++u) Vec<X>::get(next[u], x[u]);
+    if (v + 64 * U < to) {
+      fetch(v + 64 * U);
+    } else if (v + 64 * U > to) {
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int i = 0; i < N; ++i) x[u][i] = v + 64 * u + lane < to ? x[u][i] : -__builtin_inff();
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      most[u] = Scan::most_of<N>(x[u]);
+      scan.lane_most = fmaxf(scan.lane_most, most[u]);
+    }
+  };
+  if (v < to) fetch(v);
+  if (ended(a, row) || !(fabsf(a.scores[row]) <= __FLT_MAX__)) return;  // its logits do not matter
+
+  // What is below one wave's bar need not enter any of the workgroup's lists.
+  uint32_t bar = 0;
+  if (v < to) {
+    unpack();
+    scan.follow(scan.lane_most);
+    bar = scan.bar();
+  }
+  if (lane == 0) bars[wave] = bar;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kScanWaves; ++i) bar = max(bar, bars[i]);
+  scan.raise(bar);
+  for (uint32_t turn = 1; v < to; ++turn) {
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (v + 64 * u < to) scan.take<N>(x[u], most[u], (uint32_t)((v + 64 * u + lane) * N));
+    v += 64 * U;
+    if (v >= to) break;
+    unpack();
+    if ((turn & (turn - 1)) == 0) scan.raise(scan.bar());  // at each doubling: what enters between two is about the same
+  }
+  if (part == parts - 1 && rest) {
+    const int64_t at = vectors * N + lane;
+    const float y = lane < rest ? (float)p[at] : -__builtin_inff();
+    scan.take<1>(&y, y, (uint32_t)at);
+  }
+
   const double sum = wave_sum(scan.sum);
-  if (lane == 0) runs[wave] = {sum, scan.ref};
-  lists[wave][lane] = scan.top.key;
+  if (scan.top.any && lane < a.count) buffers[wave][scan.held + lane] = scan.top.key;
+  if (lane == 0) runs[wave] = {sum, scan.ref}, helds[wave] = scan.held + (scan.top.any ? a.count : 0);
   __syncthreads();
   if (wave) return;
-  Largest top = scan.top;
-  top.least = lane_of(top.key, a.count - 1);
-  for (int first = a.count; first < kScanWaves * a.count; first += 64) {
+  Largest top(a.count);
+  int total = 0, start[kScanWaves];
+#pragma unroll
+  for (int i = 0; i < kScanWaves; ++i) start[i] = total, total += helds[i];
+  for (int first = 0; first < total; first += 64) {
     const int at = first + lane;
-    top.offer(at < kScanWaves * a.count ? lists[at / a.count][at % a.count] : 0);
+    int of = 0, from = 0;
+#pragma unroll
+    for (int i = 1; i < kScanWaves; ++i)
+      if (at >= start[i]) of = i, from = start[i];
+    top.offer(at < total ? buffers[of][at - from] : 0);
   }
   Run all = runs[0];
 #pragma unroll
   for (int i = 1; i < kScanWaves; ++i) all.ref = fmaxf(all.ref, runs[i].ref);
+  const double part_sum = lane < kScanWaves ? runs[lane].sum * exp((double)runs[lane].ref - (double)all.ref) : 0.;
   all.sum = 0.;
 #pragma unroll
-  for (int i = 0; i < kScanWaves; ++i) all.sum += runs[i].sum * exp((double)runs[i].ref - (double)all.ref);
+  for (int i = 0; i < kScanWaves; ++i) all.sum += __longlong_as_double((int64_t)lane_of((uint64_t)__double_as_longlong(part_sum), i));
   if (lane == 0) a.runs[row * a.splits + split] = all;
   if (lane < a.count) a.keys[(row * a.splits + split) * a.count + lane] = top.key;
 }
@@ -304,56 +400,68 @@ __device__ __forceinline__ double total_of(uint64_t u) {
 // those over it: of its own beam the ones before it, of a lower beam those of no smaller
 // total, of a higher one those of a larger.
 __global__ __launch_bounds__(kMergeThreads) void merge_kernel(SelectArgs a) {
-  extern __shared__ Candidate found[];  // [beams, count], each beam's sorted
+  extern __shared__ Candidate found[];  // [beams, count], each beam's sorted; then their ranks
+  int *const ranks = reinterpret_cast<int *>(found + a.beams * a.count);
+  __shared__ int have;
   const int64_t n = blockIdx.x;
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  if (threadIdx.x == 0) have = 0;
+  __syncthreads();
   for (int b = wave; b < a.beams; b += kMergeWaves) {
     const int64_t row = n * a.beams + b;
     const float score = a.scores[row];
+    const uint64_t *const keys = a.keys + row * a.splits * a.count;
+    auto key_at = [&](int at) -> uint64_t {  // the runs' largest first, then their second ones, ..: what comes later seldom enters
+      const int rank = at / a.splits;
+      return rank < a.count ? keys[(at - rank * a.splits) * a.count + rank] : 0;
+    };
+    const uint64_t first_key = key_at(lane);
+    Run run{0., -__FLT_MAX__};
+    if (lane < a.splits) run = a.runs[row * a.splits + lane];
     Candidate mine{0, -1};
     if (!(fabsf(score) <= __FLT_MAX__)) {
     } else if (ended(a, row)) {
       if (lane == 0) mine = {ordered64(score), a.stop};
     } else {
-      Run run{0., -__FLT_MAX__};
-      if (lane < a.splits) run = a.runs[row * a.splits + lane];
+      Largest top(a.count);
+      top.offer(first_key);
+      for (int first = 64; first < a.splits * a.count; first += 64) top.offer(key_at(first + lane));
       const float ref = wave_max(run.ref);
       const double sum = wave_sum(run.sum * exp((double)run.ref - (double)ref));
-      Largest top(a.count);
-      const uint64_t *const keys = a.keys + row * a.splits * a.count;
-      for (int first = 0; first < a.splits * a.count; first += 64) top.offer(first + lane < a.splits * a.count ? keys[first + lane] : 0);
       if (sum > 0. && sum <= __DBL_MAX__ && top.key)
         mine = {ordered64((double)score + (((double)logit_of(top.key) - (double)ref) - log(sum))), (int64_t)token_of(top.key)};
     }
-    if (lane < a.count) found[b * a.count + lane] = mine;
+    if (lane < a.count) {
+      found[b * a.count + lane] = mine;
+      ranks[b * a.count + lane] = lane;
+    }
+    const uint64_t some = __ballot(lane < a.count && mine.total);
+    if (lane == 0 && some) atomicAdd(&have, (int)__popcll(some));
   }
   __syncthreads();
-  // how many of beam b's are over `total`, or level with it too: they stand first
-  auto over = [&](int b, uint64_t total, bool level) {
-    int lo = 0, hi = a.count;
+  const int all = a.beams * a.count;
+  for (int i = threadIdx.x; i < all * a.beams; i += kMergeThreads) {  // a candidate, another beam
+    const int b = i / all, c = i - b * all, of = c / a.count;
+    const uint64_t total = found[c].total;
+    if (!total || b == of) continue;
+    int lo = 0, hi = a.count;  // how many of beam b's are over it
     while (lo < hi) {
       const int mid = (lo + hi) >> 1;
       const uint64_t t = found[b * a.count + mid].total;
-      if (t > total || (level && t == total)) lo = mid + 1;
+      if (t > total || (b < of && t == total)) lo = mid + 1;
       else hi = mid;
     }
-    return lo;
-  };
-  for (int i = threadIdx.x; i < a.beams * a.count; i += kMergeThreads) {
+    if (lo) atomicAdd(ranks + c, lo);
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < all; i += kMergeThreads) {
     const Candidate mine = found[i];
-    if (!mine.total) continue;
-    const int of = i / a.count;
-    int rank = i - of * a.count;
-    for (int b = 0; b < a.beams && rank < a.count; ++b)
-      if (b != of) rank += over(b, mine.total, b < of);
-    if (rank >= a.count) continue;
-    const int64_t to = n * a.count + rank;
+    if (!mine.total || ranks[i] >= a.count) continue;
+    const int64_t to = n * a.count + ranks[i];
     a.out_scores[to] = (float)total_of(mine.total);
-    a.parents[to] = of;
+    a.parents[to] = i / a.count;
     a.tokens[to] = mine.token;
   }
-  int have = 0;
-  for (int b = 0; b < a.beams && have < a.count; ++b) have += over(b, 0, false);
   for (int i = have + threadIdx.x; i < a.count; i += kMergeThreads) {
     const int64_t to = n * a.count + i;
     a.out_scores[to] = -__builtin_inff();
@@ -364,8 +472,23 @@ __global__ __launch_bounds__(kMergeThreads) void merge_kernel(SelectArgs a) {
 
 // ------------------------------------------------------------------ reordering
 
+constexpr int kMaxCaches = 256, kMaxRequests = 1024;  // of a launch of copy_kernel
 struct Copy {
-  int32_t from, to, tiles, pad;  // pages, and how many tiles of each head; from -1: nothing
+  int32_t from, to;  // pages
+};
+struct Copies {
+  int32_t count, tiles;  // of a request, and how many tiles of each page and head
+};
+struct CacheList {
+  uint8_t *data[kMaxCaches];
+};
+// What plan_kernel leaves to copy_kernel.  The caches' addresses are there too: read from the
+// launch's arguments, host memory, by every workgroup they cost more than the copies of a few
+// requests.
+struct Plan {
+  CacheList *caches;
+  Copies *requests;
+  Copy *copies;  // [requests, beams], the first `count` of each
 };
 
 struct ReorderArgs {
@@ -373,14 +496,15 @@ struct ReorderArgs {
   int64_t stride, width, pages;
   const int32_t *lengths;  // [requests, beams], the first of a request read
   const int32_t *parents;  // [requests, beams]
-  Copy *plan;              // [requests, beams]
+  Plan plan;
   int beams, page;
 };
 
 constexpr int kPlanThreads = 256, kPlanColumns = 64;
 
 // A workgroup a request.  Lane j of its first wave is beam j.
-__global__ __launch_bounds__(kPlanThreads) void plan_kernel(ReorderArgs a) {
+__global__ __launch_bounds__(kPlanThreads) void plan_kernel(ReorderArgs a, CacheList caches, int count) {
+  if (blockIdx.x == 0 && (int)threadIdx.x < count) a.plan.caches->data[threadIdx.x] = caches.data[threadIdx.x];
   __shared__ int32_t entries[MQ_MAX_BEAMS * kPlanColumns];
   __shared__ int parent[MQ_MAX_BEAMS], taken[MQ_MAX_BEAMS], dead[MQ_MAX_BEAMS], moves;
   const int64_t row0 = (int64_t)blockIdx.x * a.beams;
@@ -411,15 +535,19 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(ReorderArgs a) {
   }
   __syncthreads();
   // the partial page: which each row has now, and what is copied into it
-  if (threadIdx.x < a.beams) {
+  if (threadIdx.x < 64) {
     const int j = threadIdx.x;
-    Copy copy{-1, -1, 0, 0};
-    if (tail && full < a.width && moves) {
-      const int from = a.table[(row0 + parent[j]) * a.stride + full], to = a.table[(row0 + taken[j]) * a.stride + full];
-      if (taken[j] != parent[j] && from >= 0 && from < a.pages && to >= 0 && to < a.pages) copy = {from, to, (tail + kTileTokens - 1) / kTileTokens, 0};
+    bool copied = false;
+    int from = 0, to = 0;
+    if (j < a.beams && tail && full < a.width && moves) {
+      from = a.table[(row0 + parent[j]) * a.stride + full];
+      to = a.table[(row0 + taken[j]) * a.stride + full];
+      copied = taken[j] != parent[j] && from >= 0 && from < a.pages && to >= 0 && to < a.pages;
       entries[j] = to;
     }
-    a.plan[row0 + j] = copy;
+    const uint64_t all = __ballot(copied);
+    if (copied) a.plan.copies[row0 + __popcll(all & (((uint64_t)1 << j) - 1))] = {from, to};
+    if (j == 0) a.plan.requests[blockIdx.x] = {(int32_t)__popcll(all), (tail + kTileTokens - 1) / kTileTokens};
   }
   if (!moves) return;
   __syncthreads();
@@ -440,47 +568,70 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(ReorderArgs a) {
   }
 }
 
-constexpr int kMaxCaches = 64, kCopyThreads = 256, kCopyTiles = 4;
-struct CacheList {
-  uint8_t *data[kMaxCaches];
-};
-
-// A workgroup a (request, run of kCopyTiles tiles, head, cache): its beams' copies in turn.
-__global__ __launch_bounds__(kCopyThreads) void copy_kernel(CacheList caches, const Copy *plan, int beams, uint32_t tile_units, int tiles, int runs) {
-  const uint32_t request = blockIdx.x / (uint32_t)runs, first = (blockIdx.x - request * runs) * kCopyTiles;
-  const int64_t head = blockIdx.y, heads = gridDim.y;
-  uint4 *const data = reinterpret_cast<uint4 *>(caches.data[blockIdx.z]);
-  const int lane = threadIdx.x & 63;
-  Copy mine{-1, -1, 0, 0};
-  if (lane < beams) mine = plan[(int64_t)request * beams + lane];
-  for (uint64_t some = __ballot(mine.from >= 0 && mine.tiles > (int)first); some; some &= some - 1) {
-    const int j = __builtin_ctzll(some);
-    const int64_t page_from = __builtin_amdgcn_readlane(mine.from, j), page_to = __builtin_amdgcn_readlane(mine.to, j);
-    const int count = min(__builtin_amdgcn_readlane(mine.tiles, j) - (int)first, kCopyTiles);
-    const int64_t in = first * (int64_t)tile_units;
-    const uint4 *const from = data + (page_from * heads + head) * tiles * tile_units + in;
-    uint4 *const to = data + (page_to * heads + head) * tiles * tile_units + in;
-    const uint32_t units = count * tile_units;
-    uint32_t i = threadIdx.x;
-    for (; i + 3 * kCopyThreads < units; i += 4 * kCopyThreads) {
-      uint4 v[4];
+// Workgroups (x, cache), as many as fill the chip whatever the requests' shares are, each every
+// gridDim.x-th tile of what is copied in the cache.
+constexpr int kCopyThreads = 256;
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+template <int T, int D>
+__global__ __launch_bounds__(kCopyThreads) void copy_kernel(Plan plan, int requests, int beams, int kv_heads, int tiles) {
+  constexpr int kUnits = CacheTile<T, D>::kBytes / 16, kPer = kMaxRequests / kCopyThreads, U = (kUnits + kCopyThreads - 1) / kCopyThreads;
+  __shared__ uint32_t before[kMaxRequests], sums[kCopyThreads / 64];
+  u32x4 *const data = reinterpret_cast<u32x4 *>(plan.caches->data[blockIdx.y]);
+  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+  uint32_t mine[kPer], sum = 0;  // the tiles, of one head, of the requests before
 #pragma unroll
-      for (int u = 0; u < 4; ++u) v[u] = from[i + u * kCopyThreads];
-#pragma unroll
-      for (int u = 0; u < 4; ++u) to[i + u * kCopyThreads] = v[u];
+  for (int i = 0; i < kPer; ++i) {
+    const int r = tid * kPer + i;
+    mine[i] = sum;
+    if (r < requests) {
+      const Copies c = plan.requests[r];
+      sum += c.count * c.tiles;
     }
-    for (; i < units; i += kCopyThreads) to[i] = from[i];
+  }
+  uint32_t upto = sum;
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) {
+    const uint32_t u = __shfl_up(upto, off);
+    if (lane >= off) upto += u;
+  }
+  if (lane == 63) sums[wave] = upto;
+  __syncthreads();
+  uint32_t start = upto - sum, all = 0;
+#pragma unroll
+  for (int i = 0; i < kCopyThreads / 64; ++i) {
+    if (i < wave) start += sums[i];
+    all += sums[i];
+  }
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) before[tid * kPer + i] = start + mine[i];
+  __syncthreads();
+  const uint64_t units = (uint64_t)all * kv_heads;
+  for (uint64_t unit = blockIdx.x; unit < units; unit += gridDim.x) {
+    const uint32_t t = units >> 32 ? (uint32_t)(unit / kv_heads) : (uint32_t)unit / (uint32_t)kv_heads, head = (uint32_t)(unit - (uint64_t)t * kv_heads);
+    // the last request that starts at or before t (those without copies start where the next does)
+    const int row = __popcll(__ballot(lane < kMaxRequests / 64 && before[(lane & (kMaxRequests / 64 - 1)) * 64] <= t)) - 1;
+    const int r = row * 64 + __popcll(__ballot(before[row * 64 + lane] <= t)) - 1;
+    const uint32_t of = (uint32_t)plan.requests[r].tiles, in = t - before[r], c = in / of, tile = in - c * of;
+    const Copy copy = plan.copies[(int64_t)r * beams + c];
+    const u32x4 *const from = data + (((int64_t)copy.from * kv_heads + head) * tiles + tile) * kUnits;
+    u32x4 *const to = data + (((int64_t)copy.to * kv_heads + head) * tiles + tile) * kUnits;
+    u32x4 v[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) v[u] = from[min(u * kCopyThreads + tid, kUnits - 1)];  // none behind a branch, which would wait for the one before
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if ((u + 1) * kCopyThreads <= kUnits || u * kCopyThreads + tid < kUnits) to[u * kCopyThreads + tid] = v[u];
   }
 }
 
 int invalid(const char *msg) { return set_error(MQ_E_INVALID, msg); }
 bool aligned_to(const void *p, uintptr_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0; }
 
-// Runs of a row: enough workgroups for eight on each of 256 CUs, none below 4096 logits (16 a
-// thread), 64 at most (a lane each when they are joined).
+// Runs of a row: workgroups for four on each of 256 CUs, none of fewer than 4096 logits (16 a
+// thread), 64 at most (a lane each when they are joined).  512 rows of 128000 in f32: 58 us,
+// 64 with 2048 workgroups, 76 with 512; 80 rows of 151111 in bf16: 22.5, 24 and 26.
 int splits_of(int64_t rows, int64_t vocab) {
-  const int64_t want = (2048 + rows - 1) / rows, most = vocab / 4096;
-  const int64_t s = want < most ? want : most;
+  const int64_t want = (1024 + rows - 1) / rows, most = vocab / 4096, s = want < most ? want : most;
   return (int)(s < 1 ? 1 : s > 64 ? 64 : s);
 }
 
@@ -526,27 +677,30 @@ extern "C" int mq_beam_select(const void *logits, int dtype, int64_t requests, i
   const dim3 grid((unsigned)(rows * splits));
   if (dtype == MQ_F32) hipLaunchKernelGGL(scan_kernel<float>, grid, dim3(kScanThreads), 0, s, a);
   else hipLaunchKernelGGL(scan_kernel<__bf16>, grid, dim3(kScanThreads), 0, s, a);
-  hipLaunchKernelGGL(merge_kernel, dim3((unsigned)requests), dim3(kMergeThreads), sizeof(Candidate) * beams * count, s, a);
+  hipLaunchKernelGGL(merge_kernel, dim3((unsigned)requests), dim3(kMergeThreads), (sizeof(Candidate) + sizeof(int)) * beams * count, s, a);
   const hipError_t e = hipGetLastError();
   return e == hipSuccess ? MQ_OK : set_error(MQ_E_HIP, hipGetErrorString(e));
 }
 
 extern "C" size_t mq_beam_reorder_scratch_size(int64_t requests, int beams) {
+  using namespace mq;
   if (requests < 0 || requests > (int64_t(1) << 20) || beams < 1 || beams > MQ_MAX_BEAMS) return 0;
-  return (size_t)requests * beams * sizeof(mq::Copy);
+  return sizeof(CacheList) + (size_t)requests * (sizeof(Copies) + beams * sizeof(Copy));
 }
 
 extern "C" int mq_beam_reorder(const mq_kv_cache *caches, int count, int32_t *table, int64_t table_stride, int64_t max_pages,
                                const int32_t *lengths, const int32_t *parents, int64_t requests, int beams, void *scratch,
                                size_t scratch_bytes, void *stream) {
   using namespace mq;
-  if (!caches || count < 1) return invalid("mq_beam_reorder: no caches");
+  if (!caches || count < 1 || count > kMaxCaches) return invalid("mq_beam_reorder: 1 to 256 caches");
+  CacheList list{};
   for (int i = 0; i < count; ++i) {
     if (const char *fault = cache_fault(caches + i)) return invalid(fault);
     if (caches[i].dtype != caches[0].dtype || caches[i].pages != caches[0].pages || caches[i].kv_heads != caches[0].kv_heads ||
         caches[i].head_dim != caches[0].head_dim || caches[i].page_tokens != caches[0].page_tokens)
       return invalid("mq_beam_reorder: the caches of a model's layers are alike");
     if ((caches[i].pages && !caches[i].data) || !aligned16(caches[i].data)) return invalid("mq_beam_reorder: a cache's data is NULL or misaligned");
+    list.data[i] = static_cast<uint8_t *>(caches[i].data);
   }
   if (requests < 0 || requests > (int64_t(1) << 20) || beams < 1 || beams > MQ_MAX_BEAMS) return invalid("mq_beam_reorder: 0 to 2^20 requests, 1 to 64 beams");
   if (max_pages < 0 || max_pages >= (int64_t(1) << 31) || table_stride < max_pages || table_stride >= (int64_t(1) << 40))
@@ -557,18 +711,20 @@ extern "C" int mq_beam_reorder(const mq_kv_cache *caches, int count, int32_t *ta
   if (!aligned_to(table, 4) || !aligned_to(lengths, 4) || !aligned_to(parents, 4) || !aligned_to(scratch, 16))
     return invalid("mq_beam_reorder: misaligned buffer");
   const mq_kv_cache &c = caches[0];
-  const int tiles = c.page_tokens / kTileTokens, runs = (tiles + kCopyTiles - 1) / kCopyTiles;
-  if (requests * runs >= (int64_t(1) << 24)) return invalid("mq_beam_reorder: too many requests");
+  const int tiles = c.page_tokens / kTileTokens;
   const hipStream_t s = static_cast<hipStream_t>(stream);
-  Copy *const plan = static_cast<Copy *>(scratch);
+  Copies *const of = reinterpret_cast<Copies *>(static_cast<CacheList *>(scratch) + 1);
+  const Plan plan{static_cast<CacheList *>(scratch), of, reinterpret_cast<Copy *>(of + requests)};
   hipLaunchKernelGGL(plan_kernel, dim3((unsigned)requests), dim3(kPlanThreads), 0, s,
-                     ReorderArgs{table, table_stride, max_pages, c.pages, lengths, parents, plan, beams, c.page_tokens});
-  for (int from = 0; from < count; from += kMaxCaches) {
-    CacheList list{};
-    const int here = count - from < kMaxCaches ? count - from : kMaxCaches;
-    for (int i = 0; i < here; ++i) list.data[i] = static_cast<uint8_t *>(caches[from + i].data);
-    hipLaunchKernelGGL(copy_kernel, dim3((unsigned)(requests * runs), (unsigned)c.kv_heads, (unsigned)here), dim3(kCopyThreads), 0, s, list, plan, beams,
-                       (uint32_t)(cache_tile_bytes(c.dtype, c.head_dim) / 16), tiles, runs);
+                     ReorderArgs{table, table_stride, max_pages, c.pages, lengths, parents, plan, beams, c.page_tokens}, list, count);
+  for (int64_t first = 0; first < requests; first += kMaxRequests) {
+    const int here = (int)(requests - first < kMaxRequests ? requests - first : kMaxRequests);
+    // sixteen workgroups for each of 256 CUs, or as many as there can be tiles to copy
+    const int64_t most = (int64_t)here * (beams - 1) * tiles * c.kv_heads, fill = (4096 + count - 1) / count;
+    with_cache_type(&c, [&]<int T, int D>() {
+      hipLaunchKernelGGL((copy_kernel<T, D>), dim3((unsigned)(most < fill ? most : fill), (unsigned)count), dim3(kCopyThreads), 0, s,
+                         Plan{plan.caches, plan.requests + first, plan.copies + first * beams}, here, beams, c.kv_heads, tiles);
+    });
   }
   const hipError_t e = hipGetLastError();
   return e == hipSuccess ? MQ_OK : set_error(MQ_E_HIP, hipGetErrorString(e));

@@ -95,21 +95,26 @@ def _head_rows(name, t, shape, dtype, device):
     return t, st, sh
 
 
-def _vector(name, t, dtype, size, device):
-    """t, contiguous and 16-byte aligned, of `size` elements."""
-    if t.dtype is not dtype or t.shape != (size,) or t.device != device:
-        raise ValueError(f"{name} must be {str(dtype)[6:]} [{size}] on {device}")
+def _vector(name, what, t, size, device):
+    """t, f32 of `size` elements, contiguous and 16-byte aligned."""
+    if t.dtype is not torch.float32 or t.shape != (size,) or t.device != device:
+        raise ValueError(f"{name}: {what} must be float32 [{size}] on {device}")
     return t if t.is_contiguous() and not t.data_ptr() & 15 else _copied(t)
 
 
-def _rotation(name, tokens, dim, positions, inv_freq, q_weight, k_weight, device):
+def _rotation(name, q, k, v, positions, inv_freq, q_weight, k_weight, device, tokens, dim):
     """The rotation's operands as the library reads them; a weight that is None stays None."""
+    if recorded(q, k, v, inv_freq, inv_freq if q_weight is None else q_weight, inv_freq if k_weight is None else k_weight):
+        raise ValueError(f"{name}: inference only, nothing may record the call")
     if positions.dtype is not torch.int64 or positions.shape != (tokens,) or positions.device != device:
         raise ValueError(f"{name}: positions must be int64 [{tokens}] on {device}")
     if not positions.is_contiguous():
         positions = positions.contiguous()
-    inv_freq = _vector(f"{name}: inv_freq", inv_freq, torch.float32, dim // 2, device)
-    q_weight, k_weight = (w if w is None else _vector(f"{name}: norm weights", w, torch.float32, dim, device) for w in (q_weight, k_weight))
+    inv_freq = _vector(name, "inv_freq", inv_freq, dim // 2, device)
+    if q_weight is not None:
+        q_weight = _vector(name, "a norm's weight", q_weight, dim, device)
+    if k_weight is not None:
+        k_weight = _vector(name, "a norm's weight", k_weight, dim, device)
     return positions, inv_freq, q_weight, k_weight
 
 
@@ -117,25 +122,20 @@ def _address(t):
     return None if t is None else t.data_ptr()
 
 
-def _float_rows(name, q, k):
-    if q.dim() != 3 or k.dim() != 3 or q.dtype not in (_BF16, torch.float32) or q.device.type != "cuda" or q.shape[1] == 0 or k.shape[1] == 0:
-        raise ValueError(f"{name}: q and k must be bf16 or f32 [tokens, heads, dim] on a GPU")
-
-
 def rotate_heads(q, k, positions, inv_freq, q_weight=None, k_weight=None, eps: float = 1e-6):
     """Each head of q [tokens, heads, dim] and k [tokens, kv_heads, dim] (bf16 or f32, both the same;
     dim 64 or 128) RmsNormed with its weight (f32 [dim]; None: as it is) and its halves rotated by
     positions[t] * inv_freq[i] (int64 [tokens], f32 [dim / 2]) -> (q, k) in bf16."""
-    if recorded(*(t for t in (q, k, inv_freq, q_weight, k_weight) if t is not None)):
-        raise ValueError("rotate_heads: inference only, nothing may record the call")
-    _float_rows("rotate_heads", q, k)
-    (n, heads, dim), device, dtype = q.shape, q.device, q.dtype
-    if dim not in (64, 128):
-        raise ValueError("rotate_heads: heads of 64 or 128")
+    dtype, device = q.dtype, q.device
+    if q.dim() != 3 or k.dim() != 3 or dtype is not _BF16 and dtype is not torch.float32 or device.type != "cuda":
+        raise ValueError("rotate_heads: q and k must be bf16 or f32 [tokens, heads, dim] on a GPU")
+    n, heads, dim = q.shape
     kv_heads = k.shape[1]
-    q, qt, qh = _head_rows("rotate_heads: q and k", q, (n, heads, dim), dtype, device)
-    k, kt, kh = _head_rows("rotate_heads: q and k", k, (n, kv_heads, dim), dtype, device)
-    positions, inv_freq, q_weight, k_weight = _rotation("rotate_heads", n, dim, positions, inv_freq, q_weight, k_weight, device)
+    if dim != 64 and dim != 128 or heads == 0 or kv_heads == 0:
+        raise ValueError("rotate_heads: heads of 64 or 128, at least one of q and of k")
+    positions, inv_freq, q_weight, k_weight = _rotation("rotate_heads", q, k, k, positions, inv_freq, q_weight, k_weight, device, n, dim)
+    q, qt, qh = _head_rows("rotate_heads: q", q, (n, heads, dim), dtype, device)
+    k, kt, kh = _head_rows("rotate_heads: k, as q,", k, (n, kv_heads, dim), dtype, device)
     q_out = torch.empty((n, heads, dim), dtype=_BF16, device=device)
     k_out = torch.empty((n, kv_heads, dim), dtype=_BF16, device=device)
     if n:
@@ -332,17 +332,17 @@ class KvCache:
         rotated keys and v appended to `slots` in the same pass -> (q, k) in bf16, k None unless
         `keys` asks for it (a prompt's attention reads it, a step's reads the cache)."""
         name = "KvCache.append_rotated"
-        if recorded(*(t for t in (q, k, v, inv_freq, q_weight, k_weight) if t is not None)):
-            raise ValueError(f"{name}: inference only, nothing may record the call")
-        _float_rows(name, q, k)
+        device, dtype, dim = self.device, q.dtype, self.head_dim
+        if q.dim() != 3 or q.shape[1] == 0 or dtype is not _BF16 and dtype is not torch.float32:
+            raise ValueError(f"{name}: q must be bf16 or f32 [tokens, heads, {dim}]")
         slots = self._slots(name, slots)
-        n, heads, device, dtype = slots.shape[0], q.shape[1], self.device, q.dtype
-        shape = (n, self.kv_heads, self.head_dim)
-        q, qt, qh = _head_rows(f"{name}: q", q, (n, heads, self.head_dim), dtype, device)
-        k, kt, kh = _head_rows(f"{name}: q, k and v", k, shape, dtype, device)
-        v, vt, vh = _head_rows(f"{name}: q, k and v", v, shape, dtype, device)
-        positions, inv_freq, q_weight, k_weight = _rotation(name, n, self.head_dim, positions, inv_freq, q_weight, k_weight, device)
-        q_out = torch.empty((n, heads, self.head_dim), dtype=_BF16, device=device)
+        n, heads = slots.shape[0], q.shape[1]
+        shape = (n, self.kv_heads, dim)
+        positions, inv_freq, q_weight, k_weight = _rotation(name, q, k, v, positions, inv_freq, q_weight, k_weight, device, n, dim)
+        q, qt, qh = _head_rows("KvCache.append_rotated: q", q, (n, heads, dim), dtype, device)
+        k, kt, kh = _head_rows("KvCache.append_rotated: k, as q,", k, shape, dtype, device)
+        v, vt, vh = _head_rows("KvCache.append_rotated: v, as q,", v, shape, dtype, device)
+        q_out = torch.empty((n, heads, dim), dtype=_BF16, device=device)
         k_out = torch.empty(shape, dtype=_BF16, device=device) if keys else None
         if n:
             self._run(_lib.load().mq_kv_cache_append_rotated, self._ref, slots.data_ptr(), q.data_ptr(), qt, qh, heads, k.data_ptr(), kt,
@@ -360,8 +360,10 @@ class KvCache:
         if recorded(counts):
             raise ValueError("KvCache.place: inference only, nothing may record the call")
         counts = self._whole("KvCache.place: counts", counts)
+        page_count, pages_at = self.pages, None
         if pages is not None:
             pages = self._whole("KvCache.place: pages", pages)
+            page_count, pages_at = pages.shape[0], pages.data_ptr()
         if tokens < 0 or width < 0 or beams < 1:
             raise ValueError(f"KvCache.place: {tokens} tokens, {width} pages, {beams} beams")
         n, device = counts.shape[0], self.device
@@ -370,9 +372,8 @@ class KvCache:
         positions = torch.empty(tokens, dtype=torch.int64, device=device)
         lengths = torch.empty(n * beams, dtype=torch.int32, device=device)
         last = torch.empty(n, dtype=torch.int64, device=device)
-        _run_on(device, _lib.load().mq_cache_place, self._ref, counts.data_ptr(), n, beams, room, _address(pages),
-                self.pages if pages is None else pages.shape[0], table.data_ptr(), width, width, tokens, slots.data_ptr(), positions.data_ptr(),
-                lengths.data_ptr(), last.data_ptr())
+        _run_on(device, _lib.load().mq_cache_place, self._ref, counts.data_ptr(), n, beams, room, pages_at, page_count, table.data_ptr(), width, width,
+                tokens, slots.data_ptr(), positions.data_ptr(), lengths.data_ptr(), last.data_ptr())
         return Placed(table, slots, positions, lengths, last)
 
     def extend(self, page_table, held, counts=None, tokens: Optional[int] = None):

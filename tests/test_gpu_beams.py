@@ -205,11 +205,14 @@ def _states(layers, pages, kv, dim, page, t, seed=0):
     return caches
 
 
-def _bytes_of(cache, pages, length):
+def _raw(cache):
+    """The cache's bytes on the host, as [pages, heads, tiles, ..]."""
+    return cache.data.view(cache.pages, cache.kv_heads, cache.page_tokens // 32, -1).cpu()
+
+
+def _bytes_of(cache, pages, length, data=None):
     """What a sequence of `length` tokens over `pages` holds: the raw tiles that its tokens reach, as [heads, tiles, ..] of each page."""
-    tiles = cache.page_tokens // 32
-    data = cache.data.view(cache.pages, cache.kv_heads, tiles, -1).cpu()
-    out = []
+    data, out = _raw(cache) if data is None else data, []
     for c, page in enumerate(pages):
         left = min(cache.page_tokens, length - c * cache.page_tokens)
         if left <= 0:
@@ -254,10 +257,10 @@ def test_reorder(t, beams):
             parents = [[rng.choice([j, 0, rng.randrange(beams), rng.randrange(beams)]) for j in range(beams)] for _ in range(n)]
             if step == 1:
                 parents[0] = [beams - 1 - j for j in range(beams)]            # nothing but a permutation
-            before = [[_bytes_of(c, table[i * beams + j], lengths[i]) for j in range(beams)] for c in caches for i in range(n)]
-            raw = [c.data.view(c.pages, -1).clone() for c in caches]
+            raw = [_raw(c) for c in caches]
+            before = [[_bytes_of(c, table[i * beams + j], lengths[i], r) for j in range(beams)] for c, r in zip(caches, raw) for i in range(n)]
             states.reorder(dev, now, torch.tensor(parents, dtype=torch.int32, device="cuda"))
-            after = dev.tolist()
+            after, now_raw = dev.tolist(), [_raw(c) for c in caches]
             for i in range(n):
                 full = lengths[i] // page
                 rows = after[i * beams:(i + 1) * beams]
@@ -267,12 +270,12 @@ def test_reorder(t, beams):
                 for j, r in enumerate(rows):
                     assert r[:full] == table[i * beams + parents[i][j]][:full]
                     for layer, c in enumerate(caches):
-                        got = _bytes_of(c, r, lengths[i])
+                        got = _bytes_of(c, r, lengths[i], now_raw[layer])
                         assert len(got) == len(before[layer * n + i][parents[i][j]])
                         assert all(torch.equal(a, b) for a, b in zip(got, before[layer * n + i][parents[i][j]])), (i, j, layer)
                 kept = set(parents[i])
                 copies = beams - len(kept) if lengths[i] % page else 0
-                changed = sum(int((caches[0].data.view(pages + 2, -1)[p] != raw[0][p]).any()) for p in {p for r in rows for p in r[full:full + 1]})
+                changed = sum(not torch.equal(now_raw[0][p], raw[0][p]) for p in {p for r in rows for p in r[full:full + 1]})
                 assert changed <= copies
             table = after
 
@@ -386,7 +389,7 @@ def test_refusals_of_the_library():
         assert lib.mq_beam_reorder_scratch_size(*args) == 0
     two = (_lib.KvCacheC * 2)(_lib.KvCacheC(a, 4, 8, 2, 128, 64), _lib.KvCacheC(a, 4, 8, 2, 128, 64))
     ok = dict(caches=two, count=2, table=a, stride=5, width=5, lengths=a, parents=a, n=2, beams=4, scratch=a, size=lib.mq_beam_reorder_scratch_size(2, 4), stream=None)
-    for change in (dict(caches=None), dict(count=0), dict(table=None), dict(stride=4), dict(stride=1 << 40), dict(width=-1), dict(width=1 << 31), dict(lengths=None), dict(parents=None),
+    for change in (dict(caches=None), dict(count=0), dict(count=257), dict(table=None), dict(stride=4), dict(stride=1 << 40), dict(width=-1), dict(width=1 << 31), dict(lengths=None), dict(parents=None),
                    dict(n=-1), dict(n=(1 << 20) + 1), dict(beams=0), dict(beams=65), dict(scratch=None), dict(size=1), dict(table=a + 2), dict(lengths=a + 1), dict(parents=a + 2), dict(scratch=a + 8)):
         assert lib.mq_beam_reorder(*{**ok, **change}.values()) == bad, change
     assert lib.mq_beam_reorder(*{**ok, "n": 0}.values()) == 0 and lib.mq_beam_reorder(*{**ok, "beams": 1}.values()) == 0
