@@ -6,18 +6,23 @@
 //   out_i = y_i cos a_i - y_(i+D/2) sin a_i,   out_(i+D/2) = y_(i+D/2) cos a_i + y_i sin a_i
 //
 // in f32, rounded once to bf16.  The angle is taken in 64 bits as turns, of which the whole
-// ones are dropped, so that far positions lose nothing; v_sin_f32 and v_cos_f32 take turns.
+// ones are dropped, so that far positions lose nothing; v_sin_f32 and v_cos_f32 take turns
+// and are at most 2^-22.9 off over a whole one.
 //
 // A value is read and written once; the bound is HBM, the launch for a step's few tokens.
 // D / 8 lanes hold a head, each four values of its lower half and the four that they are
 // rotated with, so that only the sum of squares crosses lanes, and a wave takes four heads
 // of 128 (eight of 64) of one token at a time.  A lane's four angles serve all heads of the
 // token that the wave takes: one pass of heads while tokens are few, the more the more waves
-// there are to fill the chip anyway.
+// there are to fill the chip anyway.  4100 tokens of 16 / 8 heads of 128 in bf16, 50 MB: 14.1 us;
+// with twice the waves 17, with passes loaded four at a time 15.5.  7305 tokens of 20 / 20 heads
+// of 64 from f32, 112 MB: 19 us (5.8 TB/s, part of it from the caches).
 //
 // Into the cache, a workgroup of 2 D threads takes 32 tokens of one k head through LDS
 // (as bf16, what the attention of the prompt itself reads) into the shape in which
-// mq_cache_write.h stores tiles; workgroups of v's and of q's share the launch.
+// mq_cache_write.h stores tiles; workgroups of v's and of q's share the launch.  32768
+// tokens of 32 / 8 heads of 128 from bf16 into Q8_0, 809 MB read and written: 160 us (5.1 TB/s),
+// 175 with all of q's workgroups behind the writing ones, whose vector work is half of the time.
 #include "../../include/moldq.h"
 #include "mq_cache_write.h"
 
@@ -149,13 +154,12 @@ __device__ __forceinline__ void turn(const Piece<X> &p, const Weights &w, const 
   out[1] = make_uint2(pack2(b[0], b[1]), pack2(b[2], b[3]));
 }
 
-// Wave `item` of the tokens' q heads and, with kKeys, k heads: passes of 64 / (D / 8)
-// heads, q's first, `passes` of them from part * passes on.
+// Part `part` of a token's q heads and, with kKeys, k heads, by one wave: passes of
+// 64 / (D / 8) heads, q's first, `passes` of them from part * passes on.
 template <int D, typename X, bool kKeys>
-__device__ __forceinline__ void rotate_item(const HeadArgs &a, uint32_t item) {
+__device__ __forceinline__ void rotate_part(const HeadArgs &a, uint32_t token, uint32_t part) {
   constexpr int kLanes = D / 8, kHeads = 64 / kLanes;
   const int lane = threadIdx.x & 63, sub = lane & (kLanes - 1), in = lane / kLanes;
-  const uint32_t token = item / (uint32_t)a.parts, part = item - token * (uint32_t)a.parts;
   const int q_passes = (a.q.heads + kHeads - 1) / kHeads, all = q_passes + (kKeys ? (a.k.heads + kHeads - 1) / kHeads : 0);
   int pass = (int)part * a.passes;
   const int end = min(all, pass + a.passes);
@@ -194,8 +198,8 @@ __device__ __forceinline__ void rotate_item(const HeadArgs &a, uint32_t item) {
 
 template <int D, typename X>
 __global__ __launch_bounds__(256) void rotate_kernel(HeadArgs a) {
-  const uint32_t item = blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (item < a.tokens * a.parts) rotate_item<D, X, true>(a, item);
+  const uint32_t item = blockIdx.x * 4 + (threadIdx.x >> 6), token = item / (uint32_t)a.parts;
+  if (token < a.tokens) rotate_part<D, X, true>(a, token, item - token * (uint32_t)a.parts);
 }
 
 struct ValueRows {
@@ -203,18 +207,19 @@ struct ValueRows {
   int64_t token, head;
 };
 
-// Workgroups 0 .. 2 kv_heads groups - 1 write the cache (a group of 32 tokens: its k heads,
-// then its v heads), the rest rotate q.
+// A group of 32 tokens has a workgroup for each of its k heads, then of its v heads, which
+// write the cache, then `rotators` that rotate its q: neighbours, so that the vector work of the
+// first and the bytes of the last overlap.
 template <int T, int D, typename X>
-__global__ __launch_bounds__(2 * D) void append_rotated_kernel(CacheView c, HeadArgs a, ValueRows v, const int64_t *slots, uint32_t writers) {
+__global__ __launch_bounds__(2 * D) void append_rotated_kernel(CacheView c, HeadArgs a, ValueRows v, const int64_t *slots, uint32_t rotators) {
   constexpr int kLanes = D / 8, kPitch = D + 8;  // rows 16 bytes apart beyond their size: a column of 16 rows in all banks
   __shared__ __attribute__((aligned(16))) __bf16 rows[kRows * kPitch];
-  if (blockIdx.x >= writers) {
-    const uint32_t item = (blockIdx.x - writers) * (D / 32) + (threadIdx.x >> 6);
-    if (item < a.tokens * a.parts) rotate_item<D, X, false>(a, item);
+  const uint32_t heads = (uint32_t)c.kv_heads, each = 2 * heads + rotators, group = blockIdx.x / each, in = blockIdx.x - group * each;
+  if (in >= 2 * heads) {
+    const uint32_t item = (in - 2 * heads) * (D / 32) + (threadIdx.x >> 6), row = item / (uint32_t)a.parts, token = group * kRows + row;
+    if (token < a.tokens) rotate_part<D, X, false>(a, token, item - row * (uint32_t)a.parts);
     return;
   }
-  const uint32_t heads = (uint32_t)c.kv_heads, group = blockIdx.x / (2 * heads), in = blockIdx.x - group * 2 * heads;
   const int64_t row0 = (int64_t)group * kRows;
   const int last = (int)min(a.tokens - row0, (int64_t)kRows) - 1, b = threadIdx.x >> 6, lane = threadIdx.x & 63;
   const int head = (int)(in >= heads ? in - heads : in);
@@ -346,19 +351,19 @@ extern "C" int mq_kv_cache_append_rotated(const mq_kv_cache *c, const int64_t *s
   HeadArgs a{{q, q_token_stride, q_head_stride, heads, q_weight, static_cast<__bf16 *>(q_out)},
              {k, k_token_stride, k_head_stride, c->kv_heads, k_weight, static_cast<__bf16 *>(k_out)},
              positions, inv_freq, eps, tokens, 0, 0};
-  const int each = 64 / (c->head_dim / 8), waves = c->head_dim / 32;
-  const int64_t writers = (tokens + kRows - 1) / kRows * 2 * c->kv_heads;
-  const int64_t groups = writers + (share(a, (heads + each - 1) / each) + waves - 1) / waves;
+  const int each = 64 / (c->head_dim / 8);
+  share(a, (heads + each - 1) / each);
+  const int64_t rotators = (int64_t)kRows * a.parts / (c->head_dim / 32), groups = (tokens + kRows - 1) / kRows * (2 * c->kv_heads + rotators);
   if (!takes_grid(groups, 2 * c->head_dim)) return invalid("mq_kv_cache_append_rotated: too many tokens for the heads");
   const dim3 grid((unsigned)groups);
   const ValueRows rows{v, v_token_stride, v_head_stride};
   with_cache_type(c, [&]<int T, int D>() {
     if (x_dtype == MQ_F32)
       hipLaunchKernelGGL((append_rotated_kernel<T, D, float>), grid, dim3(2 * D), 0, static_cast<hipStream_t>(stream), view(c), a, rows, slots,
-                         (uint32_t)writers);
+                         (uint32_t)rotators);
     else
       hipLaunchKernelGGL((append_rotated_kernel<T, D, __bf16>), grid, dim3(2 * D), 0, static_cast<hipStream_t>(stream), view(c), a, rows, slots,
-                         (uint32_t)writers);
+                         (uint32_t)rotators);
   });
   const hipError_t e = hipGetLastError();
   return e == hipSuccess ? MQ_OK : set_error(MQ_E_HIP, hipGetErrorString(e));

@@ -212,8 +212,9 @@ class TextDecoder:
         finds the most probable, best first -> (tokens [n, beams, count], their log probabilities
         [n, beams]).  A continuation that has given `stop` repeats it and keeps its probability;
         where there are fewer continuations than beams, the rest have tokens -1, probability 0."""
-        if count < 0:
-            raise ValueError(f"TextDecoder.beam_search: {count} tokens")
+        vocab = self.weights["token_embd.weight"].shape[0]
+        if count < 0 or stop is not None and not 0 <= stop < vocab:
+            raise ValueError(f"TextDecoder.beam_search: {count} tokens, stop {stop} of {vocab}")
         logits, chosen = self.prefill(prompts, room=count, beams=beams)[:, None], []
         n, last = len(prompts), None
         scores = torch.zeros((n, 1), device=self.device)

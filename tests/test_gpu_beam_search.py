@@ -80,7 +80,7 @@ def test_edges(model):  # noqa: F811
     tokens, scores = dec.beam_search(PROMPTS, 3, 0)
     assert tokens.shape == (4, 3, 0) and (scores == 0).all()
     for call in (lambda: dec.beam_search(PROMPTS, 0, 4), lambda: dec.beam_search(PROMPTS, 65, 4), lambda: dec.beam_search(PROMPTS, 2, -1), lambda: dec.beam_search([], 2, 3),
-                 lambda: dec.beam_search(PROMPTS, 30, 40), lambda: dec.beam_search([[VOCAB]], 2, 2), lambda: dec.beam_search(PROMPTS, 2, 3, stop=VOCAB)):
+                 lambda: dec.beam_search(PROMPTS, 30, 40), lambda: dec.beam_search([[VOCAB]], 2, 2), lambda: dec.beam_search(PROMPTS, 2, 3, stop=VOCAB), lambda: dec.beam_search(PROMPTS, 2, 1, stop=-1)):
         with pytest.raises(ValueError):
             call()
     again = dec.beam_search(PROMPTS, 3, 5)

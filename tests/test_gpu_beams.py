@@ -319,6 +319,24 @@ def test_reorder_many_layers_and_views():
 
 
 @gpu
+def test_reorder_of_many_requests():
+    """More requests than one launch copies for, most of them without copies, the last with some."""
+    n, beams, page = 2500, 2, 32
+    table = torch.arange(n * beams * 2, dtype=torch.int32, device="cuda").view(n * beams, 2)
+    cache = _states(1, n * beams * 2, 1, 64, page, GgmlDType.Q4_0)[0]
+    parents = torch.tensor([[0, 1]] * n, dtype=torch.int32, device="cuda")
+    some = [0, 63, 64, 700, 1023, 1024, 1025, 2047, 2048, 2499]
+    parents[some] = torch.tensor([1, 1], dtype=torch.int32, device="cuda")
+    lengths = torch.full((n * beams,), 7, dtype=torch.int32, device="cuda")
+    want = _raw(cache)
+    for i in some:
+        want[4 * i] = want[4 * i + 2]
+    BeamStates([cache]).reorder(table, lengths, parents)
+    assert torch.equal(_raw(cache), want)
+    assert torch.equal(table, torch.arange(n * beams * 2, dtype=torch.int32, device="cuda").view(n * beams, 2))
+
+
+@gpu
 def test_reorder_refusals():
     caches = _states(2, 8, 1, 64, 32, GgmlDType.Q8_0)
     states = BeamStates(caches)
