@@ -387,7 +387,7 @@ size_t mq_cache_attention_scratch_size(const mq_kv_cache *cache, int64_t batch, 
  * (f32 [head_dim]) is not NULL, x / sqrt(mean(x^2) + eps) * weight, and then its halves
  * rotated by the token's position: with a = positions[t] * inv_freq[i], value i becomes
  * x_i cos a - x_(i+D/2) sin a and value i + D/2 becomes x_(i+D/2) cos a + x_i sin a (f32;
- * angles in 64 bits; rounded once to bf16).  q, k: F32 or BF16, head h of token t at t *
+ * angles in 64 bits, exact for positions of up to 2^31 either way; rounded once to bf16).  q, k: F32 or BF16, head h of token t at t *
  * token_stride + h * head_stride, unit stride inside a head, 16-byte aligned, strides
  * multiples of 16 bytes below 2^24 elements; positions int64 and inv_freq f32
  * [head_dim / 2] in device memory; head_dim 64 or 128.  q_out, k_out: bf16, contiguous,
@@ -437,7 +437,7 @@ int mq_cache_extend(const mq_kv_cache *cache, const int32_t *held, const int32_t
  * 64 bits, then the lower beam.  logits F32 or BF16, row of beam b of request n at n *
  * request_stride + b * beam_stride (elements, any alignment), unit stride inside; scores
  * f32 [requests, beams].  A beam whose last[n, b] (int64; NULL: no beam has) is `stop` has
- * ended: it has one continuation, `stop` at its score, and its logits are not read.  A beam
+ * ended: it has one continuation, `stop` at its score, whatever its logits are.  A beam
  * whose score is not finite, or among whose logits is a NaN or plus infinity, has none, nor
  * has a logit of minus infinity; places left over have score minus infinity, parent 0,
  * token -1.  out_scores f32, parents int32 and tokens int64 [requests, count]; scratch: at
@@ -450,8 +450,8 @@ size_t mq_beam_select_scratch_size(int64_t requests, int beams, int64_t vocab, i
 /* Beam j of each request goes on from beam parents[n, j] (int32; itself if outside 0 ..
  * beams - 1), whose tokens so far become its own: in the page table (row n * beams + j,
  * changed in place) whole pages are shared, the last, partial page is passed on to one child
- * of each beam and copied, in each of the `count` caches (a model's layers, alike), for the
- * others, into the pages of beams without a child.  lengths int32 [requests, beams]: the
+ * of each beam and copied, in each of the `count` caches (a model's layers, alike, up to 256), for
+ * the others, into the pages of beams without a child.  lengths int32 [requests, beams]: the
  * tokens so far, of which a request's beams have the same number (its first entry is
  * read).  From the partial page on, no two rows share a page.  scratch: at least
  * mq_beam_reorder_scratch_size bytes (device, 16-byte aligned, of this call alone).

@@ -125,7 +125,8 @@ def _address(t):
 def rotate_heads(q, k, positions, inv_freq, q_weight=None, k_weight=None, eps: float = 1e-6):
     """Each head of q [tokens, heads, dim] and k [tokens, kv_heads, dim] (bf16 or f32, both the same;
     dim 64 or 128) RmsNormed with its weight (f32 [dim]; None: as it is) and its halves rotated by
-    positions[t] * inv_freq[i] (int64 [tokens], f32 [dim / 2]) -> (q, k) in bf16."""
+    positions[t] * inv_freq[i] (int64 [tokens] of up to 2^31 either way, f32 [dim / 2]) -> (q, k) in
+    bf16."""
     dtype, device = q.dtype, q.device
     if q.dim() != 3 or k.dim() != 3 or dtype is not _BF16 and dtype is not torch.float32 or device.type != "cuda":
         raise ValueError("rotate_heads: q and k must be bf16 or f32 [tokens, heads, dim] on a GPU")
@@ -364,8 +365,8 @@ class KvCache:
         if pages is not None:
             pages = self._whole("KvCache.place: pages", pages)
             page_count, pages_at = pages.shape[0], pages.data_ptr()
-        if tokens < 0 or width < 0 or beams < 1:
-            raise ValueError(f"KvCache.place: {tokens} tokens, {width} pages, {beams} beams")
+        if tokens < 0 or width < 0 or not 1 <= beams <= _lib.MQ_MAX_BEAMS or not 0 <= room < 1 << 31:
+            raise ValueError(f"KvCache.place: {tokens} tokens, {width} pages, {beams} beams, room for {room}")
         n, device = counts.shape[0], self.device
         table = torch.empty((n * beams, width), dtype=torch.int32, device=device)
         slots = torch.empty(tokens, dtype=torch.int64, device=device)

@@ -337,6 +337,60 @@ def test_reorder_of_many_requests():
 
 
 @gpu
+def test_states_dropped_behind_another_stream():
+    """The caches' memory is not given to other tensors before a reordering that still uses it has ended."""
+    from tests.test_gpu_text_streams import _dropped_on
+    table = torch.arange(8, dtype=torch.int32, device="cuda").view(4, 2)
+    lengths, parents = torch.full((4,), 7, dtype=torch.int32, device="cuda"), torch.tensor([[1, 1, 3, 3]], dtype=torch.int32, device="cuda")
+    caches = _states(1, 8, 1, 64, 32, GgmlDType.Q8_0)
+    states = BeamStates(caches)
+    torch.cuda.synchronize()
+
+    def own():
+        nonlocal caches, states
+        at = caches[0].data.data_ptr(), caches[0].data.numel()
+        caches = states = None
+        return at
+    _, early = _dropped_on(torch.cuda.Stream(), lambda: states.reorder(table, lengths, parents), own)
+    assert not early
+
+
+@gpu
+def test_two_streams_at_once():
+    """Selections and reorderings of different sizes on two streams, neither waiting for the other."""
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    jobs = []
+    for i, (n, beams, vocab, count) in enumerate([(5, 4, 40001, 4), (40, 3, 20000, 3)]):
+        logits, scores = _logits(n, beams, vocab, seed=30 + i)
+        table = torch.arange(n * beams * 2, dtype=torch.int32, device="cuda").view(n * beams, 2)
+        caches = _states(3, n * beams * 2, 2, 64, 32, GgmlDType.Q8_0, seed=i)
+        jobs.append((logits, scores, count, BeamStates(caches), table, torch.full((n * beams,), 9, dtype=torch.int32, device="cuda"), caches))
+
+    def run(job, times):
+        out = []
+        for _ in range(times):
+            got = select_beams(job[0], job[1], job[2])
+            job[3].reorder(job[4], job[5], got[1])
+            out.append(got)
+        return out
+    start = [(j[4].clone(), [c.data.clone() for c in j[6]]) for j in jobs]
+    want = [(run(j, 20), j[4].clone(), [c.data.clone() for c in j[6]]) for j in jobs]
+    for j, (table, data) in zip(jobs, start):
+        j[4].copy_(table)
+        for c, d in zip(j[6], data):
+            c.data.copy_(d)
+    torch.cuda.synchronize()
+    got = []
+    for j, s in zip(jobs, streams):
+        with torch.cuda.stream(s):
+            got.append(run(j, 20))
+    torch.cuda.synchronize()
+    for j, g, (w, table, data) in zip(jobs, got, want):
+        assert all(torch.equal(a, b) for x, y in zip(g, w) for a, b in zip(x, y))
+        assert torch.equal(j[4], table) and all(torch.equal(c.data, d) for c, d in zip(j[6], data))
+
+
+@gpu
 def test_reorder_refusals():
     caches = _states(2, 8, 1, 64, 32, GgmlDType.Q8_0)
     states = BeamStates(caches)
