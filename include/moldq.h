@@ -446,7 +446,7 @@ int mq_cache_extend(const mq_kv_cache *cache, const int32_t *held, const int32_t
 int mq_beam_select(const void *logits, int dtype, int64_t requests, int beams, int64_t vocab, int64_t request_stride,
                    int64_t beam_stride, const float *scores, const int64_t *last, int64_t stop, int count, float *out_scores,
                    int32_t *parents, int64_t *tokens, void *scratch, size_t scratch_bytes, void *stream);
-size_t mq_beam_select_scratch_size(int64_t requests, int beams, int64_t vocab, int count);
+size_t mq_beam_select_scratch_size(int64_t requests, int beams, int64_t vocab, int count, int dtype);
 /* Beam j of each request goes on from beam parents[n, j] (int32; itself if outside 0 ..
  * beams - 1), whose tokens so far become its own: in the page table (row n * beams + j,
  * changed in place) whole pages are shared, the last, partial page is passed on to one child

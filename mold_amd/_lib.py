@@ -94,7 +94,7 @@ SIGNATURES = {
                        + [_vp] * 5),
     "mq_cache_extend": (_int, [ctypes.POINTER(KvCacheC), _vp, _vp, _i64, _vp, _i64, _i64, _i64] + [_vp] * 4),
     "mq_beam_select": (_int, [_vp, _int, _i64, _int, _i64, _i64, _i64, _vp, _vp, _i64, _int] + [_vp] * 4 + [_sz, _vp]),
-    "mq_beam_select_scratch_size": (_sz, [_i64, _int, _i64, _int]),
+    "mq_beam_select_scratch_size": (_sz, [_i64, _int, _i64, _int, _int]),
     "mq_beam_reorder": (_int, [ctypes.POINTER(KvCacheC), _int, _vp, _i64, _i64, _vp, _vp, _i64, _int, _vp, _sz, _vp]),
     "mq_beam_reorder_scratch_size": (_sz, [_i64, _int]),
     "mq_gguf_open": (_int, [ctypes.c_char_p, _pp]),

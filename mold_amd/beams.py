@@ -59,16 +59,19 @@ def select_beams(logits, scores, count=None, last=None, stop=None):
     if sv != 1 and vocab > 1 or sn >= _MAX_STRIDE or sb >= _MAX_STRIDE:
         logits = logits.contiguous()
         sn, sb, _ = logits.stride()
-    totals = torch.empty((n, count), dtype=torch.float32, device=device)
-    parents = torch.empty((n, count), dtype=torch.int32, device=device)
-    tokens = torch.empty((n, count), dtype=torch.int64, device=device)
+    if count == beams:
+        totals = torch.empty_like(scores)
+        parents, tokens = torch.empty_like(scores, dtype=torch.int32), torch.empty_like(scores, dtype=torch.int64)
+    else:
+        totals = scores.new_empty((n, count))
+        parents, tokens = scores.new_empty((n, count), dtype=torch.int32), scores.new_empty((n, count), dtype=torch.int64)
     if n:
-        lib = _lib.load()
-        nbytes = lib.mq_beam_select_scratch_size(n, beams, vocab, count)
-        scratch = torch.empty(nbytes, dtype=torch.uint8, device=device)     # freed to this stream
-        _run_on(device, lib.mq_beam_select, logits.data_ptr(), _dtype_code(logits.dtype), n, beams, vocab, sn, sb, scores.data_ptr(),
+        lib, code = _lib.load(), _dtype_code(logits.dtype)
+        nbytes = lib.mq_beam_select_scratch_size(n, beams, vocab, count, code)
+        scratch = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None     # freed to this stream
+        _run_on(device, lib.mq_beam_select, logits.data_ptr(), code, n, beams, vocab, sn, sb, scores.data_ptr(),
                 last_at, 0 if stop is None else stop, count, totals.data_ptr(), parents.data_ptr(),
-                tokens.data_ptr(), scratch.data_ptr(), nbytes)
+                tokens.data_ptr(), scratch.data_ptr() if nbytes else None, nbytes)
     return totals, parents, tokens
 
 

@@ -10,7 +10,8 @@
 // by more than 1, and those logits that reach a bar: the count-th largest of its lanes' maxima,
 // which as many logits reach.  One comparison with the lower of the two finds what needs more
 // than its exponential.  merge_kernel joins a request's runs, takes the totals in 64 bits,
-// in which beams whose totals lie close compare as their logits say, and ranks them.
+// in which beams whose totals lie close compare as their logits say, and ranks them.  Where a
+// request's logits are few, whole_kernel does all of it.
 //   Exponentials are f32 (v_exp_f32 of differences, whose error shrinks with the term's weight),
 // sums of 16 bytes of logits f32, of a lane and beyond f64.
 //   512 rows of 128000 in f32, 262 MB: 55 us (4.8 TB/s) and 5.7 of joining; 80 rows of 151111 in
@@ -51,13 +52,18 @@ __device__ __forceinline__ float logit_of(uint64_t key) {
 }
 __device__ __forceinline__ uint32_t token_of(uint64_t key) { return 0xFFFFFFFFu - (uint32_t)key; }
 
+// A permutation that gives every lane a value, so that no old one need be kept for it.
+template <int kCtrl>
+__device__ __forceinline__ uint32_t permuted(uint32_t x) {
+  return (uint32_t)__builtin_amdgcn_mov_dpp((int)x, kCtrl, 0xf, 0xf, true);
+}
 // Lane i ^ kWith's value, by vector instructions alone (an LDS permutation takes ten times as long).
 template <int kWith>
 __device__ __forceinline__ uint32_t lane_xor(uint32_t x) {
-  if constexpr (kWith == 1) return dpp<0xB1>(x);                 // quad_perm 1 0 3 2
-  else if constexpr (kWith == 2) return dpp<0x4E>(x);            // quad_perm 2 3 0 1
-  else if constexpr (kWith == 4) return dpp<0x1B>(dpp<0x141>(x));  // row_half_mirror, quad_perm 3 2 1 0
-  else if constexpr (kWith == 8) return dpp<0x128>(x);           // row_ror 8
+  if constexpr (kWith == 1) return permuted<0xB1>(x);                 // quad_perm 1 0 3 2
+  else if constexpr (kWith == 2) return permuted<0x4E>(x);            // quad_perm 2 3 0 1
+  else if constexpr (kWith == 4) return permuted<0x1B>(permuted<0x141>(x));  // row_half_mirror, quad_perm 3 2 1 0
+  else if constexpr (kWith == 8) return permuted<0x128>(x);           // row_ror 8
   else if constexpr (kWith == 16) {
     const auto r = __builtin_amdgcn_permlane16_swap(x, x, false, false);
     return threadIdx.x & 16 ? r[0] : r[1];
@@ -78,9 +84,9 @@ template <int kWith>
 __device__ __forceinline__ double lane_xor(double v) {
   return __longlong_as_double((int64_t)lane_xor<kWith>((uint64_t)__double_as_longlong(v)));
 }
-// The lane before's; lane 0's own is undefined.
+// The lane before's; 0 in lane 0.
 __device__ __forceinline__ uint64_t lane_before(uint64_t v) {
-  return ((uint64_t)dpp<0x138>((uint32_t)(v >> 32)) << 32) | dpp<0x138>((uint32_t)v);  // wave_shr 1
+  return ((uint64_t)permuted<0x138>((uint32_t)(v >> 32)) << 32) | permuted<0x138>((uint32_t)v);  // wave_shr 1
 }
 __device__ __forceinline__ uint64_t lane_of(uint64_t v, int lane) {
   return ((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), lane) << 32) | (uint32_t)__builtin_amdgcn_readlane((int)v, lane);
@@ -115,9 +121,9 @@ struct Largest {
   int count;
   bool any;
 
-  __device__ explicit Largest(int n) : key(0), least(0), count(n), any(false) {}
+  __device__ __forceinline__ explicit Largest(int n) : key(0), least(0), count(n), any(false) {}
   // A key of each lane, or 0.  All lanes join.
-  __device__ void offer(uint64_t k) {
+  __device__ __forceinline__ void offer(uint64_t k) {
     uint64_t in = __ballot(k > least);
     if (!in) return;
     if (any && __popcll(in) <= 4) {
@@ -130,16 +136,24 @@ struct Largest {
         const uint64_t before = lane_before(key);
         key = lane < at ? key : lane == at ? one : before;
       } while (in);
+      bound();
     } else {
-      k = sorted(k > least ? k : 0);
-      if (any) {
-        // ascending, so that with the list it makes one bitonic sequence
-        k = lane_xor<32>(lane_xor<16>(((uint64_t)dpp<0x140>((uint32_t)(k >> 32)) << 32) | dpp<0x140>((uint32_t)k)));  // row_mirror
-        k = merged<32>(key > k ? key : k, true);
-      }
-      key = k;
-      any = true;
+      take(k > least ? k : 0);
     }
+  }
+  // The same however many enter.
+  __device__ __forceinline__ void take(uint64_t k) {
+    k = sorted(k);
+    if (any) {
+      // ascending, so that with the list it makes one bitonic sequence
+      k = lane_xor<32>(lane_xor<16>(((uint64_t)permuted<0x140>((uint32_t)(k >> 32)) << 32) | permuted<0x140>((uint32_t)k)));  // row_mirror
+      k = merged<32>(key > k ? key : k, true);
+    }
+    key = k;
+    any = true;
+    bound();
+  }
+  __device__ __forceinline__ void bound() {
     const uint64_t last = lane_of(key, count - 1);
     if (last > least) least = last;
   }
@@ -153,7 +167,7 @@ template <>
 struct Vec<float> {
   static constexpr int kN = 4;
   typedef float raw __attribute__((ext_vector_type(4), aligned(4)));
-  __device__ static void get(const raw &r, float *x) {
+  __device__ __forceinline__ static void get(const raw &r, float *x) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) x[i] = r[i];
   }
@@ -162,7 +176,7 @@ template <>
 struct Vec<__bf16> {
   static constexpr int kN = 8;
   typedef uint32_t raw __attribute__((ext_vector_type(4), aligned(2)));
-  __device__ static void get(const raw &r, float *x) {
+  __device__ __forceinline__ static void get(const raw &r, float *x) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) x[2 * i] = __uint_as_float(r[i] << 16), x[2 * i + 1] = __uint_as_float(r[i] & 0xFFFF0000u);
   }
@@ -204,12 +218,15 @@ struct SelectArgs {
 
 __device__ __forceinline__ bool ended(const SelectArgs &a, int64_t row) { return a.last && a.last[row] == a.stop; }
 
-constexpr int kBuffer = 128;
+// Keys that a wave may put down before they are sorted: those of one vector a lane beside 63.
+template <typename X>
+constexpr int kBuffer = 64 + 64 * Vec<X>::kN;
 
 // What a wave keeps of the logits that it has seen.  Those that may be among the largest are
 // put down in `buffer` and sorted 64 at a time, most often only once, with the other waves'
 // at the end: putting each in its place at once is a chain of some 15 instructions that
-// depend on each other (80 rows of 151111, the ten largest: 30 us, 22 now).
+// depend on each other (80 rows of 151111, the ten largest: 30 us, 22 now).  One place a vector
+// sorts them, not one a logit, so that the code stays within the instruction cache.
 struct Scan {
   Largest top;
   uint64_t *buffer;
@@ -219,52 +236,39 @@ struct Scan {
   float enter;       // ..: for that or to move the reference
   float lane_most;
 
-  __device__ Scan(int count, uint64_t *b)
+  __device__ __forceinline__ Scan(int count, uint64_t *b)
       : top(count), buffer(b), held(0), sum(0.), ref(-__FLT_MAX__), least(-__FLT_MAX__), enter(-__FLT_MAX__), lane_most(-__FLT_MAX__) {}
 
-  __device__ static void fence() {
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-  }
   // A logit of each lane.
-  __device__ void put(float x, uint32_t token) {
+  __device__ __forceinline__ void put(float x, uint32_t token) {
     const uint64_t k = x >= -__FLT_MAX__ ? key_of_logit(x, token) : 0, in = __ballot(k > top.least);
     if (!in) return;
     if (k > top.least) buffer[held + __builtin_amdgcn_mbcnt_hi((uint32_t)(in >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)in, 0))] = k;
     held += (int)__popcll(in);
-    if (held < 64) return;
-    const int lane = threadIdx.x & 63;
-    fence();
-    const uint64_t first = buffer[lane], then = buffer[64 + lane];
-    fence();
-    held -= 64;
-    if (lane < held) buffer[lane] = then;
-    fence();
-    top.offer(first);
   }
   // The reference follows the largest of the lanes' logits; the sums so far with it.
-  __device__ void follow(float most) {
+  __device__ __forceinline__ void follow(float most) {
     const float to = wave_max(most);
     if (!(to > ref + 1.f)) return;  // also where `to` is the lowest value, and NaN
     sum *= (double)__builtin_amdgcn_exp2f((ref - to) * kLog2e);
     ref = to;
   }
-  __device__ void bounds() {
+  __device__ __forceinline__ void bounds() {
     least = top.least ? logit_of(top.least + 1) : -__FLT_MAX__;  // the least logit of a larger key
     enter = fminf(least, ref + 1.f);
   }
   // The bar below which a logit need not enter: the count-th largest of the lanes' maxima so
   // far, which as many logits reach.  In the order of ordered().
-  __device__ uint32_t bar() const {
+  __device__ __forceinline__ uint32_t bar() const {
     return __builtin_amdgcn_readlane((int)sorted(ordered(lane_most >= -__FLT_MAX__ ? lane_most : -__FLT_MAX__)), top.count - 1);
   }
-  __device__ void raise(uint32_t to) {
+  __device__ __forceinline__ void raise(uint32_t to) {
     const uint64_t below = to > ordered(-__FLT_MAX__) ? ((uint64_t)to << 32) - 1 : 0;  // the key that all of it pass
     if (below > top.least) top.least = below;
     bounds();
   }
   template <int N>
-  __device__ static float most_of(const float *x) {
+  __device__ __forceinline__ static float most_of(const float *x) {
     float m = x[0];
 #pragma unroll
     for (int i = 1; i < N; ++i) m = fmaxf(m, x[i]);
@@ -273,12 +277,20 @@ struct Scan {
   // N logits of each lane, the largest of them `most`, tokens token .. token + N - 1; minus
   // infinity for none.
   template <int N>
-  __device__ void take(const float *x, float most, uint32_t token) {
+  __device__ __forceinline__ void take(const float *x, float most, uint32_t token) {
     if (__any(most >= enter)) {
       follow(most);
 #pragma unroll
       for (int i = 0; i < N; ++i)
         if (__any(x[i] >= least)) put(x[i], token + i);
+      if (held >= 64) {
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        do {
+          held -= 64;
+          top.take(buffer[held + (threadIdx.x & 63)]);
+        } while (held >= 64);
+      }
       bounds();
     }
     float s[N];
@@ -292,28 +304,31 @@ struct Scan {
   }
 };
 
+// Part `part` of `parts` of a row, read by one wave.
 template <typename X>
-__global__ __launch_bounds__(kScanThreads) void scan_kernel(SelectArgs a) {
-  constexpr int N = Vec<X>::kN, U = 4;
+struct Reader {
+  static constexpr int N = Vec<X>::kN, U = 4;
   typedef typename Vec<X>::raw raw;
-  __shared__ Run runs[kScanWaves];
-  __shared__ uint64_t buffers[kScanWaves][kBuffer];
-  __shared__ uint32_t bars[kScanWaves], helds[kScanWaves];
-  const int64_t row = blockIdx.x / (uint32_t)a.splits, split = blockIdx.x - row * a.splits, n = row / a.beams;
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  const X *const p = static_cast<const X *>(a.logits) + n * a.request + (row - n * a.beams) * a.beam;
-  const raw *const body = reinterpret_cast<const raw *>(p);
-  const int64_t vectors = a.vocab / N, rest = a.vocab - vectors * N, part = split * kScanWaves + wave, parts = (int64_t)a.splits * kScanWaves;
-  const int64_t to = vectors * (part + 1) / parts;
-  int64_t v = vectors * part / parts;
+  const X *row;
+  int64_t v, to;  // in vectors
+  int rest, held;
   raw next[U];
   float x[U][N], most[U];
-  auto fetch = [&](int64_t at) {
+  Scan scan;
+
+  __device__ __forceinline__ Reader(const X *p, int64_t vocab, int64_t part, int64_t parts, int count, uint64_t *buffer) : row(p), scan(count, buffer) {
+    const int64_t vectors = vocab / N;
+    v = vectors * part / parts, to = vectors * (part + 1) / parts;
+    rest = part == parts - 1 ? (int)(vocab - vectors * N) : 0;
+    if (v < to) fetch(v);
+  }
+  __device__ __forceinline__ void fetch(int64_t at) {
+    const raw *const body = reinterpret_cast<const raw *>(row);
 #pragma unroll
-    for (int u = 0; u < U; ++u) next[u] = body[min(at + 64 * u + lane, to - 1)];
-  };
-  Scan scan(a.count, buffers[wave]);
-  auto unpack = [&] {  // and what comes after it on its way
+    for (int u = 0; u < U; ++u) next[u] = body[min(at + 64 * u + (int)(threadIdx.x & 63), to - 1)];
+  }
+  __device__ __forceinline__ void unpack() {  // and what comes after it on its way
+    const int lane = threadIdx.x & 63;
 #pragma unroll
     for (int u = 0; u < U; ++u) Vec<X>::get(next[u], x[u]);
     if (v + 64 * U < to) {
@@ -329,61 +344,100 @@ __global__ __launch_bounds__(kScanThreads) void scan_kernel(SelectArgs a) {
       most[u] = Scan::most_of<N>(x[u]);
       scan.lane_most = fmaxf(scan.lane_most, most[u]);
     }
-  };
-  if (v < to) fetch(v);
-  if (ended(a, row) || !(fabsf(a.scores[row]) <= __FLT_MAX__)) return;  // its logits do not matter
-
-  // What is below one wave's bar need not enter any of the workgroup's lists.
-  uint32_t bar = 0;
-  if (v < to) {
+  }
+  // The bar of the first logits; of several waves' that read one row the highest serves all.
+  __device__ __forceinline__ uint32_t first() {
+    if (v >= to) return 0;
     unpack();
     scan.follow(scan.lane_most);
-    bar = scan.bar();
+    return scan.bar();
   }
+  // Everything, given that bar: what is large is in the buffer then, `held` keys.
+  __device__ __forceinline__ Run read(uint32_t bar) {
+    const int lane = threadIdx.x & 63;
+    scan.raise(bar);
+    const int64_t tail = to;
+    for (uint32_t turn = 1; v < to; ++turn) {
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (v + 64 * u < to) scan.take<N>(x[u], most[u], (uint32_t)((v + 64 * u + lane) * N));
+      v += 64 * U;
+      if (v >= to) break;
+      unpack();
+      if ((turn & (turn - 1)) == 0) scan.raise(scan.bar());  // at each doubling: what enters between two is about the same
+    }
+    if (rest) {
+      const int64_t at = tail * N + lane;
+      const float y = lane < rest ? (float)row[at] : -__builtin_inff();
+      scan.take<1>(&y, y, (uint32_t)at);
+    }
+    held = scan.held;
+    if (scan.top.any) {
+      if (lane < scan.top.count) scan.buffer[held + lane] = scan.top.key;
+      held += scan.top.count;
+    }
+    return {wave_sum(scan.sum), scan.ref};
+  }
+};
+
+// What `waves` waves (up to 16) have put down, joined by one.
+__device__ __forceinline__ Largest join(const uint64_t *buffers, int stride, const uint32_t *helds, int waves, int count) {
+  const int lane = threadIdx.x & 63;
+  Largest top(count);
+  const int mine = lane < waves ? (int)helds[lane] : 0;
+  int upto = mine;
+#pragma unroll
+  for (int off = 1; off < 16; off <<= 1) {
+    const int u = __shfl_up(upto, off);
+    if (lane >= off) upto += u;
+  }
+  const int start = upto - mine, total = __builtin_amdgcn_readlane(upto, 15);
+  for (int first = 0; first < total; first += 64) {
+    const int at = first + lane;
+    int of = 0, from = 0;
+    for (int i = 1; i < waves; ++i) {
+      const int next = __builtin_amdgcn_readlane(start, i);
+      if (at >= next) of = i, from = next;
+    }
+    top.offer(at < total ? buffers[of * stride + at - from] : 0);
+  }
+  return top;
+}
+
+// One run of those that the lanes hold; a lane without one has sum 0 and the lowest reference.
+__device__ __forceinline__ Run join(const Run &mine) {
+  const float ref = wave_max(mine.ref);
+  return {wave_sum(mine.sum * exp((double)mine.ref - (double)ref)), ref};
+}
+
+template <typename X>
+__device__ __forceinline__ const X *row_of(const SelectArgs &a, int64_t n, int64_t beam) {
+  return static_cast<const X *>(a.logits) + n * a.request + beam * a.beam;
+}
+// Whether a beam's logits matter.
+__device__ __forceinline__ bool goes_on(const SelectArgs &a, int64_t row) { return !ended(a, row) && fabsf(a.scores[row]) <= __FLT_MAX__; }
+
+// A workgroup a run of a row.
+template <typename X>
+__global__ __launch_bounds__(kScanThreads) void scan_kernel(SelectArgs a) {
+  __shared__ Run runs[kScanWaves];
+  __shared__ uint64_t buffers[kScanWaves][kBuffer<X>];
+  __shared__ uint32_t bars[kScanWaves], helds[kScanWaves];
+  const int64_t row = blockIdx.x / (uint32_t)a.splits, split = blockIdx.x - row * a.splits, n = row / a.beams;
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  Reader<X> reader(row_of<X>(a, n, row - n * a.beams), a.vocab, split * kScanWaves + wave, (int64_t)a.splits * kScanWaves, a.count, buffers[wave]);
+  if (!goes_on(a, row)) return;
+  uint32_t bar = reader.first();
   if (lane == 0) bars[wave] = bar;
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < kScanWaves; ++i) bar = max(bar, bars[i]);
-  scan.raise(bar);
-  for (uint32_t turn = 1; v < to; ++turn) {
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (v + 64 * u < to) scan.take<N>(x[u], most[u], (uint32_t)((v + 64 * u + lane) * N));
-    v += 64 * U;
-    if (v >= to) break;
-    unpack();
-    if ((turn & (turn - 1)) == 0) scan.raise(scan.bar());  // at each doubling: what enters between two is about the same
-  }
-  if (part == parts - 1 && rest) {
-    const int64_t at = vectors * N + lane;
-    const float y = lane < rest ? (float)p[at] : -__builtin_inff();
-    scan.take<1>(&y, y, (uint32_t)at);
-  }
-
-  const double sum = wave_sum(scan.sum);
-  if (scan.top.any && lane < a.count) buffers[wave][scan.held + lane] = scan.top.key;
-  if (lane == 0) runs[wave] = {sum, scan.ref}, helds[wave] = scan.held + (scan.top.any ? a.count : 0);
+  const Run run = reader.read(bar);
+  if (lane == 0) runs[wave] = run, helds[wave] = reader.held;
   __syncthreads();
   if (wave) return;
-  Largest top(a.count);
-  int total = 0, start[kScanWaves];
-#pragma unroll
-  for (int i = 0; i < kScanWaves; ++i) start[i] = total, total += helds[i];
-  for (int first = 0; first < total; first += 64) {
-    const int at = first + lane;
-    int of = 0, from = 0;
-#pragma unroll
-    for (int i = 1; i < kScanWaves; ++i)
-      if (at >= start[i]) of = i, from = start[i];
-    top.offer(at < total ? buffers[of][at - from] : 0);
-  }
-  Run all = runs[0];
-#pragma unroll
-  for (int i = 1; i < kScanWaves; ++i) all.ref = fmaxf(all.ref, runs[i].ref);
-  const double part_sum = lane < kScanWaves ? runs[lane].sum * exp((double)runs[lane].ref - (double)all.ref) : 0.;
-  all.sum = 0.;
-#pragma unroll
-  for (int i = 0; i < kScanWaves; ++i) all.sum += __longlong_as_double((int64_t)lane_of((uint64_t)__double_as_longlong(part_sum), i));
+  const Largest top = join(buffers[0], kBuffer<X>, helds, kScanWaves, a.count);
+  const Run all = join(lane < kScanWaves ? runs[lane] : Run{0., -__FLT_MAX__});
   if (lane == 0) a.runs[row * a.splits + split] = all;
   if (lane < a.count) a.keys[(row * a.splits + split) * a.count + lane] = top.key;
 }
@@ -401,20 +455,76 @@ __device__ __forceinline__ double total_of(uint64_t u) {
   return __longlong_as_double((int64_t)(u >> 63 ? u ^ 0x8000000000000000ull : ~u));
 }
 
-// A workgroup a request: a wave joins a beam's runs at a time, then every candidate counts
-// those over it: of its own beam the ones before it, of a lower beam those of no smaller
-// total, of a higher one those of a larger.
+// A request's candidates in LDS, [beams, count] and each beam's sorted.
+struct Found {
+  Candidate *all;
+  int *ranks, *have;
+
+  __device__ __forceinline__ Found(Candidate *lds, const SelectArgs &a) : all(lds), ranks(reinterpret_cast<int *>(lds + a.beams * a.count)), have(ranks + a.beams * a.count) {}
+  // Beam b's, by one wave: `top` and `run` of its logits, which do not matter if it has ended.
+  __device__ __forceinline__ void put(const SelectArgs &a, int64_t row, int b, const Largest &top, const Run &run) {
+    const int lane = threadIdx.x & 63;
+    const float score = a.scores[row];
+    Candidate mine{0, -1};
+    if (!(fabsf(score) <= __FLT_MAX__)) {
+    } else if (ended(a, row)) {
+      if (lane == 0) mine = {ordered64(score), a.stop};
+    } else if (run.sum > 0. && run.sum <= __DBL_MAX__ && top.key) {
+      mine = {ordered64((double)score + (((double)logit_of(top.key) - (double)run.ref) - log(run.sum))), (int64_t)token_of(top.key)};
+    }
+    if (lane < a.count) {
+      all[b * a.count + lane] = mine;
+      ranks[b * a.count + lane] = lane;
+    }
+    const uint64_t some = __ballot(lane < a.count && mine.total);
+    if (lane == 0 && some) atomicAdd(have, (int)__popcll(some));
+  }
+  // The whole workgroup: every candidate counts those over it, of its own beam the ones before
+  // it, of a lower beam those of no smaller total, of a higher one those of a larger.
+  __device__ __forceinline__ void rank(const SelectArgs &a, int64_t n) {
+    const int total = a.beams * a.count;
+    for (int i = threadIdx.x; i < total * a.beams; i += blockDim.x) {  // a candidate, another beam
+      const int b = i / total, c = i - b * total, of = c / a.count;
+      const uint64_t mine = all[c].total;
+      if (!mine || b == of) continue;
+      int lo = 0, hi = a.count;  // how many of beam b's are over it
+      while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        const uint64_t t = all[b * a.count + mid].total;
+        if (t > mine || (b < of && t == mine)) lo = mid + 1;
+        else hi = mid;
+      }
+      if (lo) atomicAdd(ranks + c, lo);
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < total; i += blockDim.x) {
+      const Candidate mine = all[i];
+      if (!mine.total || ranks[i] >= a.count) continue;
+      const int64_t to = n * a.count + ranks[i];
+      a.out_scores[to] = (float)total_of(mine.total);
+      a.parents[to] = i / a.count;
+      a.tokens[to] = mine.token;
+    }
+    for (int i = *have + threadIdx.x; i < a.count; i += blockDim.x) {
+      const int64_t to = n * a.count + i;
+      a.out_scores[to] = -__builtin_inff();
+      a.parents[to] = 0;
+      a.tokens[to] = -1;
+    }
+  }
+};
+size_t found_bytes(int beams, int count) { return (sizeof(Candidate) + sizeof(int)) * beams * count + sizeof(int); }
+
+// A workgroup a request: a wave joins a beam's runs at a time.
 __global__ __launch_bounds__(kMergeThreads) void merge_kernel(SelectArgs a) {
-  extern __shared__ Candidate found[];  // [beams, count], each beam's sorted; then their ranks
-  int *const ranks = reinterpret_cast<int *>(found + a.beams * a.count);
-  __shared__ int have;
+  extern __shared__ Candidate lds[];
+  Found found(lds, a);
   const int64_t n = blockIdx.x;
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  if (threadIdx.x == 0) have = 0;
+  if (threadIdx.x == 0) *found.have = 0;
   __syncthreads();
   for (int b = wave; b < a.beams; b += kMergeWaves) {
     const int64_t row = n * a.beams + b;
-    const float score = a.scores[row];
     const uint64_t *const keys = a.keys + row * a.splits * a.count;
     auto key_at = [&](int at) -> uint64_t {  // the runs' largest first, then their second ones, ..: what comes later seldom enters
       const int rank = at / a.splits;
@@ -423,56 +533,54 @@ __global__ __launch_bounds__(kMergeThreads) void merge_kernel(SelectArgs a) {
     const uint64_t first_key = key_at(lane);
     Run run{0., -__FLT_MAX__};
     if (lane < a.splits) run = a.runs[row * a.splits + lane];
-    Candidate mine{0, -1};
-    if (!(fabsf(score) <= __FLT_MAX__)) {
-    } else if (ended(a, row)) {
-      if (lane == 0) mine = {ordered64(score), a.stop};
-    } else {
-      Largest top(a.count);
+    Largest top(a.count);
+    if (goes_on(a, row)) {
       top.offer(first_key);
       for (int first = 64; first < a.splits * a.count; first += 64) top.offer(key_at(first + lane));
-      const float ref = wave_max(run.ref);
-      const double sum = wave_sum(run.sum * exp((double)run.ref - (double)ref));
-      if (sum > 0. && sum <= __DBL_MAX__ && top.key)
-        mine = {ordered64((double)score + (((double)logit_of(top.key) - (double)ref) - log(sum))), (int64_t)token_of(top.key)};
+      run = join(run);
     }
-    if (lane < a.count) {
-      found[b * a.count + lane] = mine;
-      ranks[b * a.count + lane] = lane;
-    }
-    const uint64_t some = __ballot(lane < a.count && mine.total);
-    if (lane == 0 && some) atomicAdd(&have, (int)__popcll(some));
+    found.put(a, row, b, top, run);
   }
   __syncthreads();
-  const int all = a.beams * a.count;
-  for (int i = threadIdx.x; i < all * a.beams; i += kMergeThreads) {  // a candidate, another beam
-    const int b = i / all, c = i - b * all, of = c / a.count;
-    const uint64_t total = found[c].total;
-    if (!total || b == of) continue;
-    int lo = 0, hi = a.count;  // how many of beam b's are over it
-    while (lo < hi) {
-      const int mid = (lo + hi) >> 1;
-      const uint64_t t = found[b * a.count + mid].total;
-      if (t > total || (b < of && t == total)) lo = mid + 1;
-      else hi = mid;
-    }
-    if (lo) atomicAdd(ranks + c, lo);
+  found.rank(a, n);
+}
+
+// A workgroup a request that does all of it, `each` waves a beam.
+constexpr int kWholeThreads = 512, kWholeWaves = kWholeThreads / 64;
+template <typename X>
+__global__ __launch_bounds__(kWholeThreads) void whole_kernel(SelectArgs a, int each) {
+  extern __shared__ Candidate lds[];
+  __shared__ Run runs[kWholeWaves];
+  __shared__ uint64_t buffers[kWholeWaves][kBuffer<X>];
+  __shared__ uint32_t bars[kWholeWaves], helds[kWholeWaves];
+  Found found(lds, a);
+  const int64_t n = blockIdx.x;
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, b = wave / each, part = wave - b * each;
+  const int64_t row = n * a.beams + b;
+  const bool is = b < a.beams, reads = is && goes_on(a, row);
+  if (threadIdx.x == 0) *found.have = 0;
+  Reader<X> reader(row_of<X>(a, n, is ? b : 0), reads ? a.vocab : 0, part, each, a.count, buffers[wave]);
+  uint32_t bar = reader.first();
+  if (lane == 0) bars[wave] = bar;
+  __syncthreads();
+  if (reads) {
+    for (int i = 0; i < each; ++i) bar = max(bar, bars[wave - part + i]);
+    const Run run = reader.read(bar);
+    if (lane == 0) runs[wave] = run, helds[wave] = reader.held;
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < all; i += kMergeThreads) {
-    const Candidate mine = found[i];
-    if (!mine.total || ranks[i] >= a.count) continue;
-    const int64_t to = n * a.count + ranks[i];
-    a.out_scores[to] = (float)total_of(mine.total);
-    a.parents[to] = i / a.count;
-    a.tokens[to] = mine.token;
+  if (is && part == 0) {
+    Largest top(a.count);
+    Run run{0., -__FLT_MAX__};
+    if (reads) {
+      top = join(buffers[wave], kBuffer<X>, helds + wave, each, a.count);
+      if (lane < each) run = runs[wave + lane];
+      run = join(run);
+    }
+    found.put(a, row, b, top, run);
   }
-  for (int i = have + threadIdx.x; i < a.count; i += kMergeThreads) {
-    const int64_t to = n * a.count + i;
-    a.out_scores[to] = -__builtin_inff();
-    a.parents[to] = 0;
-    a.tokens[to] = -1;
-  }
+  __syncthreads();
+  found.rank(a, n);
 }
 
 // ------------------------------------------------------------------ reordering
@@ -636,11 +744,19 @@ int invalid(const char *msg) { return set_error(MQ_E_INVALID, msg); }
 bool aligned_to(const void *p, uintptr_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0; }
 
 // Runs of a row: workgroups for four on each of 256 CUs, none of fewer than 4096 logits (16 a
-// thread), 64 at most (a lane each when they are joined).  512 rows of 128000 in f32: 58 us,
+// thread), 64 at most (a lane each when they are joined).  512 rows of 128000 in f32: 57 us,
 // 64 with 2048 workgroups, 76 with 512; 80 rows of 151111 in bf16: 22.5, 24 and 26.
 int splits_of(int64_t rows, int64_t vocab) {
   const int64_t want = (1024 + rows - 1) / rows, most = vocab / 4096, s = want < most ? want : most;
   return (int)(s < 1 ? 1 : s > 64 ? 64 : s);
+}
+
+// Whether a workgroup a request reads all its logits, which spares a launch and the scratch:
+// where they are 128 KB at most and neither waves nor CUs lack.  1 to 64 requests of 4 beams
+// over 1000 to 4000 tokens in f32 12 us against 16, over 8000 15 against 16, over 16000 20
+// against 16; 300 requests over 4000 23 against 17; 12 beams over 2000 23 against 16.
+bool takes_whole(int64_t requests, int beams, int64_t vocab, int dtype) {
+  return beams <= kWholeWaves && requests <= 128 && vocab <= (128 << 10) / (beams * (dtype == MQ_F32 ? 4 : 2));
 }
 
 const char *select_fault(int64_t n, int beams, int64_t vocab, int count) {
@@ -653,10 +769,11 @@ const char *select_fault(int64_t n, int beams, int64_t vocab, int count) {
 }  // namespace
 }  // namespace mq
 
-extern "C" size_t mq_beam_select_scratch_size(int64_t requests, int beams, int64_t vocab, int count) {
+extern "C" size_t mq_beam_select_scratch_size(int64_t requests, int beams, int64_t vocab, int count, int dtype) {
   using namespace mq;
-  if (requests == 0 || select_fault(requests, beams, vocab, count)) return 0;
+  if (requests == 0 || select_fault(requests, beams, vocab, count) || (dtype != MQ_F32 && dtype != MQ_BF16)) return 0;
   const int64_t rows = requests * beams;
+  if (takes_whole(requests, beams, vocab, dtype)) return 0;
   return (size_t)rows * splits_of(rows, vocab) * (sizeof(Run) + 8 * (size_t)count);
 }
 
@@ -670,22 +787,30 @@ extern "C" int mq_beam_select(const void *logits, int dtype, int64_t requests, i
   if (requests == 0) return MQ_OK;
   for (int64_t s : {request_stride, beam_stride})
     if (s < 0 || s >= (int64_t(1) << 40)) return invalid("mq_beam_select: strides outside 0 .. 2^40");
-  if (!logits || !scores || !out_scores || !parents || !tokens || !scratch) return invalid("mq_beam_select: NULL pointer");
-  if (scratch_bytes < mq_beam_select_scratch_size(requests, beams, vocab, count)) return invalid("mq_beam_select: too little scratch");
+  const size_t need = mq_beam_select_scratch_size(requests, beams, vocab, count, dtype);
+  if (!logits || !scores || !out_scores || !parents || !tokens || (need && !scratch)) return invalid("mq_beam_select: NULL pointer");
+  if (scratch_bytes < need) return invalid("mq_beam_select: too little scratch");
   if (!aligned_to(logits, dtype == MQ_F32 ? 4 : 2) || !aligned_to(scores, 4) || !aligned_to(out_scores, 4) || !aligned_to(parents, 4) ||
       !aligned_to(last, 8) || !aligned_to(tokens, 8) || !aligned_to(scratch, 16))
     return invalid("mq_beam_select: misaligned buffer");
   const int64_t rows = requests * beams;
-  const int splits = splits_of(rows, vocab);
-  if (rows * splits >= (int64_t(1) << 24)) return invalid("mq_beam_select: too many requests");
+  const int splits = need ? splits_of(rows, vocab) : 1;
+  if (rows * splits >= (int64_t(1) << 24) || requests >= (int64_t(1) << 22)) return invalid("mq_beam_select: too many requests");
   Run *const runs = static_cast<Run *>(scratch);
   const SelectArgs a{logits, request_stride, beam_stride, vocab, requests, scores, last, stop, beams, count, splits, runs,
                      reinterpret_cast<uint64_t *>(runs + rows * splits), out_scores, parents, tokens};
   const hipStream_t s = static_cast<hipStream_t>(stream);
-  const dim3 grid((unsigned)(rows * splits));
-  if (dtype == MQ_F32) hipLaunchKernelGGL(scan_kernel<float>, grid, dim3(kScanThreads), 0, s, a);
-  else hipLaunchKernelGGL(scan_kernel<__bf16>, grid, dim3(kScanThreads), 0, s, a);
-  hipLaunchKernelGGL(merge_kernel, dim3((unsigned)requests), dim3(kMergeThreads), (sizeof(Candidate) + sizeof(int)) * beams * count, s, a);
+  const size_t lds = found_bytes(beams, count);
+  auto launch = [&]<typename X>() {
+    if (need) {
+      hipLaunchKernelGGL(scan_kernel<X>, dim3((unsigned)(rows * splits)), dim3(kScanThreads), 0, s, a);
+      hipLaunchKernelGGL(merge_kernel, dim3((unsigned)requests), dim3(kMergeThreads), lds, s, a);
+    } else {
+      hipLaunchKernelGGL(whole_kernel<X>, dim3((unsigned)requests), dim3(kWholeThreads), lds, s, a, kWholeWaves / beams);
+    }
+  };
+  if (dtype == MQ_F32) launch.operator()<float>();
+  else launch.operator()<__bf16>();
   const hipError_t e = hipGetLastError();
   return e == hipSuccess ? MQ_OK : set_error(MQ_E_HIP, hipGetErrorString(e));
 }

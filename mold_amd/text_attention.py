@@ -137,8 +137,8 @@ def rotate_heads(q, k, positions, inv_freq, q_weight=None, k_weight=None, eps: f
     positions, inv_freq, q_weight, k_weight = _rotation("rotate_heads", q, k, k, positions, inv_freq, q_weight, k_weight, device, n, dim)
     q, qt, qh = _head_rows("rotate_heads: q", q, (n, heads, dim), dtype, device)
     k, kt, kh = _head_rows("rotate_heads: k, as q,", k, (n, kv_heads, dim), dtype, device)
-    q_out = torch.empty((n, heads, dim), dtype=_BF16, device=device)
-    k_out = torch.empty((n, kv_heads, dim), dtype=_BF16, device=device)
+    q_out = q.new_empty((n, heads, dim), dtype=_BF16)
+    k_out = q.new_empty((n, kv_heads, dim), dtype=_BF16)
     if n:
         _run_on(device, _lib.load().mq_rotate_heads, q.data_ptr(), qt, qh, heads, k.data_ptr(), kt, kh, kv_heads, _dtype_code(dtype),
                 dim, n, positions.data_ptr(), inv_freq.data_ptr(), _address(q_weight), _address(k_weight), eps, q_out.data_ptr(),
@@ -343,8 +343,8 @@ class KvCache:
         q, qt, qh = _head_rows("KvCache.append_rotated: q", q, (n, heads, dim), dtype, device)
         k, kt, kh = _head_rows("KvCache.append_rotated: k, as q,", k, shape, dtype, device)
         v, vt, vh = _head_rows("KvCache.append_rotated: v, as q,", v, shape, dtype, device)
-        q_out = torch.empty((n, heads, dim), dtype=_BF16, device=device)
-        k_out = torch.empty(shape, dtype=_BF16, device=device) if keys else None
+        q_out = q.new_empty((n, heads, dim), dtype=_BF16)
+        k_out = q.new_empty(shape, dtype=_BF16) if keys else None
         if n:
             self._run(_lib.load().mq_kv_cache_append_rotated, self._ref, slots.data_ptr(), q.data_ptr(), qt, qh, heads, k.data_ptr(), kt,
                       kh, v.data_ptr(), vt, vh, _dtype_code(dtype), n, positions.data_ptr(), inv_freq.data_ptr(), _address(q_weight),
@@ -368,11 +368,9 @@ class KvCache:
         if tokens < 0 or width < 0 or not 1 <= beams <= _lib.MQ_MAX_BEAMS or not 0 <= room < 1 << 31:
             raise ValueError(f"KvCache.place: {tokens} tokens, {width} pages, {beams} beams, room for {room}")
         n, device = counts.shape[0], self.device
-        table = torch.empty((n * beams, width), dtype=torch.int32, device=device)
-        slots = torch.empty(tokens, dtype=torch.int64, device=device)
-        positions = torch.empty(tokens, dtype=torch.int64, device=device)
-        lengths = torch.empty(n * beams, dtype=torch.int32, device=device)
-        last = torch.empty(n, dtype=torch.int64, device=device)
+        table, lengths = counts.new_empty((n * beams, width)), counts.new_empty(n * beams)
+        slots, last = counts.new_empty(tokens, dtype=torch.int64), counts.new_empty(n, dtype=torch.int64)
+        positions = torch.empty_like(slots)
         _run_on(device, _lib.load().mq_cache_place, self._ref, counts.data_ptr(), n, beams, room, pages_at, page_count, table.data_ptr(), width, width,
                 tokens, slots.data_ptr(), positions.data_ptr(), lengths.data_ptr(), last.data_ptr())
         return Placed(table, slots, positions, lengths, last)
@@ -398,9 +396,8 @@ class KvCache:
         width = page_table.shape[1]
         if n > 1 and page_table.stride(0) < width or width > 1 and page_table.stride(1) != 1:
             page_table = page_table.contiguous()
-        slots = torch.empty(tokens, dtype=torch.int64, device=device)
-        positions = torch.empty(tokens, dtype=torch.int64, device=device)
-        lengths = torch.empty(n, dtype=torch.int32, device=device)
+        slots, lengths = held.new_empty(tokens, dtype=torch.int64), torch.empty_like(held)
+        positions = torch.empty_like(slots)
         _run_on(device, _lib.load().mq_cache_extend, self._ref, held.data_ptr(), _address(counts), n, page_table.data_ptr(),
                 page_table.stride(0) if n > 1 else width, width, tokens, slots.data_ptr(), positions.data_ptr(), lengths.data_ptr())
         return slots, positions, lengths

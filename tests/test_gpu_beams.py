@@ -79,7 +79,7 @@ def test_select(vocab, dtype):
 
 @gpu
 def test_many_beams():
-    for n, beams, count, vocab in [(1, 64, 64, 500), (2, 64, 1, 3), (3, 17, 33, 5000), (1, 64, 64, 1)]:
+    for n, beams, count, vocab in [(1, 64, 64, 500), (2, 64, 1, 3), (3, 17, 33, 5000), (1, 64, 64, 1), (2, 8, 64, 4096), (2, 8, 64, 4097), (2, 7, 12, 900), (129, 2, 3, 40)]:
         logits, scores = _logits(n, beams, vocab, seed=9)
         _check(logits, scores, count)
 
@@ -138,8 +138,9 @@ def test_masks_and_what_is_not_a_number(dtype):
 
 
 @gpu
-def test_stopped_beams():
-    logits, scores = _logits(6, 4, 5000, seed=5)
+@pytest.mark.parametrize("vocab", [5000, 20001])
+def test_stopped_beams(vocab):
+    logits, scores = _logits(6, 4, vocab, seed=5)
     scores[5] = -0.01
     last = torch.full((6, 4), 3, device="cuda")
     last[1, 2] = last[2, :3] = last[3] = last[4, 0] = last[5, 1] = 11
@@ -411,11 +412,12 @@ def test_reorder_refusals():
 
 
 @gpu
-def test_captured():
+@pytest.mark.parametrize("vocab", [3001, 40001])
+def test_captured(vocab):
     """A step's selection and reordering, replayed: each replay goes on from the one before."""
     rng = random.Random(4)
     table, pages = _tables(2, 4, 3, [40, 40], 32, rng)
-    logits, scores = _logits(2, 4, 3001, seed=3)
+    logits, scores = _logits(2, 4, vocab, seed=3)
     lengths = torch.full((8,), 40, dtype=torch.int32, device="cuda")
     graphed, eager = (_states(2, pages, 2, 64, 32, GgmlDType.Q8_0) for _ in range(2))
     a, b = (torch.tensor(table, dtype=torch.int32, device="cuda") for _ in range(2))
@@ -431,7 +433,7 @@ def test_captured():
     torch.cuda.current_stream().wait_stream(s)
     sb.reorder(b, lengths, select_beams(logits, scores)[1])
     for i in range(4):
-        x = _logits(2, 4, 3001, seed=20 + i)
+        x = _logits(2, 4, vocab, seed=20 + i)
         logits.copy_(x[0]), scores.copy_(x[1])
         want = select_beams(logits, scores)
         sb.reorder(b, lengths, want[1])
@@ -445,13 +447,14 @@ def test_captured():
 def test_refusals_of_the_library():
     """On the CPU: every fault is found before anything is launched."""
     lib, a, bad = _lib.load(), 4096, _lib.MQ_E_INVALID
-    need = lib.mq_beam_select_scratch_size(3, 4, 1000, 4)
-    assert need > 0 and lib.mq_beam_select_scratch_size(0, 4, 1000, 4) == 0
-    for args in ((-1, 4, 1000, 4), (3, 0, 1000, 4), (3, 65, 1000, 4), (3, 4, 0, 4), (3, 4, 1 << 31, 4), (3, 4, 1000, 0), (3, 4, 1000, 65), ((1 << 20) + 1, 4, 1000, 4)):
-        assert lib.mq_beam_select_scratch_size(*args) == 0, args
-    ok = dict(logits=a, dtype=0, n=3, beams=4, vocab=1000, rs=4000, bs=1000, scores=a, last=a, stop=7, count=4, totals=a, parents=a, tokens=a, scratch=a, size=need, stream=None)
+    need = lib.mq_beam_select_scratch_size(3, 4, 100000, 4, 0)
+    assert need > 0 and lib.mq_beam_select_scratch_size(0, 4, 100000, 4, 0) == 0 and lib.mq_beam_select_scratch_size(3, 4, 1000, 4, 30) == 0
+    for args in ((-1, 4, 100000, 4), (3, 0, 100000, 4), (3, 65, 100000, 4), (3, 4, 0, 4), (3, 4, 1 << 31, 4), (3, 4, 100000, 0), (3, 4, 100000, 65), ((1 << 20) + 1, 4, 100000, 4)):
+        assert lib.mq_beam_select_scratch_size(*args, 0) == 0, args
+    assert lib.mq_beam_select_scratch_size(3, 4, 100000, 4, 1) == 0
+    ok = dict(logits=a, dtype=0, n=3, beams=4, vocab=100000, rs=400000, bs=100000, scores=a, last=a, stop=7, count=4, totals=a, parents=a, tokens=a, scratch=a, size=need, stream=None)
     for change in (dict(logits=None), dict(dtype=1), dict(n=-1), dict(n=(1 << 20) + 1), dict(beams=0), dict(beams=65), dict(vocab=0), dict(vocab=1 << 31), dict(rs=-1),
-                   dict(bs=1 << 40), dict(scores=None), dict(stop=-1), dict(stop=1000), dict(count=0), dict(count=65), dict(totals=None), dict(parents=None),
+                   dict(bs=1 << 40), dict(scores=None), dict(stop=-1), dict(stop=100000), dict(count=0), dict(count=65), dict(totals=None), dict(parents=None),
                    dict(tokens=None), dict(scratch=None), dict(size=need - 1), dict(logits=a + 2), dict(logits=a + 1, dtype=30), dict(scores=a + 2), dict(last=a + 4),
                    dict(totals=a + 1), dict(parents=a + 2), dict(tokens=a + 4), dict(scratch=a + 8), dict(n=1 << 20, beams=64, size=1 << 60)):
         assert lib.mq_beam_select(*{**ok, **change}.values()) == bad, change
