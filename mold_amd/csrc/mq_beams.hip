@@ -27,7 +27,7 @@
 // 64 x 8 beams in BF16, 28 layers, 1585 MB read and written: 300 us (5.3 TB/s) and 4.8 of
 // planning; 8 x 4 beams in Q8_0, 51 MB: 11.6 and 4.1.
 #include "../../include/moldq.h"
-#include "mq_cache_write.h"
+#include "mq_cache.h"
 
 namespace mq {
 int set_error(int code, const char *msg);
@@ -832,7 +832,7 @@ extern "C" int mq_beam_reorder(const mq_kv_cache *caches, int count, int32_t *ta
     if (caches[i].dtype != caches[0].dtype || caches[i].pages != caches[0].pages || caches[i].kv_heads != caches[0].kv_heads ||
         caches[i].head_dim != caches[0].head_dim || caches[i].page_tokens != caches[0].page_tokens)
       return invalid("mq_beam_reorder: the caches of a model's layers are alike");
-    if ((caches[i].pages && !caches[i].data) || !aligned16(caches[i].data)) return invalid("mq_beam_reorder: a cache's data is NULL or misaligned");
+    if ((caches[i].pages && !caches[i].data) || !aligned_to(caches[i].data, 16)) return invalid("mq_beam_reorder: a cache's data is NULL or misaligned");
     list.data[i] = static_cast<uint8_t *>(caches[i].data);
   }
   if (requests < 0 || requests > (int64_t(1) << 20) || beams < 1 || beams > MQ_MAX_BEAMS) return invalid("mq_beam_reorder: 0 to 2^20 requests, 1 to 64 beams");

@@ -16,7 +16,7 @@
 // 24 prompts (7305 tokens) take 6.0 us, 256 with four beams (163 000 tokens, 38 000 table
 // entries) 6.7, one token each of 200 sequences 3.5, of which a launch of nothing is 2.
 #include "../../include/moldq.h"
-#include "mq_cache_write.h"
+#include "mq_cache.h"
 
 namespace mq {
 int set_error(int code, const char *msg);
