@@ -14,9 +14,10 @@
 // request's logits are few, whole_kernel does all of it.
 //   Exponentials are f32 (v_exp_f32 of differences, whose error shrinks with the term's weight),
 // sums of 16 bytes of logits f32, of a lane and beyond f64.
-//   512 rows of 128000 in f32, 262 MB: 55 us (4.8 TB/s) and 5.7 of joining; 80 rows of 151111 in
-// bf16: 17 and 5.0, of which vector instructions (1100 a wave, four waves a SIMD) are 8; one
-// request of 4 x 32000: 7.8 and 4.0, chains of dependent instructions behind one load.
+//   512 rows of 128000 in f32, a fifth of them of ended beams, 210 MB: 52 us and 5.6 of joining;
+// 80 rows of 151111 in bf16: 17 and 5.1, of which vector instructions (992 a wave, four waves a
+// SIMD) are 8; one request of 4 x 32000: 7.8 and 4.2, chains of dependent instructions behind one
+// load.
 //
 // mq_beam_reorder: beam j of a request goes on from beam parents[j].  Whole pages are shared: a
 // row of the page table takes its parent's entries.  The last, partial page goes to one child
@@ -38,6 +39,10 @@ namespace {
 
 constexpr int kScanThreads = 256, kScanWaves = kScanThreads / 64;
 constexpr int kMergeThreads = 512, kMergeWaves = kMergeThreads / 64;
+
+// The wave's place in its workgroup, in a scalar register, so that what follows from it is not
+// computed in every lane.
+__device__ __forceinline__ int wave_index() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
 
 // A logit and its token as one key: larger logits first, of equal ones the lower token.  0 is
 // none.  Adding 0 makes the two zeros one.
@@ -424,7 +429,7 @@ __global__ __launch_bounds__(kScanThreads) void scan_kernel(SelectArgs a) {
   __shared__ uint64_t buffers[kScanWaves][kBuffer<X>];
   __shared__ uint32_t bars[kScanWaves], helds[kScanWaves];
   const int64_t row = blockIdx.x / (uint32_t)a.splits, split = blockIdx.x - row * a.splits, n = row / a.beams;
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int wave = wave_index(), lane = threadIdx.x & 63;
   Reader<X> reader(row_of<X>(a, n, row - n * a.beams), a.vocab, split * kScanWaves + wave, (int64_t)a.splits * kScanWaves, a.count, buffers[wave]);
   if (!goes_on(a, row)) return;
   uint32_t bar = reader.first();
@@ -520,7 +525,7 @@ __global__ __launch_bounds__(kMergeThreads) void merge_kernel(SelectArgs a) {
   extern __shared__ Candidate lds[];
   Found found(lds, a);
   const int64_t n = blockIdx.x;
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int wave = wave_index(), lane = threadIdx.x & 63;
   if (threadIdx.x == 0) *found.have = 0;
   __syncthreads();
   for (int b = wave; b < a.beams; b += kMergeWaves) {
@@ -555,7 +560,7 @@ __global__ __launch_bounds__(kWholeThreads) void whole_kernel(SelectArgs a, int 
   __shared__ uint32_t bars[kWholeWaves], helds[kWholeWaves];
   Found found(lds, a);
   const int64_t n = blockIdx.x;
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, b = wave / each, part = wave - b * each;
+  const int wave = wave_index(), lane = threadIdx.x & 63, b = wave / each, part = wave - b * each;
   const int64_t row = n * a.beams + b;
   const bool is = b < a.beams, reads = is && goes_on(a, row);
   if (threadIdx.x == 0) *found.have = 0;
@@ -693,7 +698,7 @@ __global__ __launch_bounds__(kCopyThreads) void copy_kernel(Plan plan, int reque
   constexpr int kUnits = CacheTile<T, D>::kBytes / 16, kPer = kMaxRequests / kCopyThreads, U = (kUnits + kCopyThreads - 1) / kCopyThreads;
   __shared__ uint32_t before[kMaxRequests], sums[kCopyThreads / 64];
   u32x4 *const data = reinterpret_cast<u32x4 *>(plan.caches->data[blockIdx.y]);
-  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+  const int tid = threadIdx.x, wave = wave_index(), lane = tid & 63;
   uint32_t mine[kPer], sum = 0;  // the tiles, of one head, of the requests before
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {

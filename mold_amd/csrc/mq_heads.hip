@@ -6,22 +6,24 @@
 //   out_i = y_i cos a_i - y_(i+D/2) sin a_i,   out_(i+D/2) = y_(i+D/2) cos a_i + y_i sin a_i
 //
 // in f32, rounded once to bf16.  The angle is taken in 64 bits as turns, of which the whole
-// ones are dropped, so that far positions lose nothing; v_sin_f32 and v_cos_f32 take turns
-// and are at most 2^-22.9 off over a whole one.
+// ones are dropped, so that far positions lose nothing, and its sine and cosine are
+// correct to f32's rounding: with v_sin_f32 and v_cos_f32, 2^-22.9 off, 4100 tokens took
+// half a microsecond less, but half again as many results rounded to a neighbour of the right one.
 //
 // A value is read and written once; the bound is HBM, the launch for a step's few tokens.
 // D / 8 lanes hold a head, each four values of its lower half and the four that they are
 // rotated with, so that only the sum of squares crosses lanes, and a wave takes four heads
 // of 128 (eight of 64) of one token at a time.  A lane's four angles serve all heads of the
 // token that the wave takes: one pass of heads while tokens are few, the more the more waves
-// there are to fill the chip anyway.  4100 tokens of 16 / 8 heads of 128 in bf16, 50 MB: 14.1 us;
-// with twice the waves 17, with passes loaded four at a time 15.5.  7305 tokens of 20 / 20 heads
-// of 64 from f32, 112 MB: 19 us (5.8 TB/s, part of it from the caches).
+// there are to fill the chip anyway.  4100 tokens of 16 / 8 heads of 128 in bf16, 50 MB: 10.5 us;
+// 14.1 with the wave's place in a vector register, which had every lane compute addresses and
+// conditions.  7305 tokens of 20 / 20 heads of 64 from f32, 112 MB: 20 us (5.6 TB/s, part of it from
+// the caches).
 //
 // Into the cache, a workgroup of 2 D threads takes 32 tokens of one k head through LDS
 // (as bf16, what the attention of the prompt itself reads) into the shape in which
 // mq_cache_write.h stores tiles; workgroups of v's and of q's share the launch.  32768
-// tokens of 32 / 8 heads of 128 from bf16 into Q8_0, 809 MB read and written: 160 us (5.1 TB/s),
+// tokens of 32 / 8 heads of 128 from bf16 into Q8_0, 809 MB read and written: 157 us (5.15 TB/s),
 // 175 with all of q's workgroups behind the writing ones, whose vector work is half of the time.
 #include "../../include/moldq.h"
 #include "mq_cache_write.h"
@@ -35,7 +37,7 @@ namespace {
 
 struct HeadRows {
   const void *x;
-  int64_t token, head;  // strides in elements
+  uint32_t token, head;  // strides in elements
   int heads;
   const float *weight;  // NULL: no norm
   __bf16 *out;          // contiguous [tokens, heads, D]; NULL: not wanted
@@ -49,6 +51,10 @@ struct HeadArgs {
   int64_t tokens;
   int parts, passes;  // waves of a token, and of how many passes each
 };
+
+// The wave's place in its workgroup, in a scalar register, so that what follows from it is not
+// computed in every lane.
+__device__ __forceinline__ uint32_t wave_index() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
 
 // What one lane holds of a head.
 template <typename X>
@@ -98,13 +104,27 @@ struct Turns {
 #pragma unroll
     for (int i = 0; i < 4; ++i) freq[i] = (double)v[i] * 0.15915494309189535;  // 1 / (2 pi)
   }
+  // Of a = n / 4 + r turns, n the nearest whole number: sine and cosine of 2 pi r by their series
+  // (what is left out is below 2^-29 for |r| <= 1/8), in 64 bits and rounded once, then by quarter.
   __device__ void at(int64_t position) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const double a = (double)position * freq[i];
-      const float t = (float)(a - __builtin_rint(a));
-      c[i] = __builtin_amdgcn_cosf(t);
-      s[i] = __builtin_amdgcn_sinf(t);
+      const double a = (double)position * freq[i], f = a - __builtin_rint(a);
+      const float quarter = __builtin_rintf(4.f * (float)f);
+      const int n = (int)quarter;
+      const double r = __builtin_fma((double)quarter, -0.25, f), z = r * r;
+      double x = __builtin_fma(z, 42.05869394489765, -76.70585975306136);
+      x = __builtin_fma(z, x, 81.60524927607504);
+      x = __builtin_fma(z, x, -41.341702240399755);
+      x = __builtin_fma(z, x, 6.283185307179586);
+      double y = __builtin_fma(z, -26.42625678337438, 60.24464137187666);
+      y = __builtin_fma(z, y, -85.45681720669373);
+      y = __builtin_fma(z, y, 64.93939402266829);
+      y = __builtin_fma(z, y, -19.739208802178716);
+      const float sine = (float)(r * x), cosine = (float)__builtin_fma(z, y, 1.);
+      const float u = n & 1 ? cosine : sine, v = n & 1 ? sine : cosine;
+      s[i] = n & 2 ? -u : u;
+      c[i] = (n + 1) & 2 ? -v : v;
     }
   }
 };
@@ -115,10 +135,10 @@ struct Weights {
   template <int D>
   __device__ void load(const float *weight, int sub) {
     norm = weight != nullptr;
-    const float4 one = make_float4(1.f, 1.f, 1.f, 1.f);
+    if (!norm) return;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const float4 v = norm ? *reinterpret_cast<const float4 *>(weight + 4 * sub + i * (D / 2)) : one;
+      const float4 v = *reinterpret_cast<const float4 *>(weight + 4 * sub + i * (D / 2));
       w[i][0] = v.x, w[i][1] = v.y, w[i][2] = v.z, w[i][3] = v.w;
     }
   }
@@ -164,12 +184,12 @@ __device__ __forceinline__ void rotate_part(const HeadArgs &a, uint32_t token, u
   int pass = (int)part * a.passes;
   const int end = min(all, pass + a.passes);
   if (pass >= end) return;
-  const X *const q = static_cast<const X *>(a.q.x) + token * a.q.token + 4 * sub;
-  const X *const k = kKeys ? static_cast<const X *>(a.k.x) + token * a.k.token + 4 * sub : nullptr;
+  const X *const q = static_cast<const X *>(a.q.x) + (uint64_t)token * a.q.token + 4 * sub;
+  const X *const k = kKeys ? static_cast<const X *>(a.k.x) + (uint64_t)token * a.k.token + 4 * sub : nullptr;
   Piece<X> next;
   auto load = [&](int p) {
-    if (!kKeys || p < q_passes) next.load(q + min(p * kHeads + in, a.q.heads - 1) * a.q.head, D / 2);
-    else next.load(k + min((p - q_passes) * kHeads + in, a.k.heads - 1) * a.k.head, D / 2);
+    if (!kKeys || p < q_passes) next.load(q + (uint64_t)min(p * kHeads + in, a.q.heads - 1) * a.q.head, D / 2);
+    else next.load(k + (uint64_t)min((p - q_passes) * kHeads + in, a.k.heads - 1) * a.k.head, D / 2);
   };
   load(pass);
   const int64_t position = a.positions[token];
@@ -198,13 +218,13 @@ __device__ __forceinline__ void rotate_part(const HeadArgs &a, uint32_t token, u
 
 template <int D, typename X>
 __global__ __launch_bounds__(256) void rotate_kernel(HeadArgs a) {
-  const uint32_t item = blockIdx.x * 4 + (threadIdx.x >> 6), token = item / (uint32_t)a.parts;
+  const uint32_t item = blockIdx.x * 4 + wave_index(), token = item / (uint32_t)a.parts;
   if (token < a.tokens) rotate_part<D, X, true>(a, token, item - token * (uint32_t)a.parts);
 }
 
 struct ValueRows {
   const void *x;
-  int64_t token, head;
+  uint32_t token, head;
 };
 
 // A group of 32 tokens has a workgroup for each of its k heads, then of its v heads, which
@@ -216,26 +236,26 @@ __global__ __launch_bounds__(2 * D) void append_rotated_kernel(CacheView c, Head
   __shared__ __attribute__((aligned(16))) __bf16 rows[kRows * kPitch];
   const uint32_t heads = (uint32_t)c.kv_heads, each = 2 * heads + rotators, group = blockIdx.x / each, in = blockIdx.x - group * each;
   if (in >= 2 * heads) {
-    const uint32_t item = (in - 2 * heads) * (D / 32) + (threadIdx.x >> 6), row = item / (uint32_t)a.parts, token = group * kRows + row;
+    const uint32_t item = (in - 2 * heads) * (D / 32) + wave_index(), row = item / (uint32_t)a.parts, token = group * kRows + row;
     if (token < a.tokens) rotate_part<D, X, false>(a, token, item - row * (uint32_t)a.parts);
     return;
   }
   const int64_t row0 = (int64_t)group * kRows;
-  const int last = (int)min(a.tokens - row0, (int64_t)kRows) - 1, b = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int last = (int)min(a.tokens - row0, (int64_t)kRows) - 1, b = (int)wave_index(), lane = threadIdx.x & 63;
   const int head = (int)(in >= heads ? in - heads : in);
   const Rows<T, D> to(c, head, row0, slots, a.tokens);
   if (in >= heads) {
-    append_values<T, D>(to, b, lane, static_cast<const X *>(v.x) + row0 * v.token + head * v.head, (int)v.token, last);
+    append_values<T, D>(to, b, lane, static_cast<const X *>(v.x) + row0 * v.token + (uint64_t)head * v.head, (int)v.token, last);
     return;
   }
   const int sub = threadIdx.x & (kLanes - 1), at = threadIdx.x / kLanes;  // 16 rows at a time
-  const X *const base = static_cast<const X *>(a.k.x) + row0 * a.k.token + head * a.k.head + 4 * sub;
+  const X *const base = static_cast<const X *>(a.k.x) + row0 * a.k.token + (uint64_t)head * a.k.head + 4 * sub;
   Piece<X> p[2];
   int64_t position[2];
 #pragma unroll
   for (int u = 0; u < 2; ++u) {
     const int row = min(16 * u + at, last);
-    p[u].load(base + row * a.k.token, D / 2);
+    p[u].load(base + (uint64_t)row * a.k.token, D / 2);
     position[u] = a.positions[row0 + row];
   }
   Turns t;
@@ -314,8 +334,8 @@ extern "C" int mq_rotate_heads(const void *q, int64_t q_token_stride, int64_t q_
   if (!aligned16(q) || !aligned16(k) || !aligned16(q_out) || !aligned16(k_out) || !aligned16(inv_freq) || !aligned16(q_weight) ||
       !aligned16(k_weight) || (reinterpret_cast<uintptr_t>(positions) & 7))
     return invalid("mq_rotate_heads: buffers must be 16-byte aligned");
-  HeadArgs a{{q, q_token_stride, q_head_stride, heads, q_weight, static_cast<__bf16 *>(q_out)},
-             {k, k_token_stride, k_head_stride, kv_heads, k_weight, static_cast<__bf16 *>(k_out)},
+  HeadArgs a{{q, (uint32_t)q_token_stride, (uint32_t)q_head_stride, heads, q_weight, static_cast<__bf16 *>(q_out)},
+             {k, (uint32_t)k_token_stride, (uint32_t)k_head_stride, kv_heads, k_weight, static_cast<__bf16 *>(k_out)},
              positions, inv_freq, eps, tokens, 0, 0};
   const int each = 64 / (head_dim / 8);
   const int64_t groups = (share(a, (heads + each - 1) / each + (kv_heads + each - 1) / each) + 3) / 4;
@@ -348,15 +368,15 @@ extern "C" int mq_kv_cache_append_rotated(const mq_kv_cache *c, const int64_t *s
   if (!aligned16(c->data) || !aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(q_out) || !aligned16(k_out) || !aligned16(inv_freq) ||
       !aligned16(q_weight) || !aligned16(k_weight) || ((reinterpret_cast<uintptr_t>(positions) | reinterpret_cast<uintptr_t>(slots)) & 7))
     return invalid("mq_kv_cache_append_rotated: buffers must be 16-byte aligned");
-  HeadArgs a{{q, q_token_stride, q_head_stride, heads, q_weight, static_cast<__bf16 *>(q_out)},
-             {k, k_token_stride, k_head_stride, c->kv_heads, k_weight, static_cast<__bf16 *>(k_out)},
+  HeadArgs a{{q, (uint32_t)q_token_stride, (uint32_t)q_head_stride, heads, q_weight, static_cast<__bf16 *>(q_out)},
+             {k, (uint32_t)k_token_stride, (uint32_t)k_head_stride, c->kv_heads, k_weight, static_cast<__bf16 *>(k_out)},
              positions, inv_freq, eps, tokens, 0, 0};
   const int each = 64 / (c->head_dim / 8);
   share(a, (heads + each - 1) / each);
   const int64_t rotators = (int64_t)kRows * a.parts / (c->head_dim / 32), groups = (tokens + kRows - 1) / kRows * (2 * c->kv_heads + rotators);
   if (!takes_grid(groups, 2 * c->head_dim)) return invalid("mq_kv_cache_append_rotated: too many tokens for the heads");
   const dim3 grid((unsigned)groups);
-  const ValueRows rows{v, v_token_stride, v_head_stride};
+  const ValueRows rows{v, (uint32_t)v_token_stride, (uint32_t)v_head_stride};
   with_cache_type(c, [&]<int T, int D>() {
     if (x_dtype == MQ_F32)
       hipLaunchKernelGGL((append_rotated_kernel<T, D, float>), grid, dim3(2 * D), 0, static_cast<hipStream_t>(stream), view(c), a, rows, slots,

@@ -4,8 +4,9 @@
 Bounds: a result is rounded once to bf16, at most 2^-8 of its value off.  Before that, in float32: the
 sum of D <= 128 squares, each product and sum off by 2^-24 of it, D 2^-24 = 2^-17 in all at most,
 half of that in the root; the root, two products, the rotation's two products and its sum, each at most 2^-23: 2^-20
-together; sine and cosine of an angle that is off by 2^-26 turns (6 * 2^-26) and v_sin_f32's and
-v_cos_f32's own errors, below 2^-20 over all of a turn.  2^-16 (|y_i| + |y_(i + D/2)|) holds them all."""
+together; sine and cosine of an angle that is off by 2^-24 turns at the farthest positions (2^28.4
+turns in 64 bits, whose product is rounded twice: 6.3 * 2^-24), rounded to f32 themselves, below 2^-20
+together.  2^-16 (|y_i| + |y_(i + D/2)|) holds them all."""
 import ctypes
 
 import pytest
