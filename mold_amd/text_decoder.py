@@ -58,6 +58,13 @@ def rms_norm(x, weight, eps: float):
     return x * torch.rsqrt(x.square().mean(-1, keepdim=True) + eps) * weight
 
 
+def rotate(x, cos, sin):
+    """Rotary embedding of the halves of each head: x [tokens, heads, dim], cos and sin [tokens, dim / 2]."""
+    a, b = x.float().chunk(2, -1)
+    c, s = cos[:, None], sin[:, None]
+    return torch.cat([a * c - b * s, b * c + a * s], -1)
+
+
 class TextDecoder:
     """weights: {GGUF name: QTensor (as Content.var_builder gives them all) or float32 tensor};
     `output.weight` falls back to the embedding, `attn_{q,k}_norm` and biases are optional.
@@ -77,7 +84,7 @@ class TextDecoder:
         self.table = self.lengths = self._buffers = None
         self._captured, self._retired = False, []     # what graphs of earlier batches hold
         half = config.head_dim // 2
-        self._states = BeamStates(self.caches)
+        self._states = None       # of the caches, once beams are reordered
         self._inv_freq = config.rope_theta ** (-torch.arange(half, device=device, dtype=torch.float32) / half)
 
     @staticmethod
@@ -100,7 +107,12 @@ class TextDecoder:
 
     def _norm(self, name: str):
         weight = self.weights.get(name)
-        return weight if weight is None else weight.reshape(-1)
+        return weight if weight is None else weight.reshape(-1).float()
+
+    def _beam_states(self):
+        if self._states is None:
+            self._states = BeamStates(self.caches)
+        return self._states
 
     def _forward(self, tokens, positions, slots, attention, keys: bool):
         """Hidden states of `tokens` [n] at `positions`, their keys and values written to `slots`;
@@ -138,6 +150,8 @@ class TextDecoder:
             raise ValueError("TextDecoder.prefill: at least one prompt, of at least one token each")
         if room < 0 or not 1 <= beams <= MQ_MAX_BEAMS:
             raise ValueError(f"TextDecoder.prefill: room for {room} tokens, {beams} beams")
+        if beams > 1:
+            self._beam_states()
         page = self.page_tokens
         per = -(-(max(lengths) + room) // page)
         shared = [n // page if beams > 1 else 0 for n in lengths]
@@ -155,7 +169,7 @@ class TextDecoder:
         x = self._forward(tokens, at.positions, at.slots, lambda layer, q, k, v: prompt_attention(q, k, v, plan), keys=True)
         logits = self._logits(x[at.last])
         if beams > 1:                # the partial page of each prompt, of which the first beam has the tokens
-            self._states.reorder(at.table, at.lengths, torch.zeros((len(lengths), beams), dtype=torch.int32, device=self.device))
+            self._beam_states().reorder(at.table, at.lengths, torch.zeros((len(lengths), beams), dtype=torch.int32, device=self.device))
         self._begin(at.table, at.lengths)
         return logits
 
@@ -223,8 +237,8 @@ class TextDecoder:
                 logits = self.step(last.reshape(-1)).view(n, beams, -1)
             ended = {} if stop is None or last is None else {"last": last, "stop": stop}
             scores, parents, last = select_beams(logits, scores, beams, **ended)
-            if at:
-                self._states.reorder(self.table, self.lengths, parents)
+            if at and beams > 1:
+                self._beam_states().reorder(self.table, self.lengths, parents)
             chosen.append((parents, last))
         if not chosen:
             return torch.empty((n, beams, 0), dtype=torch.int64, device=self.device), scores.expand(n, beams).contiguous()

@@ -6,12 +6,15 @@ weights and caches of the same values; what may differ is the order of sums in a
 rounding (2^-8) here and there of what goes into a layer's linears, far below the 2e-2 by which a step's
 logits are allowed to be off a float64 model (test_gpu_text_decoder), so 2e-2 of the logits' size a
 step is asserted.  A row with another row's cache is off by their whole size."""
+from dataclasses import replace
+
 import pytest
 
 torch = pytest.importorskip("torch")
 
 from mold_amd import GgmlDType
-from tests.test_gpu_text_decoder import PROMPTS, VOCAB, _decoder, model  # noqa: F401
+from mold_amd.text_decoder import TextDecoder
+from tests.test_gpu_text_decoder import CFG, PROMPTS, VOCAB, _decoder, model  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -121,3 +124,26 @@ def test_a_search_step_in_a_graph(model):  # noqa: F811
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(out, want))
+
+
+def test_head_norms_in_bf16(model):  # noqa: F811
+    """Weights that come in another type than the documented float32 are taken by their values."""
+    weights = {k: w.bfloat16() if k.endswith(("_q_norm.weight", "_k_norm.weight")) else w for k, w in model[0].items()}
+    same = {k: w.float() if k.endswith(("_q_norm.weight", "_k_norm.weight")) else w for k, w in weights.items()}
+    a, b = (_decoder((w, None), GgmlDType.BF16) for w in (weights, same))
+    assert torch.equal(a.prefill(PROMPTS, room=1), b.prefill(PROMPTS, room=1))
+    token = torch.arange(len(PROMPTS), device="cuda")
+    assert torch.equal(a.step(token), b.step(token))
+
+
+def test_more_layers_than_are_reordered_at_once(model):  # noqa: F811
+    """A decoder of 257 layers runs; beams of it are refused before anything ends."""
+    layers = 257
+    weights = {k: w for k, w in model[0].items() if not k.startswith("blk.")}
+    for i in range(layers):
+        weights.update({k.replace("blk.0.", f"blk.{i}."): w for k, w in model[0].items() if k.startswith("blk.0.")})
+    dec = TextDecoder(replace(CFG, layers=layers), weights, pages=8, page_tokens=32, cache_dtype=GgmlDType.BF16)
+    assert dec.prefill(PROMPTS[:2], room=4).shape == (2, VOCAB)
+    with pytest.raises(ValueError):
+        dec.beam_search(PROMPTS[:1], 2, 3)
+    assert torch.isfinite(dec.step(torch.tensor([1, 2], device="cuda"))).all()
