@@ -406,7 +406,7 @@ int mq_kv_cache_append_rotated(const mq_kv_cache *cache, const int64_t *slots, c
                                const int64_t *positions, const float *inv_freq, const float *q_weight, const float *k_weight,
                                float eps, void *q_out, void *k_out, void *stream);
 
-/* Pages for `sequences` (up to 65536) prompts of counts[i] tokens (int32, device memory; below
+/* Pages for `sequences` (up to 2^20) prompts of counts[i] tokens (int32, device memory; below
  * 0 counts as 0) with room for `room` more each, and where their tokens go.  With
  * beams > 1 a sequence has so many rows of the page table, which share the pages that
  * its tokens fill and have the others each to itself.  Pages are taken in the order of

@@ -196,7 +196,7 @@ int launch_place(const PlaceArgs &a, void *stream) {
 
 const char *place_fault(const mq_kv_cache *c, int64_t n, int64_t tokens, int64_t width, int64_t stride, int64_t rows) {
   if (const char *fault = cache_fault(c)) return fault;
-  if (n < 0 || n > 65536) return "placing tokens: 0 to 65536 sequences";
+  if (n < 0 || n > (int64_t(1) << 20)) return "placing tokens: 0 to 2^20 sequences";
   if (tokens < 0 || tokens >= (int64_t(1) << 31)) return "placing tokens: tokens outside 0 .. 2^31";
   if (width < 0 || width >= (int64_t(1) << 31) || stride < (rows > 1 ? width : 0) || stride >= (int64_t(1) << 40))
     return "placing tokens: a table's rows are apart, of 0 to 2^31 pages";

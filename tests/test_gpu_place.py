@@ -69,6 +69,21 @@ def test_prompts(beams, page):
 
 
 @gpu
+def test_more_sequences_than_16_bits():
+    rng = random.Random(3)
+    counts = [rng.choice([0, 1, 2, 33]) for _ in range(70001)]
+    c = torch.tensor(counts, dtype=torch.int32, device="cuda")
+    cache, tokens = _cache(150000), sum(counts) + 3
+    at = cache.place(c, tokens, 2)
+    _same(at, _place(counts, tokens, 2, 0, 1, range(150000), 32))
+    slots, positions, lengths = cache.extend(at.table, at.lengths)
+    table = at.table.tolist()
+    want = [t[n // 32] if n // 32 < 2 else -1 for t, n in zip(table, counts)]
+    assert slots.tolist() == [-1 if p < 0 else 32 * p + n % 32 for p, n in zip(want, counts)]
+    assert positions.tolist() == counts and lengths.tolist() == [n + 1 for n in counts]
+
+
+@gpu
 def test_what_does_not_fit():
     """Pages that run out or are not the cache's, a narrow table, rows cut off, counts that mean nothing."""
     page, counts = 32, [70, 0, -5, 33, 200, 1]
@@ -200,14 +215,14 @@ def test_refusals_of_the_library():
     lib, a, bad = _lib.load(), 4096, _lib.MQ_E_INVALID
     cache = _lib.KvCacheC(a, 4, 8, 2, 128, 64)
     place = dict(counts=a, n=3, beams=2, room=1, pages=a, page_count=4, table=a, stride=5, width=5, tokens=7, slots=a, positions=a, lengths=a, last=a, stream=None)
-    for change in (dict(counts=None), dict(n=-1), dict(n=65537), dict(beams=0), dict(beams=65), dict(room=-1), dict(room=1 << 31), dict(page_count=-1),
+    for change in (dict(counts=None), dict(n=-1), dict(n=(1 << 20) + 1), dict(beams=0), dict(beams=65), dict(room=-1), dict(room=1 << 31), dict(page_count=-1),
                    dict(page_count=1 << 31), dict(table=None), dict(stride=4), dict(stride=1 << 40), dict(width=-1), dict(width=1 << 31, stride=1 << 31), dict(tokens=-1), dict(tokens=1 << 31),
                    dict(slots=None), dict(positions=None), dict(lengths=None), dict(last=None), dict(slots=a + 4), dict(counts=a + 2), dict(table=a + 1),
                    dict(last=a + 4), dict(positions=a + 4), dict(lengths=a + 2), dict(pages=a + 2)):
         assert lib.mq_cache_place(ctypes.byref(cache), *{**place, **change}.values()) == bad, change
     assert lib.mq_cache_place(ctypes.byref(cache), *{**place, "n": 0, "tokens": 0}.values()) == 0
     extend = dict(held=a, counts=a, n=3, table=a, stride=5, width=5, tokens=7, slots=a, positions=a, lengths=a, stream=None)
-    for change in (dict(held=None), dict(n=-1), dict(n=65537), dict(table=None), dict(stride=4), dict(width=-1), dict(tokens=-1), dict(slots=None),
+    for change in (dict(held=None), dict(n=-1), dict(n=(1 << 20) + 1), dict(table=None), dict(stride=4), dict(width=-1), dict(tokens=-1), dict(slots=None),
                    dict(positions=None), dict(lengths=None), dict(held=a + 2), dict(counts=a + 1), dict(slots=a + 4)):
         assert lib.mq_cache_extend(ctypes.byref(cache), *{**extend, **change}.values()) == bad, change
     cache.page_tokens = 48
