@@ -14,10 +14,10 @@
 // request's logits are few, whole_kernel does all of it.
 //   Exponentials are f32 (v_exp_f32 of differences, whose error shrinks with the term's weight),
 // sums of 16 bytes of logits f32, of a lane and beyond f64.
-//   512 rows of 128000 in f32, a fifth of them of ended beams, 210 MB: 52 us and 5.6 of joining;
-// 80 rows of 151111 in bf16: 17 and 5.1, of which vector instructions (992 a wave, four waves a
-// SIMD) are 8; one request of 4 x 32000: 7.8 and 4.2, chains of dependent instructions behind one
-// load.
+//   512 rows of 128000 in f32, a fifth of them of ended beams, 210 MB: 49 us and 5.9 of joining;
+// 80 rows of 151111 in bf16: 14.4 and 4.8, of which reading alone takes 8.6, exponentials 0.9, the
+// bars 2, putting down and sorting 3; one request of 4 x 32000: 6.7 and 4.1, chains of dependent
+// instructions behind one load.
 //
 // mq_beam_reorder: beam j of a request goes on from beam parents[j].  Whole pages are shared: a
 // row of the page table takes its parent's entries.  The last, partial page goes to one child
@@ -101,6 +101,11 @@ template <int kWith, typename K>
 __device__ __forceinline__ K exchange(K v, bool high) {
   const K other = lane_xor<kWith>(v);
   return high == (v > other) ? v : other;
+}
+template <int kWith>
+__device__ __forceinline__ uint32_t exchange(uint32_t v, bool high) {
+  const uint32_t other = lane_xor<kWith>(v), most = max(v, other), least = min(v, other);
+  return high ? most : least;
 }
 // A bitonic sequence sorted over runs of 2 kWith lanes, the largest first where `down`.
 template <int kWith, typename K>
@@ -251,10 +256,11 @@ struct Scan {
     if (k > top.least) buffer[held + __builtin_amdgcn_mbcnt_hi((uint32_t)(in >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)in, 0))] = k;
     held += (int)__popcll(in);
   }
-  // The reference follows the largest of the lanes' logits; the sums so far with it.
+  // The reference follows the largest of the lanes' logits where that passes it by more than 1;
+  // the sums so far with it.
   __device__ __forceinline__ void follow(float most) {
+    if (!__any(most > ref + 1.f)) return;  // also where all are the lowest value, or NaN
     const float to = wave_max(most);
-    if (!(to > ref + 1.f)) return;  // also where `to` is the lowest value, and NaN
     sum *= (double)__builtin_amdgcn_exp2f((ref - to) * kLog2e);
     ref = to;
   }
@@ -262,11 +268,10 @@ struct Scan {
     least = top.least ? logit_of(top.least + 1) : -__FLT_MAX__;  // the least logit of a larger key
     enter = fminf(least, ref + 1.f);
   }
-  // The bar below which a logit need not enter: the count-th largest of the lanes' maxima so
-  // far, which as many logits reach.  In the order of ordered().
-  __device__ __forceinline__ uint32_t bar() const {
-    return __builtin_amdgcn_readlane((int)sorted(ordered(lane_most >= -__FLT_MAX__ ? lane_most : -__FLT_MAX__)), top.count - 1);
-  }
+  // The lanes' maxima so far in the order of ordered(), the largest in lane 0.
+  __device__ __forceinline__ uint32_t maxima() const { return sorted(ordered(lane_most >= -__FLT_MAX__ ? lane_most : -__FLT_MAX__)); }
+  // The bar below which a logit need not enter: the count-th of them, which as many logits reach.
+  __device__ __forceinline__ uint32_t bar(uint32_t of) const { return __builtin_amdgcn_readlane((int)of, top.count - 1); }
   __device__ __forceinline__ void raise(uint32_t to) {
     const uint64_t below = to > ordered(-__FLT_MAX__) ? ((uint64_t)to << 32) - 1 : 0;  // the key that all of it pass
     if (below > top.least) top.least = below;
@@ -354,8 +359,9 @@ struct Reader {
   __device__ __forceinline__ uint32_t first() {
     if (v >= to) return 0;
     unpack();
-    scan.follow(scan.lane_most);
-    return scan.bar();
+    const uint32_t maxima = scan.maxima();
+    scan.ref = logit_of((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)maxima) << 32);
+    return scan.bar(maxima);
   }
   // Everything, given that bar: what is large is in the buffer then, `held` keys.
   __device__ __forceinline__ Run read(uint32_t bar) {
@@ -369,7 +375,8 @@ struct Reader {
       v += 64 * U;
       if (v >= to) break;
       unpack();
-      if ((turn & (turn - 1)) == 0) scan.raise(scan.bar());  // at each doubling: what enters between two is about the same
+      // at each doubling: what enters between two is about the same; sooner the bar of all the waves serves
+      if (turn > 1 && (turn & (turn - 1)) == 0) scan.raise(scan.bar(scan.maxima()));
     }
     if (rest) {
       const int64_t at = tail * N + lane;
@@ -390,18 +397,13 @@ __device__ __forceinline__ Largest join(const uint64_t *buffers, int stride, con
   const int lane = threadIdx.x & 63;
   Largest top(count);
   const int mine = lane < waves ? (int)helds[lane] : 0;
-  int upto = mine;
-#pragma unroll
-  for (int off = 1; off < 16; off <<= 1) {
-    const int u = __shfl_up(upto, off);
-    if (lane >= off) upto += u;
-  }
-  const int start = upto - mine, total = __builtin_amdgcn_readlane(upto, 15);
+  int total = 0;
+  for (int i = 0; i < waves; ++i) total += __builtin_amdgcn_readlane(mine, i);
   for (int first = 0; first < total; first += 64) {
     const int at = first + lane;
-    int of = 0, from = 0;
+    int of = 0, from = 0, next = 0;
     for (int i = 1; i < waves; ++i) {
-      const int next = __builtin_amdgcn_readlane(start, i);
+      next += __builtin_amdgcn_readlane(mine, i - 1);
       if (at >= next) of = i, from = next;
     }
     top.offer(at < total ? buffers[of * stride + at - from] : 0);
@@ -748,20 +750,25 @@ __global__ __launch_bounds__(kCopyThreads) void copy_kernel(Plan plan, int reque
 int invalid(const char *msg) { return set_error(MQ_E_INVALID, msg); }
 bool aligned_to(const void *p, uintptr_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0; }
 
-// Runs of a row: workgroups for four on each of 256 CUs, none of fewer than 4096 logits (16 a
-// thread), 64 at most (a lane each when they are joined).  512 rows of 128000 in f32: 57 us,
-// 64 with 2048 workgroups, 76 with 512; 80 rows of 151111 in bf16: 22.5, 24 and 26.
+// Runs of a row: no more workgroups than four on each of 256 CUs, as many as can be there at once in
+// bf16 (registers); none of fewer than 4096 logits (16 a thread), 64 at most (a lane each when
+// they are joined).  In a graph, with joining: 80 rows of 151111 in bf16 18.3 us with 960 workgroups, 20.0
+// with 1040, whose last start when others end, 19.3 with 1600, 18.6 with 480; 512 rows of 128000
+// in f32 59.6 with 1024, 63.3 with 2048, 63.6 with 512.
 int splits_of(int64_t rows, int64_t vocab) {
-  const int64_t want = (1024 + rows - 1) / rows, most = vocab / 4096, s = want < most ? want : most;
+  const int64_t want = 1024 / rows, most = vocab / 4096, s = want < most ? want : most;
   return (int)(s < 1 ? 1 : s > 64 ? 64 : s);
 }
 
 // Whether a workgroup a request reads all its logits, which spares a launch and the scratch:
-// where they are 128 KB at most and neither waves nor CUs lack.  1 to 64 requests of 4 beams
-// over 1000 to 4000 tokens in f32 12 us against 16, over 8000 15 against 16, over 16000 20
-// against 16; 300 requests over 4000 23 against 17; 12 beams over 2000 23 against 16.
+// where a wave has 16 KB of them at most, or where the requests are as many as the CUs and no wave
+// is left over.  Against two launches, 4 beams in f32: 1 to 384 requests of 1000 to 4000 tokens
+// 12 to 15 us against 16, of 8000 12 to 20 against 16 to 21, one of 16000 17 against 16; 5000 of 1000
+// 58 against 84; 256 to 2048 of 32000 35 to 186 against 37 to 199.  With 5 beams, three of eight waves
+// idle, 256 of 32000 53 against 42.
 bool takes_whole(int64_t requests, int beams, int64_t vocab, int dtype) {
-  return beams <= kWholeWaves && requests <= 128 && vocab <= (128 << 10) / (beams * (dtype == MQ_F32 ? 4 : 2));
+  if (beams > kWholeWaves) return false;
+  return vocab * (dtype == MQ_F32 ? 4 : 2) <= (16 << 10) * (kWholeWaves / beams) || (requests >= 256 && kWholeWaves % beams == 0);
 }
 
 const char *select_fault(int64_t n, int beams, int64_t vocab, int count) {

@@ -86,6 +86,15 @@ def test_many_beams():
 
 @gpu
 @pytest.mark.parametrize("dtype", [torch.float32, BF], ids=["f32", "bf16"])
+@pytest.mark.parametrize("n,beams,count,vocab", [(255, 4, 3, 9001), (256, 4, 3, 9001), (301, 1, 2, 33333), (256, 2, 5, 20003), (260, 8, 1, 5003), (257, 5, 2, 7001)])
+def test_many_requests(n, beams, count, vocab, dtype):
+    """On both sides of where a workgroup reads a whole request."""
+    logits, scores = _logits(n, beams, vocab, dtype, seed=n)
+    _check(logits, scores, count)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, BF], ids=["f32", "bf16"])
 def test_ties(dtype):
     """Equal logits in any number and place: the lowest tokens, of equal beams the lowest beam."""
     for vocab in (5, 64, 300, 9000):
