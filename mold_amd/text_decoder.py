@@ -246,4 +246,4 @@ class TextDecoder:
         for parents, tokens in reversed(chosen):
             out.append(torch.gather(tokens, 1, row))
             row = torch.gather(parents.long(), 1, row)
-        return torch.stack(out[::-1], 2), scores
+        return torch.where((last < 0)[:, :, None], -1, torch.stack(out[::-1], 2)), scores     # a place left over has no parent
