@@ -234,7 +234,7 @@ class TextDecoder:
         scores = torch.zeros((n, 1), device=self.device)
         for at in range(count):
             if at:
-                logits = self.step(last.reshape(-1)).view(n, beams, -1)
+                logits = self.step(last.clamp(min=0).reshape(-1)).view(n, beams, -1)      # a place left over steps some token
             ended = {} if stop is None or last is None else {"last": last, "stop": stop}
             scores, parents, last = select_beams(logits, scores, beams, **ended)
             if at and beams > 1:

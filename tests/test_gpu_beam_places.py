@@ -50,3 +50,16 @@ def test_logits_that_are_no_numbers_end_every_hypothesis(model):  # noqa: F811
     dec.step = broken
     tokens, scores = dec.beam_search(PROMPTS, 2, 3)
     assert (tokens == -1).all() and (scores == -INF).all() and len(steps) == 2
+
+
+def test_steps_take_tokens_of_the_vocabulary(model):  # noqa: F811
+    """Also in the rows of places left over."""
+    dec = _small(model, 3)
+    step, taken = dec.step, []
+
+    def watched(tokens):
+        taken.append(tokens.clone())
+        return step(tokens)
+    dec.step = watched
+    dec.beam_search(PROMPTS, 12, 4)
+    assert len(taken) == 3 and all(((t >= 0) & (t < 3)).all() for t in taken)
