@@ -125,3 +125,5 @@ class BeamStates:
             self._streams.add(stream)
         _run_on(device, lib.mq_beam_reorder, self.c, len(self.caches), page_table.data_ptr(), page_table.stride(0), width,
                 lengths.data_ptr(), parents.data_ptr(), n, beams, scratch.data_ptr(), nbytes)
+        if not page_table.is_inference():      # which has no version
+            torch.autograd.graph.increment_version(page_table)      # written in place, as a copy_ tells autograd
