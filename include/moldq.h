@@ -432,9 +432,9 @@ int mq_cache_extend(const mq_kv_cache *cache, const int32_t *held, const int32_t
                     int64_t table_stride, int64_t max_pages, int64_t tokens, int64_t *slots, int64_t *positions, int32_t *lengths,
                     void *stream);
 
-/* The `count` best continuations of each request's beams (both up to MQ_MAX_BEAMS): of all
- * (beam, token) those with the largest scores[beam] + log softmax(logits of beam)[token],
- * in order.  Within a beam logits decide, then the lower token; between beams the totals in
+/* The `count` best continuations of each request's beams (both up to MQ_MAX_BEAMS; up to 2^20
+ * requests, fewer than 2^24 requests * beams): of all (beam, token) those with the largest
+ * scores[beam] + log softmax(logits of beam)[token], in order.  Within a beam logits decide, then the lower token; between beams the totals in
  * 64 bits, then the lower beam.  logits F32 or BF16, row of beam b of request n at n *
  * request_stride + b * beam_stride (elements, any alignment), unit stride inside; scores
  * f32 [requests, beams].  A beam whose last[n, b] (int64; NULL: no beam has) is `stop` has
@@ -442,14 +442,15 @@ int mq_cache_extend(const mq_kv_cache *cache, const int32_t *held, const int32_t
  * whose score is not finite, or among whose logits is a NaN or plus infinity, has none, nor
  * has a logit of minus infinity; places left over have score minus infinity, parent 0,
  * token -1.  out_scores f32, parents int32 and tokens int64 [requests, count]; scratch: at
- * least mq_beam_select_scratch_size bytes (device, 16-byte aligned, of this call alone).
+ * least mq_beam_select_scratch_size bytes (device, 16-byte aligned, of this call alone; 0 also
+ * for what the call refuses).
  * Asynchronous on stream. */
 int mq_beam_select(const void *logits, int dtype, int64_t requests, int beams, int64_t vocab, int64_t request_stride,
                    int64_t beam_stride, const float *scores, const int64_t *last, int64_t stop, int count, float *out_scores,
                    int32_t *parents, int64_t *tokens, void *scratch, size_t scratch_bytes, void *stream);
 size_t mq_beam_select_scratch_size(int64_t requests, int beams, int64_t vocab, int count, int dtype);
-/* Beam j of each request goes on from beam parents[n, j] (int32; itself if outside 0 ..
- * beams - 1), whose tokens so far become its own: in the page table (row n * beams + j,
+/* Beam j of each request (up to 2^20) goes on from beam parents[n, j] (int32; itself if outside
+ * 0 .. beams - 1), whose tokens so far become its own: in the page table (row n * beams + j,
  * changed in place) whole pages are shared, the last, partial page is passed on to one child
  * of each beam and copied, in each of the `count` caches (a model's layers, alike, up to 256), for
  * the others, into the pages of beams without a child.  lengths int32 [requests, beams]: the

@@ -31,7 +31,8 @@ def select_beams(logits, scores, count=None, last=None, stop=None):
     log_softmax(logits[beam])[token] first; ties go to the lower beam, within a beam to the lower
     token.  With `stop`, a beam whose `last` token (int64 [n, beams]) was `stop` has that one
     continuation, at its total as it is.  A beam of a score that is not finite or with a NaN or plus
-    infinity among its logits has none; places left over have total -inf, parent 0, token -1."""
+    infinity among its logits has none; places left over have total -inf, parent 0, token -1.  Up to
+    2^20 requests, fewer than 2^24 rows of logits."""
     if recorded(logits, scores):
         raise ValueError("select_beams: inference only, nothing may record the call")
     if logits.dim() != 3 or logits.dtype not in (torch.float32, torch.bfloat16) or logits.device.type != "cuda":
@@ -40,6 +41,8 @@ def select_beams(logits, scores, count=None, last=None, stop=None):
     device, count = logits.device, beams if count is None else int(count)
     if not 1 <= beams <= _lib.MQ_MAX_BEAMS or not 1 <= count <= _lib.MQ_MAX_BEAMS or vocab < 1:
         raise ValueError(f"select_beams: 1 to {_lib.MQ_MAX_BEAMS} beams and continuations, of at least one token; got {beams}, {count}, {vocab}")
+    if n > 1 << 20 or n * beams >= 1 << 24:
+        raise ValueError(f"select_beams: up to 2^20 requests, fewer than 2^24 rows of logits; got {n} of {beams} beams")
     if (last is None) != (stop is None):
         raise ValueError("select_beams: last and stop go together")
     if stop is not None and not 0 <= stop < vocab:

@@ -774,6 +774,8 @@ bool takes_whole(int64_t requests, int beams, int64_t vocab, int dtype) {
 const char *select_fault(int64_t n, int beams, int64_t vocab, int count) {
   if (n < 0 || n > (int64_t(1) << 20)) return "mq_beam_select: 0 to 2^20 requests";
   if (beams < 1 || beams > MQ_MAX_BEAMS || count < 1 || count > MQ_MAX_BEAMS) return "mq_beam_select: 1 to 64 beams and continuations";
+  // a launch's threads are counted in 32 bits, and where there are more than 1024 rows a workgroup of 256 takes one
+  if (n * beams >= (int64_t(1) << 24)) return "mq_beam_select: fewer than 2^24 rows of logits (requests * beams)";
   if (vocab < 1 || vocab >= (int64_t(1) << 31)) return "mq_beam_select: a vocabulary of 1 to 2^31 tokens";
   return nullptr;
 }
@@ -807,7 +809,6 @@ extern "C" int mq_beam_select(const void *logits, int dtype, int64_t requests, i
     return invalid("mq_beam_select: misaligned buffer");
   const int64_t rows = requests * beams;
   const int splits = need ? splits_of(rows, vocab) : 1;
-  if (rows * splits >= (int64_t(1) << 24) || requests >= (int64_t(1) << 22)) return invalid("mq_beam_select: too many requests");
   Run *const runs = static_cast<Run *>(scratch);
   const SelectArgs a{logits, request_stride, beam_stride, vocab, requests, scores, last, stop, beams, count, splits, runs,
                      reinterpret_cast<uint64_t *>(runs + rows * splits), out_scores, parents, tokens};
