@@ -391,15 +391,17 @@ size_t mq_cache_attention_scratch_size(const mq_kv_cache *cache, int64_t batch, 
  * bf16).  q, k: F32 or BF16, head h of token t at t *
  * token_stride + h * head_stride, unit stride inside a head, 16-byte aligned, strides
  * multiples of 16 bytes below 2^24 elements; positions int64 and inv_freq f32
- * [head_dim / 2] in device memory; head_dim 64 or 128.  q_out, k_out: bf16, contiguous,
- * 16-byte aligned, apart from the inputs.  Asynchronous on stream. */
+ * [head_dim / 2] in device memory; head_dim 64 or 128; up to 65536 heads of q and of k, up to
+ * 2^26 - 4 tokens.  q_out, k_out: bf16, contiguous, 16-byte aligned, apart from the inputs.
+ * Asynchronous on stream. */
 int mq_rotate_heads(const void *q, int64_t q_token_stride, int64_t q_head_stride, int heads, const void *k,
                     int64_t k_token_stride, int64_t k_head_stride, int kv_heads, int x_dtype, int head_dim, int64_t tokens,
                     const int64_t *positions, const float *inv_freq, const float *q_weight, const float *k_weight, float eps,
                     void *q_out, void *k_out, void *stream);
 /* mq_rotate_heads, and its k (as rounded to bf16) together with v written to the cache's
  * slots, as mq_kv_cache_append would write them.  k_out may be NULL where the rotated keys
- * are wanted in the cache only.  Asynchronous on stream. */
+ * are wanted in the cache only.  One launch, whose threads are counted in 32 bits: tokens, rounded
+ * up to 32, * (kv_heads + 512 / head_dim) below 2^35 / head_dim.  Asynchronous on stream. */
 int mq_kv_cache_append_rotated(const mq_kv_cache *cache, const int64_t *slots, const void *q, int64_t q_token_stride,
                                int64_t q_head_stride, int heads, const void *k, int64_t k_token_stride, int64_t k_head_stride,
                                const void *v, int64_t v_token_stride, int64_t v_head_stride, int x_dtype, int64_t tokens,

@@ -339,7 +339,8 @@ extern "C" int mq_rotate_heads(const void *q, int64_t q_token_stride, int64_t q_
              positions, inv_freq, eps, tokens, 0, 0};
   const int each = 64 / (head_dim / 8);
   const int64_t groups = (share(a, (heads + each - 1) / each + (kv_heads + each - 1) / each) + 3) / 4;
-  if (!takes_grid(groups, 256)) return invalid("mq_rotate_heads: too many tokens for the heads");
+  // of 8192 tokens and more a wave takes one whole, and a workgroup four
+  if (!takes_grid(groups, 256)) return invalid("mq_rotate_heads: up to 2^26 - 4 tokens");
   const dim3 grid((unsigned)groups);
   auto launch = [&]<int D>() {
     if (x_dtype == MQ_F32) hipLaunchKernelGGL((rotate_kernel<D, float>), grid, dim3(256), 0, static_cast<hipStream_t>(stream), a);
@@ -374,7 +375,7 @@ extern "C" int mq_kv_cache_append_rotated(const mq_kv_cache *c, const int64_t *s
   const int each = 64 / (c->head_dim / 8);
   share(a, (heads + each - 1) / each);
   const int64_t rotators = (int64_t)kRows * a.parts / (c->head_dim / 32), groups = (tokens + kRows - 1) / kRows * (2 * c->kv_heads + rotators);
-  if (!takes_grid(groups, 2 * c->head_dim)) return invalid("mq_kv_cache_append_rotated: too many tokens for the heads");
+  if (!takes_grid(groups, 2 * c->head_dim)) return invalid("mq_kv_cache_append_rotated: tokens * (kv_heads + 512 / head_dim) below 2^35 / head_dim");
   const dim3 grid((unsigned)groups);
   const ValueRows rows{v, (uint32_t)v_token_stride, (uint32_t)v_head_stride};
   with_cache_type(c, [&]<int T, int D>() {

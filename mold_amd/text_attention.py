@@ -126,7 +126,7 @@ def rotate_heads(q, k, positions, inv_freq, q_weight=None, k_weight=None, eps: f
     """Each head of q [tokens, heads, dim] and k [tokens, kv_heads, dim] (bf16 or f32, both the same;
     dim 64 or 128) RmsNormed with its weight (f32 [dim]; None: as it is) and its halves rotated by
     positions[t] * inv_freq[i] (int64 [tokens] of up to 2^31 either way, f32 [dim / 2]) -> (q, k) in
-    bf16."""
+    bf16.  Up to 2^26 - 4 tokens."""
     dtype, device = q.dtype, q.device
     if q.dim() != 3 or k.dim() != 3 or dtype is not _BF16 and dtype is not torch.float32 or device.type != "cuda":
         raise ValueError("rotate_heads: q and k must be bf16 or f32 [tokens, heads, dim] on a GPU")
@@ -331,7 +331,8 @@ class KvCache:
                        keys: bool = False):
         """rotate_heads of q and k (k and v [tokens, kv_heads, head_dim], all of one type), with the
         rotated keys and v appended to `slots` in the same pass -> (q, k) in bf16, k None unless
-        `keys` asks for it (a prompt's attention reads it, a step's reads the cache)."""
+        `keys` asks for it (a prompt's attention reads it, a step's reads the cache).  tokens * (kv_heads +
+        512 / head_dim) below 2^35 / head_dim."""
         name = "KvCache.append_rotated"
         device, dtype, dim = self.device, q.dtype, self.head_dim
         if q.dim() != 3 or q.shape[1] == 0 or dtype is not _BF16 and dtype is not torch.float32:
