@@ -105,9 +105,13 @@ class TextDecoder:
         y = x.float() @ w.t()
         return (y if bias is None else y + bias).to(out_dtype)
 
-    def _norm(self, name: str):
+    def _head_norm(self, name: str, x):
+        """x and the weight of the norm that goes with its rotation, f32 [head_dim]; a weight that varies over
+        the heads, or is one for the whole head, is applied to x here, which gives float32."""
         weight = self.weights.get(name)
-        return weight if weight is None else weight.reshape(-1).float()
+        if weight is None or weight.shape[-1:].numel() == weight.numel() == self.config.head_dim:
+            return x, weight if weight is None else weight.reshape(-1).float()
+        return rms_norm(x, weight, self.config.eps).float(), None
 
     def _beam_states(self):
         if self._states is None:
@@ -124,8 +128,9 @@ class TextDecoder:
             h = rms_norm(x, self.weights[f"{blk}.attn_norm.weight"], c.eps).bfloat16()
             q, k, v = (self._linear(f"{blk}.attn_{w}", h, torch.bfloat16).unflatten(-1, (n, c.head_dim))
                        for w, n in (("q", c.heads), ("k", c.kv_heads), ("v", c.kv_heads)))
-            q, k = self.caches[layer].append_rotated(q, k, v, slots, positions, self._inv_freq, self._norm(f"{blk}.attn_q_norm.weight"),
-                                                     self._norm(f"{blk}.attn_k_norm.weight"), c.eps, keys)
+            (q, qw), (k, kw) = self._head_norm(f"{blk}.attn_q_norm.weight", q), self._head_norm(f"{blk}.attn_k_norm.weight", k)
+            rows = (q, k, v) if q.dtype == k.dtype == v.dtype else (q.float(), k.float(), v.float())
+            q, k = self.caches[layer].append_rotated(*rows, slots, positions, self._inv_freq, qw, kw, c.eps, keys)
             a = attention(layer, q, k, v)
             x = x + self._linear(f"{blk}.attn_output", a.flatten(1))
             h = rms_norm(x, self.weights[f"{blk}.ffn_norm.weight"], c.eps).bfloat16()
