@@ -81,6 +81,8 @@ class TextDecoder:
         self.page_tokens, self.pages = page_tokens, pages
         self.caches = [KvCache(pages, config.kv_heads, config.head_dim, page_tokens, cache_dtype, device)
                        for _ in range(config.layers)]
+        # where tokens go is the same in every layer's, and without layers all the same
+        self._placing = self.caches[0] if self.caches else KvCache(pages, config.kv_heads, config.head_dim, page_tokens, cache_dtype, device)
         self.table = self.lengths = self._buffers = None
         self._captured, self._retired = False, []     # what graphs of earlier batches hold
         half = config.head_dim // 2
@@ -168,7 +170,7 @@ class TextDecoder:
         vocab = self.weights["token_embd.weight"].shape[0]
         if tokens.min() < 0 or tokens.max() >= vocab:
             raise ValueError(f"TextDecoder.prefill: a token outside 0 .. {vocab - 1}")
-        at = self.caches[0].place(torch.tensor(lengths, dtype=torch.int32).to(self.device), sum(lengths), per, room, beams)
+        at = self._placing.place(torch.tensor(lengths, dtype=torch.int32).to(self.device), sum(lengths), per, room, beams)
         tokens = tokens.to(self.device)
         self._end()
         x = self._forward(tokens, at.positions, at.slots, lambda layer, q, k, v: prompt_attention(q, k, v, plan), keys=True)
@@ -206,7 +208,7 @@ class TextDecoder:
             raise ValueError(f"TextDecoder.step: tokens must be int64 {list(self.lengths.shape)} on {self.lengths.device}")
         self._captured |= torch.cuda.is_current_stream_capturing()
         # past the table: written nowhere, and longer than its pages, which attention answers with NaN
-        slots, pos, lengths = self.caches[0].extend(self.table, self.lengths)
+        slots, pos, lengths = self._placing.extend(self.table, self.lengths)
         x = self._forward(tokens, pos, slots, lambda layer, q, k, v: self.caches[layer].attend(q, self.table, lengths), keys=False)
         logits = self._logits(x)
         self.lengths.copy_(lengths)      # last: a step that fails has not moved the sequences on
