@@ -421,15 +421,15 @@ int mq_kv_cache_append_rotated(const mq_kv_cache *cache, const int64_t *slots, c
  *                          last sequence have slot -1, position 0
  *   lengths                int32 [sequences * beams]
  *   last                   int64 [sequences]: the row of each one's last token, -1 if none
- * Asynchronous on stream; one launch, no scratch. */
+ * Asynchronous on stream; one launch, three for more than 4096 sequences, no scratch. */
 #define MQ_MAX_BEAMS 64
 int mq_cache_place(const mq_kv_cache *cache, const int32_t *counts, int64_t sequences, int beams, int64_t room, const int32_t *pages,
                    int64_t page_count, int32_t *table, int64_t table_stride, int64_t max_pages, int64_t tokens, int64_t *slots,
                    int64_t *positions, int32_t *lengths, int64_t *last, void *stream);
 /* Where counts[i] more tokens (NULL: one) of sequences that hold held[i] go over the pages
  * they have: slots and positions as above, -1 past the table or where it names no page of
- * the cache; lengths[i] = held[i] + counts[i], which may not be `held` itself.  Asynchronous
- * on stream; one launch, no scratch. */
+ * the cache; lengths[i] = held[i] + counts[i], which may not be `held` or `counts` itself.
+ * Asynchronous on stream; launches as above. */
 int mq_cache_extend(const mq_kv_cache *cache, const int32_t *held, const int32_t *counts, int64_t sequences, const int32_t *table,
                     int64_t table_stride, int64_t max_pages, int64_t tokens, int64_t *slots, int64_t *positions, int32_t *lengths,
                     void *stream);

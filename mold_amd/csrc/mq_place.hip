@@ -12,7 +12,8 @@
 // compute but two prefix sums over the sequences, so the launch is the cost, and there is
 // one: every workgroup takes the sums over all sequences itself (a window of 1024 at a
 // time, of which a batch has one), rather than wait for another launch or workgroup that
-// did.  A slot comes from the formula and not from the table, which is being written.
+// did.  Where that is many windows (summed), a launch before takes each one's sums, which wait in
+// entries of `lengths` that a launch after sets.  A slot comes from the formula and not from the table, which is being written.
 // 24 prompts (7305 tokens) take 6.0 us, 256 with four beams (163 000 tokens, 38 000 table
 // entries) 6.7, one token each of 200 sequences 3.5, of which a launch of nothing is 2.
 #include "../../include/moldq.h"
@@ -27,8 +28,11 @@ namespace {
 
 constexpr int kPlaceThreads = 256, kPer = 4, kWindow = kPlaceThreads * kPer;
 constexpr int kBlockTokens = 1024;  // tokens of a workgroup
-constexpr int kBlockRows = 4;       // sequences whose table rows workgroups share
-constexpr int kBlockEntries = 4096; // entries of these that one of them writes
+constexpr int kBlockEntries = 4096; // table entries of a workgroup
+// Windows of more than these are summed beforehand.  In a graph, prompts of 20 tokens: 2048 of them 8.4 us, 12.1
+// with the sums; 4096 14.0 and 14.2; 8192 29.8 and 18.4; 65536 233 and 25.  Sequences that go on, which need
+// the tokens' sums alone: 9.4 and 11.4, 14.6 and 12.3, 103 and 18.  A call for 2^20 prompts 43, 190 000.
+constexpr int kSummed = 4;
 constexpr uint32_t kMost = 0x7FFFFFFFu;
 
 struct PlaceArgs {
@@ -40,7 +44,8 @@ struct PlaceArgs {
   int32_t *lengths;
   uint32_t room, page;
   int beams;
-  uint32_t slices;  // workgroups for each kBlockRows sequences' rows
+  uint32_t per, slices;  // sequences whose table rows are shared by workgroups, and by how many
+  bool summed;
 };
 
 // Sums stop at kMost, so that counts that mean nothing cannot wrap them.
@@ -65,14 +70,15 @@ struct Need {
 struct Window {
   uint32_t tokens[kWindow + 1], pages[kWindow];
 };
-__device__ __forceinline__ void scan_window(const PlaceArgs &a, int64_t from, uint32_t &tokens, uint32_t &pages, Window &w, uint32_t (*sums)[2]) {
+template <typename F>  // of(i): tokens and pages of the window's i-th
+__device__ __forceinline__ void scan(const F &of, uint32_t &tokens, uint32_t &pages, Window &w, uint32_t (*sums)[2]) {
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
   uint32_t t[kPer], p[kPer], at = 0, ap = 0;
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
-    const Need need(a, from + tid * kPer + i);
+    const uint2 need = of(tid * kPer + i);
     t[i] = at, p[i] = ap;
-    at = add_capped(at, need.count), ap = add_capped(ap, need.pages);
+    at = add_capped(at, need.x), ap = add_capped(ap, need.y);
   }
   uint32_t st = at, sp = ap;  // over the lanes up to this one
 #pragma unroll
@@ -101,6 +107,53 @@ __device__ __forceinline__ void scan_window(const PlaceArgs &a, int64_t from, ui
   tokens = all_t, pages = all_p;
   __syncthreads();
 }
+__device__ __forceinline__ void scan_window(const PlaceArgs &a, int64_t from, uint32_t &tokens, uint32_t &pages, Window &w, uint32_t (*sums)[2]) {
+  scan([&](int i) {
+    const Need need(a, from + i);
+    return make_uint2(need.count, need.pages);
+  }, tokens, pages, w, sums);
+}
+// The last of the window's (below 1024) that starts at or before t and, if t is inside, holds it.
+__device__ __forceinline__ int holder(const Window &w, int64_t t) {
+  int at = 0;
+#pragma unroll
+  for (int step = kWindow / 2; step; step >>= 1)
+    if (w.tokens[at + step] <= t) at += step;
+  return at;
+}
+
+// Where a window's sums wait, of all windows but the last: the first two entries of its
+// sequences' lengths.
+__device__ __forceinline__ int64_t sums_at(const PlaceArgs &a, int64_t window) { return window * kWindow * a.beams; }
+__device__ __forceinline__ int64_t last_window(const PlaceArgs &a) { return (a.n - 1) / kWindow; }
+__device__ __forceinline__ int32_t length_of(const PlaceArgs &a, int64_t i, uint32_t count) {
+  return (int32_t)(a.held ? min((int64_t)a.held[i] + count, (int64_t)kMost) : count);
+}
+// A workgroup a window but the last.
+__global__ __launch_bounds__(kPlaceThreads) void sum_windows(PlaceArgs a) {
+  __shared__ uint32_t sums[kPlaceThreads / 64][2];
+  const int tid = threadIdx.x;
+  uint32_t t = 0, p = 0;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const Need need(a, (int64_t)blockIdx.x * kWindow + i * kPlaceThreads + tid);
+    t = add_capped(t, need.count), p = add_capped(p, need.pages);
+  }
+#pragma unroll
+  for (int off = 32; off; off >>= 1) t = add_capped(t, __shfl_xor(t, off)), p = add_capped(p, __shfl_xor(p, off));
+  if ((tid & 63) == 0) sums[tid >> 6][0] = t, sums[tid >> 6][1] = p;
+  __syncthreads();
+  if (tid >= 2) return;
+  uint32_t all = 0;
+#pragma unroll
+  for (int i = 0; i < kPlaceThreads / 64; ++i) all = add_capped(all, sums[i][tid]);
+  a.lengths[sums_at(a, blockIdx.x) + tid] = (int32_t)all;
+}
+// The lengths where the sums were.
+__global__ __launch_bounds__(kPlaceThreads) void put_lengths(PlaceArgs a) {
+  const int64_t e = (int64_t)blockIdx.x * kPlaceThreads + threadIdx.x, at = sums_at(a, e >> 1) + (e & 1), i = at / a.beams;
+  if (e >> 1 < last_window(a)) a.lengths[at] = length_of(a, i, Need(a, i).count);
+}
 
 // Page `at` of those to take, or -1.
 __device__ __forceinline__ int32_t page_at(const PlaceArgs &a, int64_t at) {
@@ -122,32 +175,45 @@ __device__ __forceinline__ void put_token(const PlaceArgs &a, int64_t t, int64_t
   a.slots[t] = page < 0 ? -1 : (int64_t)page * a.page + ((uint32_t)position - column * a.page);
 }
 
-// Workgroups 0 .. rows - 1 write table rows, every `slices` of them those of kBlockRows sequences, and the
+// Workgroups 0 .. rows - 1 write table rows, every `slices` of them those of `per` sequences, and the
 // first of these their lengths and last rows; the others write kBlockTokens tokens' slots and positions.
 __global__ __launch_bounds__(kPlaceThreads) void place_kernel(PlaceArgs a, uint32_t rows) {
   __shared__ Window w;
   __shared__ uint32_t sums[kPlaceThreads / 64][2];
   const int tid = threadIdx.x;
   uint32_t tokens = 0, pages = 0;
+  int64_t from = 0;
+  // the sums before the window in which to start, given as one that the windows' sums are known of
+  auto start = [&](auto window_of) {
+    if (!a.summed) return;
+    const int64_t last = last_window(a);
+    scan([&](int i) { return i < last ? make_uint2((uint32_t)a.lengths[sums_at(a, i)], (uint32_t)a.lengths[sums_at(a, i) + 1]) : make_uint2(0, 0); },
+         tokens, pages, w, sums);
+    const int window = (int)min(window_of(), last);
+    from = (int64_t)window * kWindow, tokens = w.tokens[window], pages = w.pages[window];
+  };
   if (blockIdx.x < rows) {
     const uint32_t group = blockIdx.x / a.slices, slice = blockIdx.x - group * a.slices;
-    const int64_t first = (int64_t)group * kBlockRows, end = min(a.n, first + kBlockRows);
-    int64_t from = 0;
-    if (!a.held)
-      for (;; from += kWindow) {  // kWindow is a multiple of kBlockRows: the sequences lie in one window
+    const int64_t first = (int64_t)group * a.per, end = min(a.n, first + a.per);
+    if (!a.held) {
+      start([&] { return first / kWindow; });
+      for (;; from += kWindow) {  // kWindow is a multiple of a.per: the sequences lie in one window
         scan_window(a, from, tokens, pages, w, sums);
         if (first < from + kWindow) break;
       }
-    if (slice == 0 && tid < end - first) {
-      const int64_t i = first + tid;
-      const Need need(a, i);
-      const int64_t length = a.held ? min((int64_t)a.held[i] + need.count, (int64_t)kMost) : need.count;
-      for (int j = 0; j < a.beams; ++j) a.lengths[i * a.beams + j] = (int32_t)length;
-      if (!a.held) {
-        const int64_t at = (int64_t)w.tokens[i - from] + need.count - 1;
-        a.last[i] = need.count == 0 || at >= a.tokens ? -1 : at;
-      }
     }
+    if (slice == 0)
+      for (int64_t i = first + tid; i < end; i += kPlaceThreads) {
+        const Need need(a, i);
+        const int32_t length = length_of(a, i, need.count);
+        const int64_t kept = a.summed && i / kWindow < last_window(a) ? sums_at(a, i / kWindow) + 2 : 0;  // before it sums wait
+        for (int j = 0; j < a.beams; ++j)
+          if (i * a.beams + j >= kept) a.lengths[i * a.beams + j] = length;
+        if (!a.held) {
+          const int64_t at = (int64_t)w.tokens[i - from] + need.count - 1;
+          a.last[i] = need.count == 0 || at >= a.tokens ? -1 : at;
+        }
+      }
     if (a.held || a.width == 0) return;
     const uint32_t width = (uint32_t)a.width, beams = (uint32_t)a.beams;
     const uint64_t entries = (uint64_t)(end - first) * beams * width;
@@ -170,15 +236,13 @@ __global__ __launch_bounds__(kPlaceThreads) void place_kernel(PlaceArgs a, uint3
     }
     return;
   }
-  for (int64_t from = 0; from < a.n; from += kWindow) {
+  start([&] { return (int64_t)holder(w, t0); });
+  for (; from < a.n; from += kWindow) {
     const uint32_t before = tokens;
     scan_window(a, from, tokens, pages, w, sums);
     const int64_t lo = max(t0, (int64_t)before), hi = min(t1, (int64_t)tokens);
     for (int64_t t = lo + tid; t < hi; t += kPlaceThreads) {
-      int at = 0;  // the last sequence of the window that starts at or before t and, as t < tokens, holds it
-#pragma unroll
-      for (int step = kWindow / 2; step; step >>= 1)
-        if (w.tokens[at + step] <= t) at += step;
+      const int at = holder(w, t);
       put_token(a, t, from + at, (uint32_t)(t - w.tokens[at]), w.pages[at]);
     }
     if (tokens >= t1) return;
@@ -192,12 +256,18 @@ bool aligned_to(const void *p, uintptr_t to) { return (reinterpret_cast<uintptr_
 // 4 prompts with 64 beams of 2004 pages, 513 000 table entries: a call of 13.7 us, 905 with one workgroup
 // for every four sequences' rows, however many entries these have.
 int launch_place(PlaceArgs a, void *stream) {
-  const int64_t groups = (a.n + kBlockRows - 1) / kBlockRows, entries = a.held ? 0 : min(a.n, (int64_t)kBlockRows) * a.beams * a.width;
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  for (a.per = 4; a.per < kWindow && a.n > (int64_t)a.per * 2048;) a.per *= 2;
+  const int64_t groups = (a.n + a.per - 1) / a.per, entries = a.held ? 0 : min(a.n, (int64_t)a.per) * a.beams * a.width;
   const int64_t slices = (entries + kBlockEntries - 1) / kBlockEntries, most = groups ? (int64_t(1) << 20) / groups : 1;  // a launch has so many workgroups at most
   a.slices = (uint32_t)(slices < 1 ? 1 : slices < most ? slices : most);
   const int64_t rows = groups * a.slices, blocks = rows + (a.tokens + kBlockTokens - 1) / kBlockTokens;
   if (blocks == 0) return MQ_OK;
-  hipLaunchKernelGGL(place_kernel, dim3((unsigned)blocks), dim3(kPlaceThreads), 0, static_cast<hipStream_t>(stream), a, (uint32_t)rows);
+  const int64_t windows = (a.n + kWindow - 1) / kWindow;
+  a.summed = a.counts && windows > kSummed;
+  if (a.summed) hipLaunchKernelGGL(sum_windows, dim3((unsigned)windows - 1), dim3(kPlaceThreads), 0, s, a);
+  hipLaunchKernelGGL(place_kernel, dim3((unsigned)blocks), dim3(kPlaceThreads), 0, s, a, (uint32_t)rows);
+  if (a.summed) hipLaunchKernelGGL(put_lengths, dim3((unsigned)((2 * (windows - 1) + kPlaceThreads - 1) / kPlaceThreads)), dim3(kPlaceThreads), 0, s, a);
   const hipError_t e = hipGetLastError();
   return e == hipSuccess ? MQ_OK : set_error(MQ_E_HIP, hipGetErrorString(e));
 }
@@ -228,7 +298,7 @@ extern "C" int mq_cache_place(const mq_kv_cache *c, const int32_t *counts, int64
       !aligned_to(positions, 8) || !aligned_to(last, 8))
     return invalid("mq_cache_place: misaligned buffer");
   return launch_place({counts, nullptr, pages, table, sequences, tokens, max_pages, table_stride, page_count, c->pages, slots,
-                       positions, last, lengths, (uint32_t)room, (uint32_t)c->page_tokens, beams, 1},
+                       positions, last, lengths, (uint32_t)room, (uint32_t)c->page_tokens, beams, 4, 1, false},
                       stream);
 }
 
@@ -243,6 +313,6 @@ extern "C" int mq_cache_extend(const mq_kv_cache *c, const int32_t *held, const 
       !aligned_to(positions, 8))
     return invalid("mq_cache_extend: misaligned buffer");
   return launch_place({counts, held, nullptr, const_cast<int32_t *>(table), sequences, tokens, max_pages, table_stride, 0, c->pages, slots,
-                       positions, nullptr, lengths, 0, (uint32_t)c->page_tokens, 1, 1},
+                       positions, nullptr, lengths, 0, (uint32_t)c->page_tokens, 1, 4, 1, false},
                       stream);
 }

@@ -353,7 +353,7 @@ class KvCache:
         return q_out, k_out
 
     def place(self, counts, tokens: int, width: int, room: int = 0, beams: int = 1, pages=None) -> "Placed":
-        """Pages for prompts of `counts` tokens (int32 [n], on the device) with room for `room` more
+        """Pages for up to 2^20 prompts of `counts` tokens (int32 [n], on the device) with room for `room` more
         each, and the slots of their packed `tokens` tokens (rows past the last prompt's have
         none).  A prompt has `beams` rows of the page table, of `width` pages, which share the
         pages that its tokens fill and have the others each to itself.  `pages` (int32, on the
@@ -377,7 +377,7 @@ class KvCache:
         return Placed(table, slots, positions, lengths, last)
 
     def extend(self, page_table, held, counts=None, tokens: Optional[int] = None):
-        """(slots, positions, lengths) of more tokens of the sequences that hold `held` (int32 [n])
+        """(slots, positions, lengths) of more tokens of the up to 2^20 sequences that hold `held` (int32 [n])
         over the pages page_table [n, pages] (int32): one each, or `counts` of them (int32 [n]),
         packed in `tokens` rows.  A token past the table, or on a page that is not the cache's,
         has slot -1; rows past the last sequence's have slot -1 and position 0."""
