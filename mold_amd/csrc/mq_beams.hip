@@ -622,9 +622,10 @@ struct ReorderArgs {
 
 constexpr int kPlanThreads = 256, kPlanColumns = 64;
 
-// A workgroup a request.  Lane j of its first wave is beam j.
+// Workgroups (request, y): the first of a request's plans, all take every gridDim.y-th part of its
+// columns of whole pages.  Lane j of a workgroup's first wave is beam j.
 __global__ __launch_bounds__(kPlanThreads) void plan_kernel(ReorderArgs a, CacheList caches, int count) {
-  if (blockIdx.x == 0 && (int)threadIdx.x < count) a.plan.caches->data[threadIdx.x] = caches.data[threadIdx.x];
+  if (blockIdx.x == 0 && blockIdx.y == 0 && (int)threadIdx.x < count) a.plan.caches->data[threadIdx.x] = caches.data[threadIdx.x];
   __shared__ int32_t entries[MQ_MAX_BEAMS * kPlanColumns];
   __shared__ int parent[MQ_MAX_BEAMS], taken[MQ_MAX_BEAMS], dead[MQ_MAX_BEAMS], moves;
   const int64_t row0 = (int64_t)blockIdx.x * a.beams;
@@ -655,7 +656,7 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(ReorderArgs a, Cache
   }
   __syncthreads();
   // the partial page: which each row has now, and what is copied into it
-  if (threadIdx.x < 64) {
+  if (blockIdx.y == 0 && threadIdx.x < 64) {
     const int j = threadIdx.x;
     bool copied = false;
     int from = 0, to = 0;
@@ -671,9 +672,9 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(ReorderArgs a, Cache
   }
   if (!moves) return;
   __syncthreads();
-  if (tail && full < a.width && threadIdx.x < a.beams) a.table[(row0 + threadIdx.x) * a.stride + full] = entries[threadIdx.x];
+  if (blockIdx.y == 0 && tail && full < a.width && threadIdx.x < a.beams) a.table[(row0 + threadIdx.x) * a.stride + full] = entries[threadIdx.x];
   const int64_t columns = min((int64_t)full, a.width);
-  for (int64_t c0 = 0; c0 < columns; c0 += kPlanColumns) {
+  for (int64_t c0 = (int64_t)blockIdx.y * kPlanColumns; c0 < columns; c0 += (int64_t)gridDim.y * kPlanColumns) {
     const int here = (int)min(columns - c0, (int64_t)kPlanColumns);
     __syncthreads();
     for (int i = threadIdx.x; i < a.beams * kPlanColumns; i += kPlanThreads) {
@@ -861,7 +862,11 @@ extern "C" int mq_beam_reorder(const mq_kv_cache *caches, int count, int32_t *ta
   const hipStream_t s = static_cast<hipStream_t>(stream);
   Copies *const of = reinterpret_cast<Copies *>(static_cast<CacheList *>(scratch) + 1);
   const Plan plan{static_cast<CacheList *>(scratch), of, reinterpret_cast<Copy *>(of + requests)};
-  hipLaunchKernelGGL(plan_kernel, dim3((unsigned)requests), dim3(kPlanThreads), 0, s,
+  // a workgroup for each kPlanColumns columns, while there are fewer than fill the chip.  4 requests of 64 beams
+  // over 31 250 whole pages: a call of 21 us, 3190 with a workgroup a request.
+  const int64_t parts = (max_pages + kPlanColumns - 1) / kPlanColumns, most_parts = 2048 / requests;
+  const unsigned part = (unsigned)(parts < most_parts ? (parts ? parts : 1) : most_parts ? most_parts : 1);
+  hipLaunchKernelGGL(plan_kernel, dim3((unsigned)requests, part), dim3(kPlanThreads), 0, s,
                      ReorderArgs{table, table_stride, max_pages, c.pages, lengths, parents, plan, beams, c.page_tokens}, list, count);
   for (int64_t first = 0; first < requests; first += kMaxRequests) {
     const int here = (int)(requests - first < kMaxRequests ? requests - first : kMaxRequests);
