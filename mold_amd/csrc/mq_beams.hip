@@ -621,6 +621,7 @@ struct ReorderArgs {
 };
 
 constexpr int kPlanThreads = 256, kPlanColumns = 64;
+static_assert(kPlanThreads >= kMaxCaches);  // a thread passes on each address
 
 // Workgroups (request, y): the first of a request's plans, all take every gridDim.y-th part of its
 // columns of whole pages.  Lane j of a workgroup's first wave is beam j.

@@ -13,6 +13,12 @@ from tests.test_gpu_place_sizes import _i32, _least
 pytestmark = pytest.mark.gpu
 
 
+def _tokens(cache, pages, tail):
+    """The bits of the first `tail` tokens of each of `pages`, as they are read."""
+    slots = (pages.reshape(-1, 1).long() * cache.page_tokens + torch.arange(tail)).reshape(-1)
+    return torch.stack(cache.read(slots.cuda())).view(torch.int16).cpu()
+
+
 @pytest.mark.parametrize("n,beams,full,tail", [(1, 2, 63, 1), (1, 5, 64, 0), (2, 64, 65, 31), (3, 3, 128, 32), (7, 4, 129, 5), (1, 64, 5000, 40), (30, 2, 700, 9), (2100, 2, 130, 3)])
 def test_long_tables(n, beams, full, tail):
     """Whole pages of any numbers, which the kernel only moves about; partial ones of the cache's."""
@@ -25,18 +31,18 @@ def test_long_tables(n, beams, full, tail):
     parents = torch.randint(-1, beams + 1, (n, beams), dtype=torch.int32, generator=g)
     parents[rng.randrange(n)] = torch.arange(beams)          # of one request every beam goes on as it is
     whose = torch.where((parents < 0) | (parents >= beams), torch.arange(beams), parents).long()
-    raw, length = _raw(cache), full * page + tail
+    length = full * page + tail
+    raw, held = _raw(cache), _tokens(cache, torch.gather(table, 1, whose[:, :, None].expand(n, beams, width))[:, :, full], tail)
     dev = table.view(n * beams, width).cuda()
     BeamStates([cache]).reorder(dev, _i32([length] * n * beams), parents.cuda())
-    got, now = dev.cpu().view(n, beams, width), _raw(cache)
+    got = dev.cpu().view(n, beams, width)
     want = torch.gather(table, 1, whose[:, :, None].expand(n, beams, width))
     assert torch.equal(got[:, :, :full], want[:, :, :full]) and torch.equal(got[:, :, full + 1], table[:, :, full + 1])
     if not tail:
-        assert torch.equal(got[:, :, full], table[:, :, full]) and torch.equal(raw, now)
+        assert torch.equal(got[:, :, full], table[:, :, full]) and torch.equal(_raw(cache), raw)
         return
     assert torch.equal(got[:, :, full].sort(1).values, table[:, :, full].sort(1).values)
-    tiles = -(-tail // 32)
-    assert torch.equal(now[got[:, :, full].long()][:, :, :, :tiles], raw[want[:, :, full].long()][:, :, :, :tiles])
+    assert torch.equal(_tokens(cache, got[:, :, full], tail), held)
 
 
 def test_its_time_is_that_of_the_table():
@@ -50,3 +56,18 @@ def test_its_time_is_that_of_the_table():
     rows = (torch.arange(n, device="cuda")[:, None] * beams + parents).view(-1)
     ours, plain = _least(lambda: states.reorder(table, lengths, parents)), _least(lambda: table.copy_(table[rows]))
     assert ours <= 8 * plain, (ours, plain)
+
+
+@pytest.mark.parametrize("caches", [255, 256])
+def test_as_many_caches_as_one_reordering_takes(caches):
+    """Each by itself: its copies are of its own bytes."""
+    page, length = 32, 21
+    alike = _states(caches, 8, 1, 64, page, GgmlDType.Q4_0)
+    pages = torch.tensor([2, 2, 4, 4])       # the parents'
+    held = [_tokens(c, pages, length) for c in alike]
+    table = torch.arange(8, dtype=torch.int32, device="cuda").view(4, 2)
+    BeamStates(alike).reorder(table, _i32([length] * 4), _i32([[1, 1], [0, 0]]))
+    assert table.tolist() == [[0, 1], [2, 3], [4, 5], [6, 7]]
+    assert all(torch.equal(_tokens(c, torch.tensor([0, 2, 4, 6]), length), h) for c, h in zip(alike, held))
+    with pytest.raises(ValueError, match="256"):
+        BeamStates(alike + _states(257 - caches, 8, 1, 64, page, GgmlDType.Q4_0))
