@@ -387,8 +387,8 @@ size_t mq_cache_attention_scratch_size(const mq_kv_cache *cache, int64_t batch, 
  * (f32 [head_dim]) is not NULL, x / sqrt(mean(x^2) + eps) * weight, and then its halves
  * rotated by the token's position: with a = positions[t] * inv_freq[i], value i becomes
  * x_i cos a - x_(i+D/2) sin a and value i + D/2 becomes x_(i+D/2) cos a + x_i sin a (f32;
- * angles in 64 bits, good to 2^-24 turns for positions of up to 2^31 either way; rounded once to
- * bf16).  q, k: F32 or BF16, head h of token t at t *
+ * angles in 64 bits, good to 2^-23 turns for positions of up to 2^31 either way and |inv_freq| of up
+ * to 1; rounded once to bf16).  q, k: F32 or BF16, head h of token t at t *
  * token_stride + h * head_stride, unit stride inside a head, 16-byte aligned, strides
  * multiples of 16 bytes below 2^24 elements; positions int64 and inv_freq f32
  * [head_dim / 2] in device memory; head_dim 64 or 128; up to 65536 heads of q and of k, up to
