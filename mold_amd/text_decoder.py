@@ -59,7 +59,8 @@ def rms_norm(x, weight, eps: float):
 
 
 def rotate(x, cos, sin):
-    """Rotary embedding of the halves of each head: x [tokens, heads, dim], cos and sin [tokens, dim / 2]."""
+    """Rotary embedding of the halves of each head: x [tokens, heads, dim], cos and sin [tokens, dim / 2] -> float32.
+    The plain form, for angles that a caller has; the decoder's own are taken by KvCache.append_rotated."""
     a, b = x.float().chunk(2, -1)
     c, s = cos[:, None], sin[:, None]
     return torch.cat([a * c - b * s, b * c + a * s], -1)
