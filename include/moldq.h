@@ -436,17 +436,19 @@ int mq_cache_extend(const mq_kv_cache *cache, const int32_t *held, const int32_t
 
 /* The `count` best continuations of each request's beams (both up to MQ_MAX_BEAMS; up to 2^20
  * requests, fewer than 2^24 requests * beams): of all (beam, token) those with the largest
- * scores[beam] + log softmax(logits of beam)[token], in order.  Within a beam logits decide, then the lower token; between beams the totals in
- * 64 bits, then the lower beam.  logits F32 or BF16, row of beam b of request n at n *
- * request_stride + b * beam_stride (elements, any alignment), unit stride inside; scores
- * f32 [requests, beams].  A beam whose last[n, b] (int64; NULL: no beam has) is `stop` has
- * ended: it has one continuation, `stop` at its score, whatever its logits are.  A beam
- * whose score is not finite, or among whose logits is a NaN or plus infinity, has none, nor
- * has a logit of minus infinity; places left over have score minus infinity, parent 0,
- * token -1.  out_scores f32, parents int32 and tokens int64 [requests, count]; scratch: at
- * least mq_beam_select_scratch_size bytes (device, 16-byte aligned, of this call alone; 0 also
- * for what the call refuses).
- * Asynchronous on stream. */
+ * scores[beam] + log softmax(logits of beam)[token], in order.  Within a beam logits decide, then
+ * the lower token; between beams the totals, compared in 64 bits, then the lower beam.  The
+ * exponentials in a total are f32, so that its logarithm is good to some 2^-22: totals of
+ * different beams that lie closer may come in either order, which can differ with the batch (how
+ * a row is shared by workgroups goes by its size); beams alike in score and logits tie.
+ * logits F32 or BF16, row of beam b of request n at n * request_stride + b * beam_stride
+ * (elements, any alignment), unit stride inside; scores f32 [requests, beams].  A beam whose
+ * last[n, b] (int64; NULL: no beam has) is `stop` has ended: it has one continuation, `stop` at
+ * its score, whatever its logits are.  A beam whose score is not finite, or among whose logits is
+ * a NaN or plus infinity, has none, nor has a logit of minus infinity; places left over have
+ * score minus infinity, parent 0, token -1.  out_scores f32, parents int32 and tokens int64
+ * [requests, count]; scratch: at least mq_beam_select_scratch_size bytes (device, 16-byte
+ * aligned, of this call alone; 0 also for what the call refuses).  Asynchronous on stream. */
 int mq_beam_select(const void *logits, int dtype, int64_t requests, int beams, int64_t vocab, int64_t request_stride,
                    int64_t beam_stride, const float *scores, const int64_t *last, int64_t stop, int count, float *out_scores,
                    int32_t *parents, int64_t *tokens, void *scratch, size_t scratch_bytes, void *stream);

@@ -11,9 +11,10 @@
 // which as many logits reach.  One comparison with the lower of the two finds what needs more
 // than its exponential.  merge_kernel joins a request's runs, takes the totals in 64 bits,
 // in which beams whose totals lie close compare as their logits say, and ranks them.  Where a
-// request's logits are few, whole_kernel does all of it.
+// request's logits are few, or the requests as many as the CUs, whole_kernel does all of it
+// (takes_whole).
 //   Exponentials are f32 (v_exp_f32 of differences, whose error shrinks with the term's weight),
-// sums of 16 bytes of logits f32, of a lane and beyond f64.
+// sums of 16 bytes of logits f32, of a lane and beyond f64: totals are good to some 2^-22.
 //   512 rows of 128000 in f32, a fifth of them of ended beams, 210 MB: 49 us and 5.9 of joining;
 // 80 rows of 151111 in bf16: 14.4 and 4.8, of which reading alone takes 8.6, exponentials 0.9, the
 // bars 2, putting down and sorting 3; one request of 4 x 32000: 6.7 and 4.1, chains of dependent
