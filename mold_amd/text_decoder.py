@@ -26,8 +26,9 @@ import torch
 from ._lib import MQ_MAX_BEAMS
 from .beams import BeamStates, select_beams
 from .quantized import GgmlDType, QMatMul, QTensor
-from .text_attention import KvCache, PromptPlan, prompt_attention
+from .text_attention import KvCache, Placed, PromptPlan, prompt_attention
 
+_MOST = 1 << 20      # sequences that place and extend take at once
 
 @dataclass(frozen=True)
 class TextConfig:
@@ -121,6 +122,25 @@ class TextDecoder:
             self._states = BeamStates(self.caches)
         return self._states
 
+    def _place(self, lengths, need, per, room, beams):
+        """Where prompts of these lengths go, which need so many pages each of the cache's."""
+        parts, page, row = [], 0, 0
+        for i in range(0, len(lengths), _MOST):
+            some, pages = lengths[i:i + _MOST], sum(need[i:i + _MOST])
+            order = torch.arange(page, page + pages, dtype=torch.int32, device=self.device) if page else None
+            at = self._placing.place(torch.tensor(some, dtype=torch.int32).to(self.device), sum(some), per, room, beams, order)
+            parts.append(at._replace(last=at.last + row) if row else at)
+            page, row = page + pages, row + sum(some)
+        return parts[0] if len(parts) == 1 else Placed(*(torch.cat(p) for p in zip(*parts)))
+
+    def _extend(self):
+        """Where one more token of each sequence goes."""
+        n = self.lengths.shape[0]
+        if n <= _MOST:
+            return self._placing.extend(self.table, self.lengths)
+        parts = [self._placing.extend(self.table[i:i + _MOST], self.lengths[i:i + _MOST]) for i in range(0, n, _MOST)]
+        return tuple(torch.cat(p) for p in zip(*parts))
+
     def _forward(self, tokens, positions, slots, attention, keys: bool):
         """Hidden states of `tokens` [n] at `positions`, their keys and values written to `slots`;
         attention(layer, q, k, v) -> [n, heads, dim], k only if it needs the `keys`."""
@@ -159,19 +179,21 @@ class TextDecoder:
         if room < 0 or not 1 <= beams <= MQ_MAX_BEAMS:
             raise ValueError(f"TextDecoder.prefill: room for {room} tokens, {beams} beams")
         if beams > 1:
+            if len(lengths) > _MOST:
+                raise ValueError(f"TextDecoder.prefill: beams of up to 2^20 prompts, not of {len(lengths)}")
             self._beam_states()
         page = self.page_tokens
         per = -(-(max(lengths) + room) // page)
         shared = [n // page if beams > 1 else 0 for n in lengths]
-        need = sum(s + beams * (-(-(n + room) // page) - s) for s, n in zip(shared, lengths))
-        if need > self.pages:
-            raise ValueError(f"TextDecoder.prefill: {need} pages needed, the cache has {self.pages}")
+        need = [s + beams * (-(-(n + room) // page) - s) for s, n in zip(shared, lengths)]
+        if sum(need) > self.pages:
+            raise ValueError(f"TextDecoder.prefill: {sum(need)} pages needed, the cache has {self.pages}")
         plan = PromptPlan(lengths, self.config.heads, self.config.kv_heads, self.config.head_dim, self.device)
         tokens = torch.tensor([t for p in prompts for t in p])
         vocab = self.weights["token_embd.weight"].shape[0]
         if tokens.min() < 0 or tokens.max() >= vocab:
             raise ValueError(f"TextDecoder.prefill: a token outside 0 .. {vocab - 1}")
-        at = self._placing.place(torch.tensor(lengths, dtype=torch.int32).to(self.device), sum(lengths), per, room, beams)
+        at = self._place(lengths, need, per, room, beams)
         tokens = tokens.to(self.device)
         self._end()
         x = self._forward(tokens, at.positions, at.slots, lambda layer, q, k, v: prompt_attention(q, k, v, plan), keys=True)
@@ -209,7 +231,7 @@ class TextDecoder:
             raise ValueError(f"TextDecoder.step: tokens must be int64 {list(self.lengths.shape)} on {self.lengths.device}")
         self._captured |= torch.cuda.is_current_stream_capturing()
         # past the table: written nowhere, and longer than its pages, which attention answers with NaN
-        slots, pos, lengths = self._placing.extend(self.table, self.lengths)
+        slots, pos, lengths = self._extend()
         x = self._forward(tokens, pos, slots, lambda layer, q, k, v: self.caches[layer].attend(q, self.table, lengths), keys=False)
         logits = self._logits(x)
         self.lengths.copy_(lengths)      # last: a step that fails has not moved the sequences on
