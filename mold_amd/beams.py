@@ -96,8 +96,8 @@ class BeamStates:
         self._streams = set()      # that all caches know to use them
 
     def reorder(self, page_table, lengths, parents):
-        """Beam j of each request goes on from beam parents[n, j] (int32 [n, beams]; itself if it is
-        no beam): its row of page_table (int32 [n * beams, pages], changed in place) and the tokens so
+        """Beam j of each of up to 2^20 requests goes on from beam parents[n, j] (int32 [n, beams]; itself if it
+        is no beam): its row of page_table (int32 [n * beams, pages], changed in place) and the tokens so
         far, lengths (int32 [n * beams], the same for a request's beams), become the parent's.
         Whole pages are shared; of the last, partial one, which no two rows may share before,
         each row has its own after it too, copied where a parent has several children."""
