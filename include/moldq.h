@@ -419,7 +419,7 @@ int mq_kv_cache_append_rotated(const mq_kv_cache *cache, const int64_t *slots, c
  *   slots, positions       int64 [tokens]: of the packed tokens, sequence by sequence, in
  *                          beam 0's pages (-1 where the table has none); rows past the
  *                          last sequence have slot -1, position 0
- *   lengths                int32 [sequences * beams]
+ *   lengths                int32 [sequences * beams], not `counts` itself
  *   last                   int64 [sequences]: the row of each one's last token, -1 if none
  * Asynchronous on stream; one launch, three for more than 4096 sequences, no scratch. */
 #define MQ_MAX_BEAMS 64

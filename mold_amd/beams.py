@@ -26,13 +26,14 @@ _MAX_STRIDE = 1 << 40
 
 def select_beams(logits, scores, count=None, last=None, stop=None):
     """The `count` (default: as many as beams) best continuations of each request: logits [n, beams,
-    vocab] (bf16 or f32) after its beams, scores f32 [n, beams] their totals so far ->
-    (totals f32, parents int32, tokens int64), each [n, count], the largest scores[beam] +
-    log_softmax(logits[beam])[token] first; ties go to the lower beam, within a beam to the lower
-    token (totals of different beams within some 2^-22 of each other may come in either order).  With `stop`, a beam whose `last` token (int64 [n, beams]) was `stop` has that one
-    continuation, at its total as it is.  A beam of a score that is not finite or with a NaN or plus
-    infinity among its logits has none; places left over have total -inf, parent 0, token -1.  Up to
-    2^20 requests, fewer than 2^24 rows of logits."""
+    vocab] (bf16 or f32) after its beams, scores f32 [n, beams] their totals so far -> (totals f32,
+    parents int32, tokens int64), each [n, count], the largest scores[beam] +
+    log_softmax(logits[beam])[token] first; ties go to the lower beam, within a beam to the lower token
+    (totals of different beams within some 2^-22 of each other may come in either order). With `stop`, a
+    beam whose `last` token (int64 [n, beams]) was `stop` has that one continuation, at its total as it
+    is. A beam of a score that is not finite or with a NaN or plus infinity among its logits has none;
+    places left over have total -inf, parent 0, token -1. Up to 2^20 requests, fewer than 2^24 rows of
+    logits."""
     if recorded(logits, scores):
         raise ValueError("select_beams: inference only, nothing may record the call")
     if logits.dim() != 3 or logits.dtype not in (torch.float32, torch.bfloat16) or logits.device.type != "cuda":

@@ -7,8 +7,9 @@
 //
 // in f32, rounded once to bf16.  The angle is taken in 64 bits as turns, of which the whole
 // ones are dropped, so that far positions keep their fraction (three roundings: within 2^-23 turns at
-// 2^31), and its sine and cosine are within 0.53 and 0.51 of f32's last place: with v_sin_f32 and v_cos_f32, 2^-22.9 off, 4100 tokens took
-// half a microsecond less, but half again as many results rounded to a neighbour of the right one.
+// 2^31), and its sine and cosine are within 0.53 and 0.51 of f32's last place: with v_sin_f32 and
+// v_cos_f32, 2^-22.9 off, 4100 tokens took half a microsecond less, but half again as many results
+// rounded to a neighbour of the right one.
 //
 // A value is read and written once; the bound is HBM, the launch for a step's few tokens.
 // D / 8 lanes hold a head, each four values of its lower half and the four that they are
@@ -105,7 +106,8 @@ struct Turns {
     for (int i = 0; i < 4; ++i) freq[i] = (double)v[i] * 0.15915494309189535;  // 1 / (2 pi)
   }
   // Of a = n / 4 + r turns, n the nearest whole number: sine and cosine of 2 pi r by their series
-  // (what is left out is below 2^-29 of the sine, 2^-32 of the cosine, for |r| <= 1/8), in 64 bits and rounded once, then by quarter.
+  // (what is left out is below 2^-29 of the sine, 2^-32 of the cosine, for |r| <= 1/8), in 64 bits
+  // and rounded once, then by quarter.
   __device__ void at(int64_t position) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
