@@ -60,7 +60,7 @@ def test_many_sequences(n, beams):
     """On both sides of where the sequences' sums are taken beforehand; windows of nothing but empty sequences."""
     rng = random.Random(n + beams)
     counts = [rng.choice([0, 0, 1, 2, 33]) for _ in range(n)]
-    counts[1024:3072] = [0] * 2048
+    counts[1000:3500] = [0] * 2500
     counts[-1] = 40
     page, room, width = 32, 3, 2
     need = sum((c // page if beams > 1 else 0) + beams * (-(-(c + room) // page) - (c // page if beams > 1 else 0)) for c in counts)
